@@ -5,7 +5,7 @@ Three kinds of case, each a dict of plain values; ``run`` takes one pass through
 * ``append``: the keys and values of a step's tokens go into an 8-bit paged cache, rotated by their positions on the way.
   A block is the ``page`` tokens of one page and one kv head; its scale is a power of two, held as a float. With ``n0`` the
   slots of the page that were held before the step and ``a`` the largest magnitude among the step's elements in the block:
-  ``e`` is the least integer, not below -100 and at most 121, with ``a <= 127 * 2^e``; the new scale is ``2^e`` where the
+  ``e`` is the least integer, not below -80 and at most 121, with ``a <= 127 * 2^e``; the new scale is ``2^e`` where the
   page is fresh (``n0`` = 0, or scale 0) and else the larger one of the old scale and ``2^e``; codes held before become
   ``rint(code * old / new)``, new ones are ``rint(x / new)`` within -127..127. Back come the rotated queries, the scales and
   the values that the pools' codes stand for.
@@ -169,10 +169,10 @@ def _pow2(e):
 
 
 def _pow2_at_least(largest):
-    """2^e with the least integer e, -100 <= e <= 121, so that largest <= 127 * 2^e (64-bit in, 64-bit out)."""
+    """2^e with the least integer e, -80 <= e <= 121, so that largest <= 127 * 2^e (64-bit in, 64-bit out)."""
     _, e = torch.frexp(largest / 127.0)                 # largest / 127 = f * 2^e, 1/2 <= f < 1
     e = torch.where(largest > 127.0 * _pow2(e - 1), e, e - 1)            # (the quotient is 1/2 or rounded up to it)
-    return _pow2(torch.where(largest > 0, e, -100).clamp(-100, 121))
+    return _pow2(torch.where(largest > 0, e, -80).clamp(-80, 121))
 
 
 def _quantize_pages(x):
@@ -414,7 +414,7 @@ def _exact_append(s):
                 b = table[i][at // page]
                 mine = rows[s["starts"][i] + at - p:s["starts"][i] + at - p + end - begin].permute(1, 0, 2)      # [kv, slots, d]
                 top = mine.abs().amax(dim=(1, 2))
-                step = torch.tensor([next((2.0 ** e for e in range(-100, 121) if a <= 127.0 * 2.0 ** e), 2.0 ** 121) for a in top.tolist()],
+                step = torch.tensor([next((2.0 ** e for e in range(-80, 121) if a <= 127.0 * 2.0 ** e), 2.0 ** 121) for a in top.tolist()],
                                     dtype=torch.float64, device="cuda")
                 before = final[b]
                 if begin > 0:
