@@ -1,0 +1,403 @@
+// The 8-bit cache of keys and values: appending a step's tokens with the position rotation on the way, and reading pages
+// back as 16- or 32-bit numbers.
+//
+// A block is the page_size tokens of one page and one kv head; it has one scale for its keys and one for its values, powers
+// of two held as floats, and a value is code * scale with a signed 8-bit code. code * 2^e is exact in bfloat16 (8 significant
+// bits) and in 32 bits, so every reader sees the same numbers. For the tokens that a step adds to a block, of which n0 were
+// held before:
+//     a  = max |x|                      over the step's elements in the block (keys after the rotation)
+//     s' = 2^e, e least in -80..121 with a <= 127 * 2^e;  max(s, s') where n0 > 0 and the block has a scale s already
+//     code = rint(x / s')               new elements, within -127..127
+//     code = rint(code * s / s')        elements held before (only where the scale grew)
+// A scale grows by factors of two, so the roundings of one element add up to less than s'/2 (1 + 1/2 + 1/4 + ...) = s'; with
+// scales of any value every growth could add another half step. An element that is not finite makes the block's scale NaN:
+// whoever reads the block sees that it is undefined. Slots behind the last token keep their codes.
+//
+// The rotated key is formed in 64 bits (bfloat16 or float times float is exact there): a code is a rounding to whole steps,
+// and a key that lies between two must not change its side with the order of the products.
+#include "common.cuh"
+
+namespace {
+
+constexpr int E_MIN = -80, E_MAX = 121;
+
+// 2^e with the least e in E_MIN..E_MAX that has a <= 127 * 2^e; NaN unless a is finite.
+__device__ __forceinline__ float block_scale(float a) {
+    const unsigned bits = __float_as_uint(a);
+    if ((bits & 0x7f800000u) == 0x7f800000u) return __uint_as_float(0x7fc00000u);
+    // a = 1.f * 2^x: 127 * 2^(x - 6) = 1.984375 * 2^x is enough unless a's fraction is above 0.984375 = 126/128
+    int e = (int)(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    e = max(E_MIN, min(E_MAX, e));
+    return __uint_as_float((unsigned)(e + 127) << 23);
+}
+
+// Where a unit of work lies: the tokens of one request in one page. Units are counted request by request; request r has at
+// most (q_len + page_size - 2) / page_size + 1 of them, whatever its position.
+struct Unit { int row, count, slot; long long page; };
+
+__device__ __forceinline__ Unit find_unit(int u, const int* __restrict__ q_start, const int* __restrict__ ctx_lens, int n_req,
+                                          const int* __restrict__ block_table, int bt_stride, int bt_width, int page_size, int num_pages, int lane) {
+    Unit out{0, 0, 0, -1};
+    int base = 0;
+    for (int r0 = 0; r0 < n_req; r0 += 32) {
+        const int r = r0 + lane;
+        int begin = 0, n = 0;
+        if (r < n_req) { begin = __ldg(q_start + r); n = __ldg(q_start + r + 1) - begin; }
+        int units = n > 0 ? (n + page_size - 2) / page_size + 1 : 0, sum = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const unsigned mine = __ballot_sync(0xffffffffu, u < base + sum);
+        if (mine) {
+            const int src = __ffs(mine) - 1;
+            const int before = base + __shfl_sync(0xffffffffu, sum - units, src);
+            const int row = __shfl_sync(0xffffffffu, begin, src), q_len = __shfl_sync(0xffffffffu, n, src);
+            const int first = __ldg(ctx_lens + r0 + src) - q_len;            // position of the request's first token of the step
+            if (first < 0) return out;                                      // a padding row
+            const int lp = first / page_size + (u - before);
+            const int lo = max(first, lp * page_size), hi = min(first + q_len, (lp + 1) * page_size);
+            if (hi <= lo || lp >= bt_width) return out;
+            const int page = __ldg(block_table + (size_t)(r0 + src) * bt_stride + lp);
+            out.row = row + (lo - first);
+            out.count = hi - lo;
+            out.slot = lo - lp * page_size;
+            out.page = page >= 0 && page < num_pages ? page : -1;
+            return out;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return out;
+}
+
+template <typename T, int V> struct Vec;
+template <> struct Vec<__nv_bfloat16, 4> {
+    static __device__ __forceinline__ void load(float (&f)[4], const __nv_bfloat16* p) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
+        f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
+};
+template <> struct Vec<float, 4> {
+    static __device__ __forceinline__ void load(float (&f)[4], const float* p) { *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(p); }
+};
+template <typename T> struct Vec<T, 1> {
+    static __device__ __forceinline__ void load(float (&f)[1], const T* p) { f[0] = Elem<T>::load(p); }
+};
+
+template <int V> __device__ __forceinline__ void store_codes(signed char* p, const int (&c)[V]) {
+    if (V == 4) {
+        *reinterpret_cast<unsigned*>(p) = (unsigned)(c[0] & 0xff) | ((unsigned)(c[V > 1 ? 1 : 0] & 0xff) << 8) |
+                                          ((unsigned)(c[V > 2 ? 2 : 0] & 0xff) << 16) | ((unsigned)(c[V > 3 ? 3 : 0] & 0xff) << 24);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = (signed char)c[i];
+    }
+}
+
+// rint(x / s) within -127..127; inv = 1 / s exactly. Of a NaN: 0 (its block's scale says so).
+__device__ __forceinline__ int code_of(double x, double inv) {
+    const double y = fmin(fmax(x * inv, -127.0), 127.0);
+    return y == y ? __double2int_rn(y) : 0;
+}
+
+constexpr int KV_WARPS = 4;
+constexpr int Q_THREADS = KV_WARPS * 32;
+
+struct AppendArgs {
+    const int* positions; const int* q_start; const int* ctx_lens; const float* cos_t; const float* sin_t;
+    const int* block_table; signed char* k_pages; signed char* v_pages; float* k_scales; float* v_scales;
+    int table_rows, rot, bt_stride, bt_width, page_size, num_pages, m, n_req, heads, kv_heads, head_dim, q_stride, out_stride;
+    int units, kv_blocks;       // the first kv_blocks CTAs append, a warp for each (unit, kv head, keys or values); the others rotate queries
+};
+
+// V: elements of a chunk (4, or 1 where widths or addresses do not allow it).
+template <typename T, int V>
+__global__ void __launch_bounds__(Q_THREADS)
+append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_out may be qkv)
+    const int half = a.rot >> 1, hd = a.head_dim, lane = threadIdx.x & 31;
+    // This kernel lets the one behind it in only after its own wait: whatever starts early behind it then knows that everything
+    // before it in the stream is complete (the attention reads the pages of earlier steps on that ground).
+    pdl_wait();
+    pdl_launch_dependents();
+    if ((int)blockIdx.x >= a.kv_blocks) {
+        // ---- queries: an item is a chunk of pairs (or a chunk beyond the rotated width) of one head of one token
+        const int per_head = half / V + (hd - a.rot) / V;
+        const long long items = (long long)a.m * a.heads * per_head;
+        const long long i = (long long)(blockIdx.x - a.kv_blocks) * Q_THREADS + threadIdx.x;
+        if (i >= items) return;
+        const int c = (int)(i % per_head);
+        const long long th = i / per_head;
+        const int head = (int)(th % a.heads), tok = (int)(th / a.heads);
+        const T* p = qkv + (size_t)tok * a.q_stride + (size_t)head * hd;
+        T* o = q_out + (size_t)tok * a.out_stride + (size_t)head * hd;
+        float x1[V], x2[V];
+        if (c < half / V) {
+            const int d = c * V, pos = a.positions[tok];
+            Vec<T, V>::load(x1, p + d);
+            Vec<T, V>::load(x2, p + d + half);
+            const bool known = pos >= 0 && pos < a.table_rows;
+            float cs[V], sn[V];
+            const size_t at = (size_t)(known ? pos : 0) * half + d;
+            Vec<float, V>::load(cs, a.cos_t + at);
+            Vec<float, V>::load(sn, a.sin_t + at);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                Elem<T>::store(o + d + j, known ? x1[j] * cs[j] - x2[j] * sn[j] : NAN);
+                Elem<T>::store(o + d + half + j, known ? x2[j] * cs[j] + x1[j] * sn[j] : NAN);
+            }
+        } else {
+            const int d = a.rot + (c - half / V) * V;
+            Vec<T, V>::load(x1, p + d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) Elem<T>::store(o + d + j, x1[j]);
+        }
+        return;
+    }
+    // ---- keys and values
+    const int job = blockIdx.x * KV_WARPS + (threadIdx.x >> 5);
+    const int per_unit = 2 * a.kv_heads;
+    if (job >= a.units * per_unit) return;
+    const int u = job / per_unit, kvh = (job - u * per_unit) >> 1, values = job & 1;
+    const Unit unit = find_unit(u, a.q_start, a.ctx_lens, a.n_req, a.block_table, a.bt_stride, a.bt_width, a.page_size, a.num_pages, lane);
+    if (unit.page < 0) return;
+    const size_t block = (size_t)unit.page * a.kv_heads + kvh;
+    signed char* codes = (values ? a.v_pages : a.k_pages) + block * a.page_size * hd;
+    float* scale_at = (values ? a.v_scales : a.k_scales) + block;
+    const T* rows = qkv + (size_t)unit.row * a.q_stride + (size_t)(a.heads + (values ? a.kv_heads : 0) + kvh) * hd;
+    const float old = unit.slot > 0 ? *scale_at : 0.f;
+    const int rot = values ? 0 : a.rot, pairs = (rot >> 1) / V, per_token = pairs + (hd - rot) / V;
+    const int items = unit.count * per_token;
+
+    // the two chunks of an item (the second only of a rotated pair), in 64 bits
+    auto item = [&](int i, int& tok, int& d, bool& pair, double (&y1)[V], double (&y2)[V]) {
+        tok = i / per_token;
+        const int c = i - tok * per_token;
+        pair = c < pairs;
+        d = pair ? c * V : rot + (c - pairs) * V;
+        const T* p = rows + (size_t)tok * a.q_stride;
+        float x1[V], x2[V];
+        Vec<T, V>::load(x1, p + d);
+        if (pair) {
+            Vec<T, V>::load(x2, p + d + half);
+            const int pos = a.positions[unit.row + tok];
+            const bool known = pos >= 0 && pos < a.table_rows;
+            float cs[V], sn[V];
+            const size_t at = (size_t)(known ? pos : 0) * half + d;
+            Vec<float, V>::load(cs, a.cos_t + at);
+            Vec<float, V>::load(sn, a.sin_t + at);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const double c64 = known ? (double)cs[j] : (double)NAN, s64 = sn[j];
+                y1[j] = (double)x1[j] * c64 - (double)x2[j] * s64;
+                y2[j] = (double)x2[j] * c64 + (double)x1[j] * s64;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) y1[j] = y2[j] = (double)x1[j];
+        }
+    };
+    // the largest magnitude, rounded up to 32 bits (127 * 2^e is one of those numbers, so the comparison with it stays what it
+    // is); as an integer, in whose order a NaN's bits are above everything
+    unsigned top = 0;
+    for (int i = lane; i < items; i += 32) {
+        int tok, d;
+        bool pair;
+        double y1[V], y2[V];
+        item(i, tok, d, pair, y1, y2);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            top = max(top, __float_as_uint(__double2float_ru(fabs(y1[j]))) & 0x7fffffffu);
+            top = max(top, __float_as_uint(__double2float_ru(fabs(y2[j]))) & 0x7fffffffu);
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    float scale = block_scale(__uint_as_float(top));
+    if (unit.slot > 0) {
+        const bool undefined = scale != scale || old != old;
+        scale = undefined ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale);
+        if (scale > old) {          // (not where it is undefined)
+            const float by = old / scale;       // a power of two, or 0 where the block had no scale yet
+            for (int i = lane; i < unit.slot * hd; i += 32) codes[i] = (signed char)__float2int_rn((float)codes[i] * by);
+        }
+    }
+    const double inv = 1.0 / (double)scale;
+    for (int i = lane; i < items; i += 32) {
+        int tok, d, c[V];
+        bool pair;
+        double y1[V], y2[V];
+        item(i, tok, d, pair, y1, y2);
+        signed char* dst = codes + (size_t)(unit.slot + tok) * hd + d;
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] = code_of(y1[j], inv);
+        store_codes<V>(dst, c);
+        if (pair) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[j] = code_of(y2[j], inv);
+            store_codes<V>(dst + half, c);
+        }
+    }
+    if (lane == 0) *scale_at = scale;
+}
+
+// ------------------------------------------------------------------------------------------ reading pages back
+template <typename T> __device__ __forceinline__ void store16(T* out, const uint4& codes, float scale);
+template <> __device__ __forceinline__ void store16<float>(float* out, const uint4& u, float scale) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float4 f;
+        f.x = (float)(signed char)(w[i]) * scale; f.y = (float)(signed char)(w[i] >> 8) * scale;
+        f.z = (float)(signed char)(w[i] >> 16) * scale; f.w = (float)(signed char)(w[i] >> 24) * scale;
+        reinterpret_cast<float4*>(out)[i] = f;
+    }
+}
+template <> __device__ __forceinline__ void store16<__nv_bfloat16>(__nv_bfloat16* out, const uint4& u, float scale) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+    unsigned r[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __nv_bfloat162 a = __floats2bfloat162_rn((float)(signed char)(w[i]) * scale, (float)(signed char)(w[i] >> 8) * scale);
+        __nv_bfloat162 b = __floats2bfloat162_rn((float)(signed char)(w[i] >> 16) * scale, (float)(signed char)(w[i] >> 24) * scale);
+        r[2 * i] = *reinterpret_cast<unsigned*>(&a);
+        r[2 * i + 1] = *reinterpret_cast<unsigned*>(&b);
+    }
+    reinterpret_cast<uint4*>(out)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    reinterpret_cast<uint4*>(out)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+// out = codes * scale, block by block. Wide: the block's bytes are a multiple of 16.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256)
+unpack_int8_kernel(const signed char* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, long long items, int per_block) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= items) return;
+    const float s = __ldg(scales + i / per_block);
+    if (WIDE) {
+        store16<T>(out + i * 16, reinterpret_cast<const uint4*>(codes)[i], s);
+    } else {
+        Elem<T>::store(out + i, (float)codes[i] * s);
+    }
+}
+
+// A step's requests as pages of GATHER tokens in the order of their positions: page r * width + i of the result holds
+// positions i * GATHER .. of request r; the table says so (-1 where a request has no such page). Positions before ``lo`` of a
+// window are not read by any of the request's tokens and stay unwritten where a whole result page lies before it. A block with
+// an undefined scale becomes undefined keys and values of zero: a score is left out by choosing, not by multiplying with nothing,
+// so that a token that does not see the block is not made undefined by it.
+constexpr int GATHER = 64;
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(128)
+gather_int8_kernel(const signed char* __restrict__ k_pages, const signed char* __restrict__ v_pages, const float* __restrict__ k_scales,
+                   const float* __restrict__ v_scales, T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table_out,
+                   const int* __restrict__ q_start, const int* __restrict__ ctx_lens, const int* __restrict__ block_table, int bt_stride,
+                   int bt_width, int page_size, int num_pages, int kv_heads, int head_dim, int width, int window) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int i = blockIdx.x, kvh = blockIdx.y, r = blockIdx.z;
+    const int ctx = ctx_lens[r], first = ctx - (q_start[r + 1] - q_start[r]);
+    const int lo = window > 0 ? max(0, first - window + 1) : 0;
+    const bool used = i * GATHER < ctx && (i + 1) * GATHER > lo;
+    if (kvh == 0 && threadIdx.x == 0) table_out[(size_t)r * width + i] = used ? r * width + i : -1;
+    if (!used) return;
+    constexpr int E = WIDE ? 16 : 1;
+    const int chunks = head_dim / E;
+    const size_t to = (((size_t)r * width + i) * kv_heads + kvh) * GATHER * head_dim;
+    for (int j = threadIdx.x; j < GATHER * chunks; j += 128) {
+        const int row = j / chunks, d = (j - row * chunks) * E;
+        const int pos = i * GATHER + row, lp = pos / page_size;
+        int page = -1;
+        if (pos < ctx && pos >= lo && lp < bt_width) page = __ldg(block_table + (size_t)r * bt_stride + lp);
+        if (page >= num_pages) page = -1;
+        const size_t block = (size_t)max(page, 0) * kv_heads + kvh;
+        const size_t from = (block * page_size + (pos - lp * page_size)) * head_dim + d, dst = to + (size_t)row * head_dim + d;
+        float ks = page >= 0 ? __ldg(k_scales + block) : 0.f, vs = page >= 0 ? __ldg(v_scales + block) : 0.f;
+        if (ks != ks || vs != vs) { ks = NAN; vs = 0.f; }
+        if (WIDE) {
+            uint4 k = make_uint4(0, 0, 0, 0), v = k;         // slots that nobody sees are finite
+            if (page >= 0) { k = *reinterpret_cast<const uint4*>(k_pages + from); v = *reinterpret_cast<const uint4*>(v_pages + from); }
+            store16<T>(k_out + dst, k, ks);
+            store16<T>(v_out + dst, v, vs);
+        } else {
+            Elem<T>::store(k_out + dst, page >= 0 ? (float)k_pages[from] * ks : 0.f);
+            Elem<T>::store(v_out + dst, page >= 0 ? (float)v_pages[from] * vs : 0.f);
+        }
+    }
+}
+
+template <typename T, int V>
+int launch_append(const void* qkv, void* q_out, const AppendArgs& a, cudaStream_t stream) {
+    const int per_head = (a.rot >> 1) / V + (a.head_dim - a.rot) / V;
+    const long long q_blocks = ((long long)a.m * a.heads * per_head + Q_THREADS - 1) / Q_THREADS;
+    NIB_REQUIRE(q_blocks + a.kv_blocks < (1LL << 31) - 1, "rope_store_int8: too many elements for one launch");
+    NIB_CUDA(launch_pdl(append_int8_kernel<T, V>, dim3((unsigned)(q_blocks + a.kv_blocks)), dim3(Q_THREADS), (size_t)0, stream,
+                        (const T*)qkv, (T*)q_out, a));
+    return 0;
+}
+
+}  // namespace
+
+// Rotates the queries of the rows [q heads | k heads | v heads] of ``qkv`` (row stride q_stride elements) into ``q_out`` (row
+// stride out_stride; may be qkv itself), and appends the rotated keys and the values to the 8-bit pages. ``units``: the sum over
+// the requests of (q_len + page_size - 2) / page_size + 1.
+NIB_API int nib_rope_store_int8(const void* qkv, int q_stride, void* q_out, int out_stride, const int* positions, const int* q_start,
+                                const int* ctx_lens, int n_req, int units, const float* cos_t, const float* sin_t, int table_rows, int rot,
+                                const int* block_table, int bt_stride, int bt_width, int page_size, void* k_pages, void* v_pages,
+                                float* k_scales, float* v_scales, int num_pages, int m, int heads, int kv_heads, int head_dim, int dtype,
+                                cudaStream_t stream) {
+    NIB_REQUIRE(m >= 0 && n_req >= 0 && units >= 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && page_size > 0 && num_pages > 0, "rope_store_int8: bad sizes");
+    NIB_REQUIRE(rot >= 0 && rot <= head_dim && rot % 2 == 0, "rope_store_int8: rotated width %d must be even and <= head_dim %d", rot, head_dim);
+    NIB_REQUIRE(rot == 0 || (cos_t && sin_t && table_rows > 0), "rope_store_int8: a rotated width without tables");
+    NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "rope_store_int8: unknown dtype %d", dtype);
+    if (m == 0) return 0;
+    AppendArgs a{positions, q_start, ctx_lens, cos_t, sin_t, block_table, (signed char*)k_pages, (signed char*)v_pages, k_scales, v_scales,
+                 table_rows, rot, bt_stride, bt_width, page_size, num_pages, m, n_req, heads, kv_heads, head_dim, q_stride, out_stride, units, 0};
+    const long long jobs = (long long)units * 2 * kv_heads;
+    NIB_REQUIRE(jobs < (1LL << 31) - KV_WARPS, "rope_store_int8: too many pages for one launch");
+    a.kv_blocks = (int)((jobs + KV_WARPS - 1) / KV_WARPS);
+    const int esize = dtype == NIB_F32 ? 4 : 2;
+    const bool wide = (rot / 2) % 4 == 0 && head_dim % 4 == 0 && q_stride % 4 == 0 && ((uintptr_t)qkv) % (4 * esize) == 0 &&
+                      (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15) == 0 && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 3) == 0;
+    if (dtype == NIB_F32) return wide ? launch_append<float, 4>(qkv, q_out, a, stream) : launch_append<float, 1>(qkv, q_out, a, stream);
+    return wide ? launch_append<__nv_bfloat16, 4>(qkv, q_out, a, stream) : launch_append<__nv_bfloat16, 1>(qkv, q_out, a, stream);
+}
+
+// out = codes * scale for ``blocks`` blocks of ``per_block`` codes each.
+NIB_API int nib_unpack_int8(const void* codes, const float* scales, void* out, long long blocks, int per_block, int dtype, cudaStream_t stream) {
+    NIB_REQUIRE(blocks >= 0 && per_block > 0, "unpack_int8: bad sizes");
+    NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "unpack_int8: unknown dtype %d", dtype);
+    if (blocks == 0) return 0;
+    const bool wide = per_block % 16 == 0 && (((uintptr_t)codes | (uintptr_t)out) & 15) == 0;
+    const int per = wide ? per_block / 16 : per_block;
+    const long long items = blocks * per, grid = (items + 255) / 256;
+    NIB_REQUIRE(grid < (1LL << 31) - 1, "unpack_int8: too many elements for one launch");
+#define CALL(T, W) NIB_CUDA(launch_pdl(unpack_int8_kernel<T, W>, dim3((unsigned)grid), dim3(256), (size_t)0, stream, (const signed char*)codes, scales, (T*)out, items, per))
+    if (dtype == NIB_F32) { if (wide) CALL(float, true); else CALL(float, false); }
+    else { if (wide) CALL(__nv_bfloat16, true); else CALL(__nv_bfloat16, false); }
+#undef CALL
+    return 0;
+}
+
+// The pages of n_req requests as pages of 64 tokens [n_req * width, kv_heads, 64, head_dim] in the order of their positions,
+// with the block table [n_req, width] that addresses them.
+NIB_API int nib_gather_int8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales, void* k_out, void* v_out,
+                            int* table_out, const int* q_start, const int* ctx_lens, int n_req, const int* block_table, int bt_stride,
+                            int bt_width, int page_size, int num_pages, int kv_heads, int head_dim, int width, int window, int dtype,
+                            cudaStream_t stream) {
+    NIB_REQUIRE(n_req >= 0 && width > 0 && page_size > 0 && num_pages > 0 && kv_heads > 0 && head_dim > 0 && window >= 0, "gather_int8: bad sizes");
+    NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "gather_int8: unknown dtype %d", dtype);
+    NIB_REQUIRE(n_req <= 65535 && kv_heads <= 65535 && (long long)n_req * width < (1LL << 31), "gather_int8: too many requests or heads for one launch");
+    if (n_req == 0) return 0;
+    const bool wide = head_dim % 16 == 0 && (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0;
+#define CALL(T, W) NIB_CUDA(launch_pdl(gather_int8_kernel<T, W>, dim3(width, kv_heads, n_req), dim3(128), (size_t)0, stream, (const signed char*)k_pages, \
+                                       (const signed char*)v_pages, k_scales, v_scales, (T*)k_out, (T*)v_out, table_out, q_start, ctx_lens, block_table, \
+                                       bt_stride, bt_width, page_size, num_pages, kv_heads, head_dim, width, window))
+    if (dtype == NIB_F32) { if (wide) CALL(float, true); else CALL(float, false); }
+    else { if (wide) CALL(__nv_bfloat16, true); else CALL(__nv_bfloat16, false); }
+#undef CALL
+    return 0;
+}

@@ -42,6 +42,13 @@ def _need(t: torch.Tensor, dtype, what: str, contiguous: bool = True):
         raise KernelError(f"{what}: tensor must be contiguous")
 
 
+def _here(t: torch.Tensor, dtype, what: str, contiguous: bool = True):
+    """``_need``, and the tensor lies on the device that the kernels are launched on."""
+    _need(t, dtype, what, contiguous)
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
 class _StreamScope:
     def __init__(self, ops):
         self.ops = ops
@@ -137,7 +144,8 @@ class Kernels:
                      "nib_rmsnorm_add", "nib_moe_route", "nib_moe_max_tiles", "nib_moe_group", "nib_moe_gemm_simt", "nib_moe_combine",
                      "nib_moe_tc_supported", "nib_moe_tc_error", "nib_moe_gather_rows", "nib_moe_gemm_tc", "nib_moe_step", "nib_moe_step_supported", "nib_moe_identity", "nib_stream_mix", "nib_grouped_state_scan", "nib_grouped_state_error", "nib_pdl_skip_next", "nib_memory_gates", "nib_layernorm",
                      "nib_decay_state_scan", "nib_decay_state_chunks_supported",
-                     "nib_gemm_stream", "nib_gemm_stream_supported", "nib_gemm_stream_error", "nib_sample_rows", "nib_sample_rows_most"):
+                     "nib_gemm_stream", "nib_gemm_stream_supported", "nib_gemm_stream_error", "nib_sample_rows", "nib_sample_rows_most",
+                     "nib_rope_store_int8", "nib_unpack_int8", "nib_gather_int8", "nib_attention_int8_decode", "nib_attention_int8_decode_kind"):
             getattr(self._lib, name).restype = c_int
         self.sample_rows_most = int(self._lib.nib_sample_rows_most())      # rows whose parameters a launch takes by value
         self._lib.nib_grouped_state_scratch.restype = self._lib.nib_decay_state_scratch.restype = c_longlong
@@ -605,14 +613,15 @@ class Kernels:
             c_int(_DT[qkv.dtype]), self._stream()), "rope_store")
 
     def attention(self, qkv, out, heads, kv_heads, head_dim, scale, window, ctx, block_table,
-                  page_size, k_pages, v_pages, own_kv=False):
+                  page_size, k_pages, v_pages, own_kv=False, first=0):
         """Attention of every token of the step over its request's cached keys (positions lo..own).
 
         bfloat16 with a supported head size runs on the tensor cores: the leading requests that bring one
         token each go to the decode kernel (keys split over CTAs), the others to the prefill kernel.
         Everything else (32-bit, other head sizes) runs the general kernel. ``own_kv``: the rows of ``qkv`` also
         hold each token's own rotated key and its value, the same that its page holds (a decode kernel may then
-        take them from the row instead of waiting for the page write)."""
+        take them from the row instead of waiting for the page write). ``first``: the rows of the requests before this one (all of
+        a single token) are somebody else's work."""
         _need(qkv, None, "attention qkv"); _need(out, qkv.dtype, "attention out")
         _need(k_pages, qkv.dtype, "k_pages"); _need(v_pages, qkv.dtype, "v_pages")
         _need(block_table, torch.int32, "block_table", contiguous=False)
@@ -626,18 +635,19 @@ class Kernels:
             self._lib.nib_attention_mma_supported(c_int(heads), c_int(kv_heads), c_int(head_dim)) == 1
         if not fast:
             self._check(self._lib.nib_attention_generic(
-                _ptr(qkv), c_int(qkv.stride(0)), _ptr(out), _ptr(ctx.positions), _ptr(ctx.req_index), _ptr(block_table),
+                _ptr(qkv[first:]), c_int(qkv.stride(0)), _ptr(out[first:]), c_void_p(ctx.positions.data_ptr() + 4 * first),
+                c_void_p(ctx.req_index.data_ptr() + 4 * first), _ptr(block_table),
                 c_int(bt_stride), c_int(page_size), _ptr(k_pages), _ptr(v_pages), c_int(num_pages),
-                c_int(m), c_int(heads), c_int(kv_heads), c_int(head_dim), c_float(scale), c_int(window),
+                c_int(m - first), c_int(heads), c_int(kv_heads), c_int(head_dim), c_float(scale), c_int(window),
                 c_int(_DT[qkv.dtype]), c_int(max(ctx.host.ctx_lens, default=0)), self._stream()), "attention")
             return
         q_lens, ctx_lens = ctx.host.q_lens, ctx.host.ctx_lens
         n_req = len(q_lens)
-        n_dec = 0
-        if heads // kv_heads <= 16:
+        n_dec = first
+        if heads // kv_heads <= 16 and not first:
             while n_dec < n_req and q_lens[n_dec] == 1:
                 n_dec += 1
-        if n_dec:
+        if n_dec > first:
             tma = self._decode_tma_ok(heads, kv_heads, head_dim, page_size)
             splits = self.decode_splits(n_dec, kv_heads, max(ctx_lens[:n_dec]), window, tma, head_dim)
             part_o = part_ml = counters = None
@@ -677,6 +687,132 @@ class Kernels:
                     _ptr(k_pages), _ptr(v_pages), c_int(num_pages), c_int(n_req - n_dec), c_int(max(q_lens[n_dec:])),
                     c_int(heads), c_int(kv_heads), c_int(head_dim), c_float(scale), c_int(window), self._stream()),
                     "attention prefill")
+
+    # ---- the 8-bit cache of keys and values (cache_int8.cu) ----------------------------------------------------------------
+    @staticmethod
+    def _cache_int8(what, kv_heads, page_size, head_dim, block_table, k_pages, v_pages, k_scales, v_scales) -> None:
+        """Refuses pools, scales or a block table that the kernels of the 8-bit cache cannot take."""
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _here(t, torch.int8, f"{what} {name}")
+            if tuple(t.shape[1:]) != (kv_heads, page_size, head_dim) or t.shape[0] != k_pages.shape[0] or t.shape[0] == 0:
+                raise KernelError(f"{what}: {name} {tuple(t.shape)} do not fit kv_heads/page_size/head_dim")
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            _here(t, torch.float32, f"{what} {name}")
+            if t.numel() != k_pages.shape[0] * kv_heads:
+                raise KernelError(f"{what}: {name} {tuple(t.shape)} do not fit a scale for each page and kv head")
+        _here(block_table, torch.int32, f"{what} block_table", contiguous=False)
+        if block_table.dim() != 2 or block_table.stride(1) != 1:
+            raise KernelError(f"{what}: block_table rows must be dense")
+
+    @staticmethod
+    def _step_requests(what, ctx, m, block_table) -> int:
+        """The number of requests of a step's context whose lengths fit ``m`` rows and the table."""
+        for name in ("positions", "req_index", "q_start", "ctx_lens"):
+            _here(getattr(ctx, name), torch.int32, f"{what} {name}")
+        n_req = len(ctx.host.q_lens)
+        if sum(ctx.host.q_lens) != m or ctx.positions.numel() < m or ctx.req_index.numel() < m or ctx.q_start.numel() != n_req + 1 or ctx.ctx_lens.numel() != n_req \
+                or block_table.shape[0] < n_req:
+            raise KernelError(f"{what}: the step's lengths do not fit {m} rows and {block_table.shape[0]} rows of the block table")
+        return n_req
+
+    def rope_store_int8(self, qkv, q_out, heads, kv_heads, head_dim, ctx, rotary, block_table, page_size, k_pages, v_pages, k_scales, v_scales):
+        """Rotates the queries of the rows [q heads | k heads | v heads] of ``qkv`` by their positions into ``q_out`` [m, heads *
+        head_dim] (which may be those columns of ``qkv`` itself), and appends the rotated keys and the values to an 8-bit paged
+        cache; the keys and values in ``qkv`` stay as they are.
+
+        ``k_pages``, ``v_pages``: int8 codes [pages, kv_heads, page_size, head_dim]; ``k_scales``, ``v_scales``: a float for each page
+        and kv head, a power of two; a value is code * scale. What a page held before the step's first token keeps its value up to
+        the rounding to a larger scale, if a new token needs one; a page that the step begins anew forgets its old scale. A
+        token whose key or value is not finite, or whose position the tables of ``rotary`` do not hold, makes its block's scale NaN.
+        No two requests may append to the same page."""
+        self._cache_int8("rope_store_int8", kv_heads, page_size, head_dim, block_table, k_pages, v_pages, k_scales, v_scales)
+        self._rows_here(qkv, None, "rope_store_int8 qkv"); self._rows_here(q_out, qkv.dtype, "rope_store_int8 q_out")
+        m = qkv.shape[0]
+        if qkv.dtype not in _DT:
+            raise KernelError(f"rope_store_int8: rows of {qkv.dtype}")
+        if qkv.shape[1] != (heads + 2 * kv_heads) * head_dim or tuple(q_out.shape) != (m, heads * head_dim):
+            raise KernelError("rope_store_int8: widths do not fit the head counts")
+        n_req = self._step_requests("rope_store_int8", ctx, m, block_table)
+        cos = sin = None
+        rot = 0
+        if rotary is not None:
+            cos, sin, rot = rotary
+            _here(cos, torch.float32, "cos"); _here(sin, torch.float32, "sin")
+            if cos.shape[1] != rot // 2 or sin.shape != cos.shape:
+                raise KernelError("rope_store_int8: table width must be rot/2")
+        units = sum((n + page_size - 2) // page_size + 1 for n in ctx.host.q_lens)
+        self._check(self._lib.nib_rope_store_int8(
+            _ptr(qkv), c_int(qkv.stride(0)), _ptr(q_out), c_int(q_out.stride(0)), _ptr(ctx.positions), _ptr(ctx.q_start), _ptr(ctx.ctx_lens),
+            c_int(n_req), c_int(units), _ptr(cos), _ptr(sin), c_int(0 if cos is None else cos.shape[0]), c_int(rot), _ptr(block_table),
+            c_int(block_table.stride(0)), c_int(block_table.shape[1]), c_int(page_size), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales),
+            _ptr(v_scales), c_int(k_pages.shape[0]), c_int(m), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(_DT[qkv.dtype]),
+            self._stream()), "rope_store (8-bit cache)")
+
+    def unpack_int8(self, pages, scales, out):
+        """out = what the codes of a pool stand for: ``pages`` int8 [pages, kv_heads, page_size, head_dim], ``scales`` a float for each
+        page and kv head, ``out`` of the pool's shape in bfloat16 or float32 (both hold the values exactly)."""
+        _here(pages, torch.int8, "unpack_int8 pages"); _here(scales, torch.float32, "unpack_int8 scales"); _here(out, None, "unpack_int8 out")
+        if pages.dim() != 4 or scales.numel() != pages.shape[0] * pages.shape[1] or out.shape != pages.shape or out.dtype not in _DT:
+            raise KernelError(f"unpack_int8: pages {tuple(pages.shape)}, scales {tuple(scales.shape)} and {out.dtype} {tuple(out.shape)} do not fit")
+        if pages.numel() == 0:
+            return
+        self._check(self._lib.nib_unpack_int8(_ptr(pages), _ptr(scales), _ptr(out), c_longlong(scales.numel()), c_int(pages.shape[2] * pages.shape[3]),
+                                              c_int(_DT[out.dtype]), self._stream()), "unpack (8-bit cache)")
+
+    def attention_int8(self, qkv, out, heads, kv_heads, head_dim, scale, window, ctx, block_table, page_size, k_pages, v_pages, k_scales, v_scales):
+        """``attention`` over the 8-bit cache that ``rope_store_int8`` fills: the rotated queries are the first columns of the rows of
+        ``qkv``, the step's own keys and values are in the pages already."""
+        self._cache_int8("attention_int8", kv_heads, page_size, head_dim, block_table, k_pages, v_pages, k_scales, v_scales)
+        self._rows_here(qkv, None, "attention_int8 qkv"); _here(out, qkv.dtype, "attention_int8 out")
+        m = qkv.shape[0]
+        if qkv.dtype not in _DT:
+            raise KernelError(f"attention_int8: rows of {qkv.dtype}")
+        if heads <= 0 or heads % kv_heads or qkv.shape[1] < heads * head_dim or tuple(out.shape) != (m, heads * head_dim) or window < 0:
+            raise KernelError("attention_int8: widths do not fit the head counts")
+        n_req = self._step_requests("attention_int8", ctx, m, block_table)
+        if m == 0:
+            return
+        pages = (c_int(page_size), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), c_int(k_pages.shape[0]))
+        n_dec, q_lens = 0, ctx.host.q_lens
+        kind = self._lib.nib_attention_int8_decode_kind(c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(page_size), c_int(_DT[qkv.dtype]))
+        while kind >= 0 and n_dec < n_req and q_lens[n_dec] == 1:
+            n_dec += 1
+        if n_dec:
+            splits = self._decode_int8_splits(n_dec, kv_heads, max(ctx.host.ctx_lens[:n_dec]), window, kind, head_dim)
+            parts, part_o, part_ml = splits // 8, None, None
+            if parts > 1:
+                part_o = torch.empty(n_dec * heads * parts * head_dim, dtype=torch.float32, device=qkv.device)
+                part_ml = torch.empty(n_dec * heads * parts * 2, dtype=torch.float32, device=qkv.device)
+                self.launches += 1
+            self._check(self._lib.nib_attention_int8_decode(
+                _ptr(qkv), c_int(qkv.stride(0)), _ptr(out), _ptr(ctx.ctx_lens), _ptr(block_table), c_int(block_table.stride(0)),
+                c_int(block_table.shape[1]), *pages, c_int(n_dec), c_int(heads), c_int(kv_heads), c_int(head_dim), c_float(scale), c_int(window),
+                c_int(splits), _ptr(part_o), _ptr(part_ml), c_int(_DT[qkv.dtype]), self._stream()), "attention decode (8-bit cache)")
+        if n_dec == n_req:
+            return
+        # The other requests' pages are read back once, in the order of their positions, and the prompt kernels run on them: a portion
+        # reads its keys once for each of its row tiles, and what the tensor cores multiply is 16 bits wide either way.
+        n_rest, width = n_req - n_dec, -(-block_table.shape[1] * page_size // 64)
+        keys = torch.empty((n_rest * width, kv_heads, 64, head_dim), dtype=qkv.dtype, device=qkv.device)
+        values = torch.empty_like(keys)
+        table = torch.empty((n_req, width), dtype=torch.int32, device=qkv.device)
+        self._check(self._lib.nib_gather_int8(
+            pages[1], pages[2], pages[3], pages[4], _ptr(keys), _ptr(values), c_void_p(table.data_ptr() + 4 * n_dec * width),
+            c_void_p(ctx.q_start.data_ptr() + 4 * n_dec), c_void_p(ctx.ctx_lens.data_ptr() + 4 * n_dec), c_int(n_rest),
+            c_void_p(block_table.data_ptr() + 4 * n_dec * block_table.stride(0)), c_int(block_table.stride(0)), c_int(block_table.shape[1]),
+            pages[0], pages[5], c_int(kv_heads), c_int(head_dim), c_int(width), c_int(window), c_int(_DT[qkv.dtype]), self._stream()),
+            "gather (8-bit cache)")
+        self._lib.nib_pdl_skip_next()       # the attention reads its table and earlier pages before its wait: here they are the kernel's before it
+        self.attention(qkv, out, heads, kv_heads, head_dim, scale, window, ctx, table, 64, keys, values, first=n_dec)
+
+    def _decode_int8_splits(self, n_tokens: int, kv_heads: int, max_ctx: int, window: int, kind: int, head_dim: int) -> int:
+        """Into how many CTAs the keys of a decoding token are split over the 8-bit cache."""
+        if self.options.fixed_decode_splits:
+            return _cluster_splits(self.options.fixed_decode_splits)
+        keys = min(max_ctx, window) if window > 0 else max_ctx
+        cta_keys = 32 if kind == 0 else 256 if head_dim == 64 else 128          # a step of every warp
+        want = -(-2 * self.sm_count // max(1, n_tokens * kv_heads))
+        return _cluster_splits(max(1, min(want, -(-keys // cta_keys), 64)))
 
     def attention_tc_error(self) -> int:
         """The error word of the tcgen05 attention's bounded waits (0 = none); synchronises and clears it."""
@@ -745,6 +881,13 @@ class Kernels:
         return max(1, min(-(-tiles // 2), most, 64))
 
     # ---- row-wise and element-wise kernels that several designs share (pointwise.cu) -------------
+    @staticmethod
+    def _rows_here(t, dtype, what):
+        """``_rows`` of the current device."""
+        _here(t, dtype, what, contiguous=False)
+        if t.dim() != 2 or t.stride(1) != 1:
+            raise KernelError(f"{what}: rows must be dense")
+
     @staticmethod
     def _rows(t, dtype, what):
         """A matrix whose rows are dense but may lie apart (a slice of the columns of a wider one)."""

@@ -1,0 +1,375 @@
+"""The 8-bit cache of keys and values: appending with the rotation, reading back, attention over it."""
+import math
+
+import pytest
+import torch
+
+import int8_cache_ref as ref
+from gpu_util import make_paged_batch
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from nanoinfer_b200.csrc.lib import load_kernels
+    return load_kernels(verbose=False)
+
+
+def rotary_tables(positions, rot, base=10000.0):
+    if rot == 0:
+        return None
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * (1.0 / base ** (2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot))
+    return angle.cos().float().cuda(), angle.sin().float().cuda(), rot
+
+
+def filled_pool(pages, kv, page, d, g, spread=1.0):
+    """Codes and scales of a pool in which every slot is held."""
+    x = torch.randn(pages, kv, page, d, generator=g, dtype=torch.float64) * torch.exp(spread * torch.randn(pages, kv, 1, 1, generator=g, dtype=torch.float64))
+    s = torch.tensor([[ref.block_scale(b.abs().max().item()) for b in p] for p in x], dtype=torch.float64)
+    return torch.round(x / s[:, :, None, None]).clamp(-127, 127), s
+
+
+class Batch:
+    """A step over a pool: inputs on the device, the pool's 64-bit copy here."""
+
+    def __init__(self, heads, kv, d, rot, page, q_lens, before, dtype, seed=0, pages=None, held=True):
+        g = torch.Generator().manual_seed(seed)
+        need = sum(-(-(b + n) // page) for b, n in zip(before, q_lens))
+        pages = pages or need + 2
+        self.heads, self.kv, self.d, self.page, self.dtype, self.q_lens, self.before = heads, kv, d, page, dtype, q_lens, before
+        self.ctx, self.table = make_paged_batch(q_lens, before, page, pages, "cuda", seed=seed)
+        self.codes, self.scales = zip(*(filled_pool(pages, kv, page, d, g) for _ in range(2)))
+        m = sum(q_lens)
+        self.rows = (torch.randn(m, heads + 2 * kv, d, generator=g) * torch.exp(torch.randn(m, heads + 2 * kv, 1, generator=g))).to(dtype)
+        self.qkv = self.rows.reshape(m, -1).cuda()
+        self.rotary = rotary_tables(max(b + n for b, n in zip(before, q_lens)), rot)
+        self.pools = [c.to(torch.int8).cuda() for c in self.codes]
+        self.pool_scales = [s.float().cuda() for s in self.scales]
+
+    def append(self, ops, q_out=None):
+        q = q_out if q_out is not None else torch.full((self.qkv.shape[0], self.heads * self.d), float("nan"), dtype=self.dtype, device="cuda")
+        ops.rope_store_int8(self.qkv, q, self.heads, self.kv, self.d, self.ctx, self.rotary, self.table, self.page, *self.pools, *self.pool_scales)
+        return q
+
+    def expected(self):
+        """(rotated queries, key codes, value codes, key scales, value scales) in 64 bits."""
+        codes, scales = [c.clone() for c in self.codes], [s.clone() for s in self.scales]
+        turned, at = [], 0
+        tables = self.table.cpu().tolist()
+        for i, (n, b) in enumerate(zip(self.q_lens, self.before)):
+            rows = self.rows[at:at + n]
+            at += n
+            qk = torch.stack([ref.rotate(rows[t, :self.heads + self.kv], b + t, self.rotary) for t in range(n)])
+            turned.append(qk[:, :self.heads])
+            for j, x in enumerate((qk[:, self.heads:], rows[:, self.heads + self.kv:].double())):
+                ref.append(codes[j], scales[j], x, b, tables[i], self.page)
+        return torch.cat(turned), codes[0], codes[1], scales[0], scales[1]
+
+
+def check_append(ops, b):
+    q = b.append(ops)
+    want_q, *want = b.expected()
+    # two products and a sum in 32 bits, and one rounding to the stored type
+    size = b.rows[:, :b.heads].double().abs().amax(dim=2, keepdim=True)
+    bound = HALF_STEP[b.dtype] * want_q.abs() + 4 * 2.0 ** -24 * size
+    assert ((q.cpu().double().reshape(want_q.shape) - want_q).abs() <= bound).all()
+    for got, w in zip(b.pools + b.pool_scales, want):
+        assert torch.equal(got.cpu().double(), w)
+
+
+SHAPES = [(14, 2, 64, 64, 16), (28, 4, 128, 128, 16), (4, 2, 64, 32, 8), (6, 3, 128, 64, 32), (4, 4, 32, 32, 5), (4, 1, 80, 80, 24), (2, 2, 18, 6, 3),
+          (3, 1, 64, 0, 64)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,rot,page", SHAPES)
+def test_append_follows_the_definition(ops, heads, kv, d, rot, page, dtype):
+    check_append(ops, Batch(heads, kv, d, rot, page, [1], [0], dtype, seed=1))
+    check_append(ops, Batch(heads, kv, d, rot, page, [1, 1, 1, 1], [7, page - 1, page, 4 * page + 2], dtype, seed=2))
+    check_append(ops, Batch(heads, kv, d, rot, page, [3 * page + 1, 1, page, 2], [0, 2 * page - 1, page + 1, page - 1], dtype, seed=3))
+
+
+def test_append_of_more_requests_than_a_warp_has_lanes(ops):
+    lens = [1 + (5 * i) % 23 for i in range(75)]
+    check_append(ops, Batch(4, 2, 64, 64, 16, lens, [(7 * i) % 40 for i in range(75)], torch.bfloat16, seed=4))
+
+
+def test_append_token_by_token_and_all_at_once_differ_by_less_than_a_step(ops):
+    n, page = 50, 16
+    whole = Batch(2, 2, 64, 64, page, [n], [0], torch.bfloat16, seed=5)
+    whole.append(ops)
+    single = Batch(2, 2, 64, 64, page, [n], [0], torch.bfloat16, seed=5)
+    for t in range(n):
+        step = Batch(2, 2, 64, 64, page, [1], [t], torch.bfloat16, seed=5)
+        step.pools, step.pool_scales, step.rotary = single.pools, single.pool_scales, single.rotary
+        step.table, step.qkv = single.table, single.qkv[t:t + 1].contiguous()
+        step.append(ops)
+    for j in range(2):
+        # the last scale of a block is that of its largest token either way
+        assert torch.equal(whole.pool_scales[j], single.pool_scales[j])
+        a, b = (ref.values(x.pools[j].cpu(), x.pool_scales[j].cpu()) for x in (whole, single))
+        for lp in range(-(-n // page)):
+            p = int(whole.table[0, lp])
+            held = min(page, n - lp * page)
+            assert ((a - b)[p, :, :held].abs() <= whole.pool_scales[j].cpu().double()[p][:, None, None]).all()
+
+
+def test_append_in_place_strided_rows_and_a_padding_row(ops):
+    b = Batch(6, 2, 64, 64, 16, [1, 4], [20, 13], torch.bfloat16, seed=6)
+    want_q, *want = b.expected()
+    wide = torch.zeros(5, 10 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    wide[:, 4:-4] = b.qkv
+    b.qkv = wide[:, 4:-4]           # rows that begin in the middle of 16 bytes
+    kept = wide[:, 4 + 6 * 64:].clone()
+    q = b.append(ops, q_out=wide[:, 4:4 + 6 * 64])
+    assert torch.equal(wide[:, 4 + 6 * 64:], kept) and (wide[:, :4] == 0).all()
+    assert ((q.cpu().double().reshape(want_q.shape) - want_q).abs() <= 2.0 ** -8 * want_q.abs() + 1e-5 * b.rows.double().abs().max()).all()
+    for got, w in zip(b.pools + b.pool_scales, want):
+        assert torch.equal(got.cpu().double(), w)
+    # a row of a request that holds nothing writes nothing
+    b.ctx.ctx_lens.fill_(0)
+    b.ctx.ctx_lens[1] = 17
+    before = [t.clone() for t in b.pools]
+    b.qkv = torch.randn_like(b.qkv)
+    b.append(ops)
+    own = int(b.table[0, 1])
+    assert torch.equal(b.pools[0][own], before[0][own]) and not torch.equal(b.pools[0], before[0])
+
+
+def test_append_where_pages_are_not_held_or_lie_outside_the_pool_writes_nothing_there(ops):
+    b = Batch(2, 1, 64, 64, 8, [9, 9], [4, 0], torch.bfloat16, seed=7)
+    b.table[0, 0] = -1
+    b.table[1, 1] = 1 << 20
+    check_append(ops, b)
+
+
+def test_append_keeps_zero_blocks_and_extreme_magnitudes(ops):
+    for factor in (0.0, 2.0 ** -120, 2.0 ** 120, 1e-30):
+        b = Batch(2, 2, 64, 64, 16, [5, 1], [3, 16], torch.float32, seed=8)
+        b.rows = (b.rows.double() * factor).float()
+        b.qkv = b.rows.reshape(6, -1).cuda()
+        b.append(ops)
+        _, *want = b.expected()
+        for got, w in zip(b.pools + b.pool_scales, want):
+            assert torch.equal(got.cpu().double(), w)
+
+
+def test_append_of_undefined_values_marks_their_block_and_no_other(ops):
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        b = Batch(2, 2, 64, 64, 16, [20, 1], [3, 40], torch.bfloat16, seed=9)
+        b.qkv[2, (2 + 2 + 1) * 64 + 5] = bad            # a value of kv head 1, position 5
+        b.qkv[20, 2 * 64 + 3] = bad                     # a key of kv head 0, position 40
+        before = [t.clone() for t in b.pool_scales]
+        b.append(ops)
+        v_page, k_page = int(b.table[0, 0]), int(b.table[1, 2])
+        assert torch.isnan(b.pool_scales[1][v_page, 1]) and torch.isnan(b.pool_scales[0][k_page, 0])
+        for j, at in ((0, (k_page, 0)), (1, (v_page, 1))):
+            rest = torch.ones_like(before[j], dtype=torch.bool)
+            rest[at] = False
+            assert torch.isfinite(b.pool_scales[j][rest]).all()
+        # the mark stays until the page begins anew
+        c = Batch(2, 2, 64, 64, 16, [1], [41], torch.bfloat16, seed=10)
+        c.pools, c.pool_scales, c.table = b.pools, b.pool_scales, b.table[1:].contiguous()
+        c.append(ops)
+        assert torch.isnan(b.pool_scales[0][k_page, 0])
+        d = Batch(2, 2, 64, 64, 16, [1], [32], torch.bfloat16, seed=10)
+        d.pools, d.pool_scales, d.table = b.pools, b.pool_scales, b.table[1:].contiguous()
+        d.append(ops)
+        assert torch.isfinite(b.pool_scales[0][k_page, 0])
+
+
+def test_append_a_scale_that_was_never_set_stands_for_zeros(ops):
+    b = Batch(2, 1, 64, 64, 16, [2], [3], torch.bfloat16, seed=11)
+    page = int(b.table[0, 0])
+    for j in range(2):
+        b.scales[j][page] = 0.0
+        b.pool_scales[j][page] = 0.0
+    check_append(ops, b)
+    assert (b.pools[0][page, :, :3] == 0).all()
+
+
+def test_append_of_a_position_behind_the_tables_is_undefined_and_reads_nothing_else(ops):
+    b = Batch(2, 1, 64, 64, 16, [1, 1], [5, 9], torch.bfloat16, seed=12)
+    cos, sin, rot = b.rotary
+    b.rotary = (cos[:6].contiguous(), sin[:6].contiguous(), rot)
+    q = b.append(ops)
+    assert torch.isfinite(q[0]).all() and torch.isnan(q[1]).all()
+    assert torch.isnan(b.pool_scales[0][int(b.table[1, 0]), 0]) and torch.isfinite(b.pool_scales[1]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(7, 2, 16, 64), (3, 1, 5, 18), (1, 1, 1, 1)])
+def test_unpack_is_exact(ops, shape, dtype):
+    codes, scales = filled_pool(*shape, torch.Generator().manual_seed(13))
+    out = torch.empty(shape, dtype=dtype, device="cuda")
+    ops.unpack_int8(codes.to(torch.int8).cuda(), scales.float().cuda(), out)
+    assert torch.equal(out.cpu().double(), ref.values(codes, scales))
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------
+def check_attention(ops, b, window=0, scale=None):
+    """The weights are rounded to 16 bits where a tensor core multiplies them with the values (half a step of bfloat16, relative to
+    sum w |v|), a bfloat16 row once more; 32-bit sums of some thousand terms lose a few steps of 2^-24 of the same size, and the
+    exponent of a score s loses |s| 2^-23, for which 2^-14 is ample.
+
+    A weight that is small beside the largest one is rounded to a multiple of the smallest 16-bit number: with p_j = 2^(t_j - M), t_j the
+    score plus the logarithm of the value scale s_j and M at most max t, that is off by at most 2^-25 each, which moves the row by at most
+    2^-25 sum_j 127 2^M / sum_j 2^(score_j) <= 2^-25 n 127 sum_j w_j s_j. One below 2^-126 of the largest is nothing in 32 bits."""
+    scale = b.d ** -0.5 if scale is None else scale
+    out = torch.full((b.qkv.shape[0], b.heads * b.d), float("nan"), dtype=b.dtype, device="cuda")
+    ops.attention_int8(b.qkv, out, b.heads, b.kv, b.d, scale, window, b.ctx, b.table, b.page, *b.pools, *b.pool_scales)
+    keys, vals = (ref.values(c.cpu(), s.cpu()) for c, s in zip(b.pools, b.pool_scales))
+    tables, at = b.table.cpu().tolist(), 0
+    rounding = (2.0 ** -8 if b.dtype == torch.bfloat16 else 0.0) + 2.0 ** -14
+    for i, (n, p) in enumerate(zip(b.q_lens, b.before)):
+        for t in range(n):
+            q = b.rows[at, :b.heads]
+            want, size, small = ref.attend(q, keys, vals, b.pool_scales[1].cpu(), tables[i], b.page, p + t, scale, window, b.kv)
+            got = out[at].cpu().double().reshape(b.heads, b.d)
+            assert ((got - want).abs() <= HALF_STEP[b.dtype] * want.abs() + rounding * size + 2.0 ** -25 * small).all(), (i, t)
+            at += 1
+    return out
+
+
+ATTENTION_SHAPES = [(14, 2, 64, 16), (12, 2, 128, 16), (28, 4, 128, 32), (16, 1, 64, 8), (12, 1, 128, 64), (32, 2, 64, 64), (3, 3, 64, 16),
+                    (6, 2, 32, 16), (4, 2, 80, 24), (20, 1, 64, 16), (4, 2, 64, 5), (2, 1, 18, 3)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,page", ATTENTION_SHAPES)
+def test_attention_of_single_tokens(ops, heads, kv, d, page, dtype):
+    check_attention(ops, Batch(heads, kv, d, 0, page, [1], [0], dtype, seed=20))
+    check_attention(ops, Batch(heads, kv, d, 0, page, [1, 1, 1, 1, 1], [1, 15, 16, 200, 517], dtype, seed=21))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,page", ATTENTION_SHAPES)
+def test_attention_of_portions_and_mixed_steps(ops, heads, kv, d, page, dtype):
+    check_attention(ops, Batch(heads, kv, d, 0, page, [1, 1, 37, 2, 70], [130, 0, 0, 63, 61], dtype, seed=22))
+
+
+@pytest.mark.parametrize("window", [1, 7, 16, 64, 100, 1000])
+def test_attention_within_a_window_whose_first_pages_are_given_back(ops, window):
+    for heads, kv, d, page in ((14, 2, 64, 16), (12, 2, 128, 8), (4, 2, 32, 16)):
+        b = Batch(heads, kv, d, 0, page, [1, 1, 1, 9, 80], [300, 4, 63, 150, 40], torch.bfloat16, seed=23)
+        for i, p in enumerate(b.before):
+            b.table[i, :max(0, p + 1 - window) // page] = -1
+        check_attention(ops, b, window=window)
+
+
+def test_attention_of_a_long_context_over_many_ctas(ops):
+    for heads, kv, d, before in ((14, 2, 64, [9000]), (4, 1, 128, [20011, 3]), (2, 2, 64, [4095, 4096, 2047, 1])):
+        check_attention(ops, Batch(heads, kv, d, 0, 16, [1] * len(before), before, torch.bfloat16, seed=24))
+
+
+def test_attention_rows_that_see_nothing_are_zero_and_masked_blocks_do_not_count(ops):
+    for dtype in (torch.bfloat16, torch.float32):
+        b = Batch(6, 2, 64, 0, 16, [1, 1], [40, 70], dtype, seed=25)
+        # undefined blocks that no token sees: behind the window's end, and slots behind a request's last token
+        window = 20
+        for t in b.pool_scales:
+            t[int(b.table[1, 0])] = float("nan")
+        got = attention_rows(ops, b, window)
+        assert torch.isfinite(got).all()
+        b.ctx.ctx_lens[0] = 0
+        b.table[0] = -1
+        out = torch.full((2, 6 * 64), float("nan"), dtype=dtype, device="cuda")
+        ops.attention_int8(b.qkv, out, 6, 2, 64, 0.125, window, b.ctx, b.table, 16, *b.pools, *b.pool_scales)
+        assert (out[0] == 0).all() and torch.equal(out[1], got[1])
+
+
+def attention_rows(ops, b, window=0):
+    out = torch.empty(b.qkv.shape[0], b.heads * b.d, dtype=b.dtype, device="cuda")
+    ops.attention_int8(b.qkv, out, b.heads, b.kv, b.d, b.d ** -0.5, window, b.ctx, b.table, b.page, *b.pools, *b.pool_scales)
+    return out
+
+
+def test_attention_of_undefined_blocks_is_undefined(ops):
+    for j in range(2):
+        for dtype in (torch.bfloat16, torch.float32):
+            b = Batch(4, 2, 64, 0, 16, [1, 1], [40, 70], dtype, seed=26)
+            b.pool_scales[j][int(b.table[0, 1]), 1] = float("nan")
+            got = attention_rows(ops, b).reshape(2, 4, 64)
+            assert torch.isnan(got[0, 2:]).all() and torch.isfinite(got[0, :2]).all() and torch.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("exponents", [(-80, 121), (-60, 60), (-20, 20), (-80, -70), (100, 119)])
+def test_attention_over_blocks_of_very_different_sizes(ops, exponents):
+    """Value scales that differ by any power of two: the rows are still right to their own size."""
+    lo, hi = exponents
+    b = Batch(6, 2, 64, 0, 16, [1, 1], [90, 170], torch.bfloat16, seed=27)
+    g = torch.Generator().manual_seed(28)
+    b.pool_scales[1].copy_(torch.pow(2.0, torch.randint(lo, hi + 1, b.scales[1].shape, generator=g).double()).float())
+    check_attention(ops, b)
+
+
+def test_attention_of_queries_of_very_different_sizes(ops):
+    for factor in (2.0 ** -100, 2.0 ** -20, 2.0 ** 14, 2.0 ** 40):
+        b = Batch(6, 2, 128, 0, 16, [1, 1], [90, 170], torch.bfloat16, seed=29)
+        b.rows = (b.rows.float() * factor).to(torch.bfloat16)
+        b.qkv = b.rows.reshape(2, -1).cuda()
+        check_attention(ops, b, scale=128 ** -0.5 / factor)
+
+
+def test_append_and_attention_run_together_as_a_model_calls_them(ops):
+    """A prompt in two portions, then tokens one at a time, all requests at different places: every row is the attention of the
+    cache as it is then."""
+    heads, kv, d, page = 14, 2, 64, 16
+    pages = 64
+    first = Batch(heads, kv, d, d, page, [33, 20], [0, 0], torch.bfloat16, seed=30, pages=pages)
+    pools, scales, table = first.pools, first.pool_scales, torch.full((2, 16), -1, dtype=torch.int32, device="cuda")
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(31)).tolist()
+    lengths = [0, 0]
+    rotary = rotary_tables(256, d)
+    for step, lens in enumerate([[33, 20], [1, 31], [40, 1], [1, 1], [1, 1], [1, 1]]):
+        b = Batch(heads, kv, d, d, page, lens, list(lengths), torch.bfloat16, seed=40 + step, pages=pages)
+        for i in range(2):
+            for lp in range(-(-(lengths[i] + lens[i]) // page)):
+                if int(table[i, lp]) < 0:
+                    table[i, lp] = order.pop()
+        b.pools, b.pool_scales, b.table, b.rotary = pools, scales, table, rotary
+        q = b.append(ops)
+        b.rows[:, :heads] = q.reshape(-1, heads, d).cpu()
+        b.qkv = q
+        check_attention(ops, b)
+        lengths = [a + n for a, n in zip(lengths, lens)]
+
+
+def test_refusals(ops):
+    from nanoinfer_b200.csrc.lib import KernelError
+    b = Batch(4, 2, 64, 64, 16, [1, 3], [5, 25], torch.bfloat16, seed=50)      # (a table of two columns: one of one column is dense turned over, too)
+    q = torch.empty(4, 256, dtype=torch.bfloat16, device="cuda")
+
+    def append(**change):
+        a = dict(qkv=b.qkv, q_out=q, heads=4, kv_heads=2, head_dim=64, ctx=b.ctx, rotary=b.rotary, block_table=b.table, page_size=16,
+                 k_pages=b.pools[0], v_pages=b.pools[1], k_scales=b.pool_scales[0], v_scales=b.pool_scales[1])
+        a.update(change)
+        ops.rope_store_int8(**a)
+
+    def attend(**change):
+        a = dict(qkv=b.qkv, out=q, heads=4, kv_heads=2, head_dim=64, scale=0.125, window=0, ctx=b.ctx, block_table=b.table, page_size=16,
+                 k_pages=b.pools[0], v_pages=b.pools[1], k_scales=b.pool_scales[0], v_scales=b.pool_scales[1])
+        a.update(change)
+        ops.attention_int8(**a)
+
+    for call in (append, attend):
+        call()
+        for change in (dict(k_pages=b.pools[0].to(torch.uint8)), dict(v_pages=b.pools[1].cpu()), dict(v_pages=b.pools[1][:-1].contiguous()),
+                       dict(k_scales=b.pool_scales[0].double()), dict(v_scales=b.pool_scales[1][:-1].contiguous()), dict(page_size=8),
+                       dict(kv_heads=1), dict(head_dim=32), dict(block_table=b.table.long()), dict(block_table=b.table[:1]),
+                       dict(block_table=b.table.t().contiguous().t()), dict(qkv=b.qkv[:3]), dict(qkv=b.qkv.half())):
+            with pytest.raises(KernelError):
+                call(**change)
+    for change in (dict(q_out=q[:, :128]), dict(q_out=q.float()), dict(rotary=(b.rotary[0], b.rotary[1], 32)), dict(rotary=(b.rotary[0].cpu(), b.rotary[1], 64))):
+        with pytest.raises(KernelError):
+            append(**change)
+    for change in (dict(out=q.float()), dict(out=q[:3]), dict(window=-1), dict(heads=3)):
+        with pytest.raises(KernelError):
+            attend(**change)
+    with pytest.raises(KernelError):
+        ops.unpack_int8(b.pools[0], b.pool_scales[0], torch.empty(b.pools[0].shape, dtype=torch.float16, device="cuda"))
+    with pytest.raises(KernelError):
+        ops.unpack_int8(b.pools[0], b.pool_scales[0], torch.empty(2, 2, dtype=torch.float32, device="cuda"))
