@@ -16,6 +16,7 @@ import torch
 from . import build as _build
 from ..config.kernel_options import KernelOptions
 from ..parts.base import LazyNorm
+from ..weights.int4 import Int4Matrix
 
 
 class KernelError(RuntimeError):
@@ -145,7 +146,8 @@ class Kernels:
                      "nib_moe_tc_supported", "nib_moe_tc_error", "nib_moe_gather_rows", "nib_moe_gemm_tc", "nib_moe_step", "nib_moe_step_supported", "nib_moe_identity", "nib_stream_mix", "nib_grouped_state_scan", "nib_grouped_state_error", "nib_pdl_skip_next", "nib_memory_gates", "nib_layernorm",
                      "nib_decay_state_scan", "nib_decay_state_chunks_supported",
                      "nib_gemm_stream", "nib_gemm_stream_supported", "nib_gemm_stream_error", "nib_sample_rows", "nib_sample_rows_most",
-                     "nib_rope_store_int8", "nib_unpack_int8", "nib_gather_int8", "nib_attention_int8_decode", "nib_attention_int8_decode_kind"):
+                     "nib_rope_store_int8", "nib_unpack_int8", "nib_gather_int8", "nib_attention_int8_decode", "nib_attention_int8_decode_kind",
+                     "nib_gemm_int4", "nib_gemm_int4_supported", "nib_unpack_int4"):
             getattr(self._lib, name).restype = c_int
         self.sample_rows_most = int(self._lib.nib_sample_rows_most())      # rows whose parameters a launch takes by value
         self._lib.nib_grouped_state_scratch.restype = self._lib.nib_decay_state_scratch.restype = c_longlong
@@ -304,7 +306,11 @@ class Kernels:
         """out[M,N] (=, +=) a[M,K] . w[N,K]^T (+ bias). mode: 'store' | 'add' (float out) | 'f32' (float out).
         ``a`` may be a LazyNorm: the small-M kernel then applies the norm while it reads the residual stream. The products of few tokens
         (small-M, and 32-bit ones) read ``w`` before they wait for the kernel before them: there it must not be what a kernel
-        launched just before writes; with more tokens that holds of an instance made by ``with_weights_ahead`` only."""
+        launched just before writes; with more tokens that holds of an instance made by ``with_weights_ahead`` only. ``w`` may be
+        an ``Int4Matrix``."""
+        if isinstance(w, Int4Matrix):
+            self._linear_int4("linear", a, w, bias32, out, mode, None)
+            return
         lazy = a if isinstance(a, LazyNorm) else None
         dtype = a.dtype
         if lazy is None:
@@ -495,7 +501,13 @@ class Kernels:
 
     def linear_swiglu(self, a, w_gate_up, out, glu=None, act="silu"):
         """out[M,I] = silu(a . w[:I]^T) * (a . w[I:]^T), with ``act`` 'gelu_tanh' gelu (its tanh form) in place of silu. With ``glu`` = (alpha, limit, shift): g = min(gate, limit),
-        u = clamp(up, -limit, limit), g * sigmoid(alpha g) * (u + shift)."""
+        u = clamp(up, -limit, limit), g * sigmoid(alpha g) * (u + shift). ``w_gate_up`` may be an ``Int4Matrix``."""
+        if act not in ("silu", "gelu_tanh") or (glu is not None and act != "silu"):
+            raise KernelError(f"linear_swiglu: no gated form with '{act}'" + (" and constants" if glu is not None else ""))
+        epi = "geglu" if act == "gelu_tanh" else ("swiglu" if glu is None else "glu")
+        if isinstance(w_gate_up, Int4Matrix):
+            self._linear_int4("linear_swiglu", a, w_gate_up, None, out, epi, _glu(glu))
+            return
         if not isinstance(a, LazyNorm):
             _need(a, None, "swiglu a")
         _need(w_gate_up, a.dtype, "swiglu w"); _need(out, a.dtype, "swiglu out")
@@ -503,10 +515,48 @@ class Kernels:
         inter = w_gate_up.shape[0] // 2
         if w_gate_up.shape[0] != 2 * inter or w_gate_up.shape[1] != k or tuple(out.shape) != (m, inter):
             raise KernelError("linear_swiglu: shapes do not fit")
-        if act not in ("silu", "gelu_tanh") or (glu is not None and act != "silu"):
-            raise KernelError(f"linear_swiglu: no gated form with '{act}'" + (" and constants" if glu is not None else ""))
-        epi = "geglu" if act == "gelu_tanh" else ("swiglu" if glu is None else "glu")
         self._gemm(a, w_gate_up, None, out, m, inter, k, _EPI[epi], _glu(glu))
+
+    def _linear_int4(self, what, a, w, bias32, out, mode, glu):
+        """A product with 4-bit weights. Up to 64 tokens of bfloat16 multiply with the codes (gemm_int4.cu); more, and 32-bit rows, with
+        the weights unpacked into a scratch matrix of their own type, by the products above. Weights whose scales need more than
+        bfloat16's 8 bits are rounded there where the result is rounded to bfloat16 itself; a 32-bit result gets what the rounding
+        left by a second product."""
+        if isinstance(a, LazyNorm):
+            a = self._resolve(a, a.shape[0] <= 16)
+        self._rows_here(a, None, f"{what} a"); self._rows_here(out, None, f"{what} out"); _here(w.packed, torch.uint8, f"{what} w")
+        dual = _EPI[mode] in _DUAL
+        (m, k), n = a.shape, w.shape[0] // 2 if dual else w.shape[0]
+        if a.dtype not in _DT or w.shape[1] != k or (dual and 2 * n != w.shape[0]) or tuple(out.shape) != (m, n):
+            raise KernelError(f"{what}: shapes a{tuple(a.shape)} w{w.shape} out{tuple(out.shape)} do not fit")
+        if out.dtype != (torch.float32 if mode in ("add", "f32") else a.dtype):
+            raise KernelError(f"{what}[{mode}]: out is {out.dtype}")
+        if bias32 is not None:
+            _here(bias32, torch.float32, f"{what} bias")
+            if bias32.numel() != n:
+                raise KernelError(f"{what}: {bias32.numel()} biases for {n} columns")
+        if m == 0:
+            return
+        if a.dtype == torch.bfloat16 and self._lib.nib_gemm_int4_supported(_ptr(a), c_int(m), c_int(n), c_int(k), c_int(a.stride(0)), c_int(w.group),
+                                                                          c_int(1 if dual else 0)) == 1:
+            if not self.weights_ahead:
+                self._lib.nib_pdl_skip_next()
+            self._check(self._lib.nib_gemm_int4(_ptr(a), _ptr(w.packed), _ptr(w.scales), _ptr(bias32), _ptr(out), c_int(m), c_int(n), c_int(k),
+                                                c_int(w.group), c_int(a.stride(0)), c_int(out.stride(0)), c_int(_EPI[mode]), glu, c_int(self.sm_count),
+                                                self._stream()), "linear (4-bit weights)")
+            return
+        plain = torch.empty(w.shape, dtype=a.dtype, device=a.device)
+        self._unpack_int4(w, plain, 0)
+        self._lib.nib_pdl_skip_next()           # the product may not read its weights ahead of the kernel that writes them
+        self._gemm(a, plain, bias32, out, m, n, k, _EPI[mode], glu)
+        if a.dtype == torch.bfloat16 and mode in ("add", "f32") and not w.bf16_exact:
+            self._unpack_int4(w, plain, 1)
+            self._lib.nib_pdl_skip_next()
+            self._gemm(a, plain, None, out, m, n, k, _ADD)
+
+    def _unpack_int4(self, w, out, part):
+        self._check(self._lib.nib_unpack_int4(_ptr(w.packed), _ptr(w.scales), _ptr(out), c_int(w.shape[0]), c_int(w.shape[1]), c_int(w.group),
+                                              c_int(part), c_int(_DT[out.dtype]), self._stream()), "unpack (4-bit weights)")
 
     def qkv_project(self, a, w_qkv, bias32, qkv, heads, kv_heads, head_dim, positions, req_index, rotary,
                     block_table, page_size, k_pages, v_pages, writes):
@@ -517,6 +567,10 @@ class Kernels:
         small-M product's epilogue, the norm its prologue); so do the tiles of 128 tokens of the one-CTA tcgen05
         product (heads of 64 or 128 that are rotated whole); everything else is the product followed by
         ``rope_store``."""
+        if isinstance(w_qkv, Int4Matrix):
+            self.linear(a, w_qkv, bias32, qkv, "store")
+            self.rope_store(qkv, heads, kv_heads, head_dim, positions, req_index, rotary, block_table, page_size, k_pages, v_pages, writes)
+            return
         lazy = a if isinstance(a, LazyNorm) else None
         if lazy is not None and not self._foldable(lazy):
             a, lazy = lazy.resolve(), None
