@@ -506,29 +506,39 @@ NIB_API int nib_attention_int8_decode_kind(int heads, int kv_heads, int head_dim
     return any_smem(heads / kv_heads, head_dim) <= MAX_SMEM ? 0 : -1;
 }
 
+// The arguments of a call, one block of memory.
+struct NibAttendInt8 {
+    const void* q; void* out; const int* ctx_lens; const int* block_table; const void* k_pages; const void* v_pages; const float* k_scales;
+    const float* v_scales; float* part_o; float* part_ml;
+    int q_stride, bt_stride, bt_width, page_size, num_pages, n_tokens, heads, kv_heads, head_dim, window, splits, dtype;
+    float scale; int pad;
+};
+
 // Attention of n_tokens single tokens (token i is request i, at position ctx_lens[i] - 1) whose keys and values are in the pages.
 // ``splits`` CTAs share the keys of a (token, kv head): 1, 2, 4, 8 or a multiple of 8, which needs part_o [tokens * heads * splits/8
 // * head_dim] and part_ml [tokens * heads * splits/8 * 2].
-NIB_API int nib_attention_int8_decode(const void* q, int q_stride, void* out, const int* ctx_lens, const int* block_table, int bt_stride,
-                                      int bt_width, int page_size, const void* k_pages, const void* v_pages, const float* k_scales,
-                                      const float* v_scales, int num_pages, int n_tokens, int heads, int kv_heads, int head_dim, float scale,
-                                      int window, int splits, float* part_o, float* part_ml, int dtype, cudaStream_t stream) {
-    NIB_REQUIRE(n_tokens >= 0 && num_pages > 0 && page_size > 0 && bt_width >= 0 && window >= 0 && splits >= 1 && splits <= 256, "attention (8-bit cache): bad sizes");
+NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
+    NibAttendInt8 c;
+    memcpy(&c, args, sizeof c);
+    const int n_tokens = c.n_tokens, heads = c.heads, kv_heads = c.kv_heads, head_dim = c.head_dim, page_size = c.page_size, splits = c.splits, dtype = c.dtype;
+    const void* q = c.q;
+    void* out = c.out;
+    NIB_REQUIRE(n_tokens >= 0 && c.num_pages > 0 && page_size > 0 && c.bt_width >= 0 && c.window >= 0 && splits >= 1 && splits <= 256, "attention (8-bit cache): bad sizes");
     NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "attention (8-bit cache): unknown dtype %d", dtype);
     const int kind = nib_attention_int8_decode_kind(heads, kv_heads, head_dim, page_size, dtype);
     NIB_REQUIRE(kind >= 0, "attention (8-bit cache): %d/%d heads of %d are not supported", heads, kv_heads, head_dim);
     const int csize = splits >= 8 ? 8 : splits;
     NIB_REQUIRE((csize & (csize - 1)) == 0 && splits % csize == 0, "attention (8-bit cache): %d splits; 1, 2, 4, 8 or a multiple of 8 are possible", splits);
-    NIB_REQUIRE(splits == csize || (part_o && part_ml), "attention (8-bit cache): more than 8 splits need scratch memory");
+    NIB_REQUIRE(splits == csize || (c.part_o && c.part_ml), "attention (8-bit cache): more than 8 splits need scratch memory");
     NIB_REQUIRE(n_tokens <= 65535 && kv_heads <= 65535 && (long long)n_tokens * heads < (1LL << 31), "attention (8-bit cache): too many tokens or heads for one launch");
     if (n_tokens == 0) return 0;
     int shift = -1;
     if ((page_size & (page_size - 1)) == 0) for (shift = 0; (1 << shift) < page_size;) ++shift;
-    const Args a{ctx_lens, block_table, (const signed char*)k_pages, (const signed char*)v_pages, k_scales, v_scales, part_o, part_ml,
-                 q_stride, bt_stride, bt_width, page_size, shift, num_pages, heads, kv_heads, heads / kv_heads, head_dim, window, splits, csize, scale};
+    const Args a{c.ctx_lens, c.block_table, (const signed char*)c.k_pages, (const signed char*)c.v_pages, c.k_scales, c.v_scales, c.part_o, c.part_ml,
+                 c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, heads, kv_heads, heads / kv_heads, head_dim, c.window, splits, csize, c.scale};
     int rc;
     if (kind == 1) {
-        NIB_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "attention (8-bit cache): the pools must be 16-byte aligned");
+        NIB_REQUIRE((((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0, "attention (8-bit cache): the pools must be 16-byte aligned");
 #define CALL(KERNEL, T, THREADS, SMEM, MOST)                                                                                    \
     do {                                                                                                                        \
         static const cudaError_t set = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MOST));  \

@@ -341,29 +341,36 @@ int launch_append(const void* qkv, void* q_out, const AppendArgs& a, cudaStream_
 
 }  // namespace
 
+// The arguments of a call come as one block of memory (a call of thirty arguments costs the host ten microseconds to marshal).
+struct NibAppendInt8 {
+    const void* qkv; void* q_out; const int* positions; const int* q_start; const int* ctx_lens; const float* cos_t; const float* sin_t;
+    const int* block_table; void* k_pages; void* v_pages; float* k_scales; float* v_scales;
+    int q_stride, out_stride, n_req, units, table_rows, rot, bt_stride, bt_width, page_size, num_pages, m, heads, kv_heads, head_dim, dtype, pad;
+};
+
 // Rotates the queries of the rows [q heads | k heads | v heads] of ``qkv`` (row stride q_stride elements) into ``q_out`` (row
 // stride out_stride; may be qkv itself), and appends the rotated keys and the values to the 8-bit pages. ``units``: the sum over
 // the requests of (q_len + page_size - 2) / page_size + 1.
-NIB_API int nib_rope_store_int8(const void* qkv, int q_stride, void* q_out, int out_stride, const int* positions, const int* q_start,
-                                const int* ctx_lens, int n_req, int units, const float* cos_t, const float* sin_t, int table_rows, int rot,
-                                const int* block_table, int bt_stride, int bt_width, int page_size, void* k_pages, void* v_pages,
-                                float* k_scales, float* v_scales, int num_pages, int m, int heads, int kv_heads, int head_dim, int dtype,
-                                cudaStream_t stream) {
-    NIB_REQUIRE(m >= 0 && n_req >= 0 && units >= 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && page_size > 0 && num_pages > 0, "rope_store_int8: bad sizes");
-    NIB_REQUIRE(rot >= 0 && rot <= head_dim && rot % 2 == 0, "rope_store_int8: rotated width %d must be even and <= head_dim %d", rot, head_dim);
-    NIB_REQUIRE(rot == 0 || (cos_t && sin_t && table_rows > 0), "rope_store_int8: a rotated width without tables");
-    NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "rope_store_int8: unknown dtype %d", dtype);
-    if (m == 0) return 0;
-    AppendArgs a{positions, q_start, ctx_lens, cos_t, sin_t, block_table, (signed char*)k_pages, (signed char*)v_pages, k_scales, v_scales,
-                 table_rows, rot, bt_stride, bt_width, page_size, num_pages, m, n_req, heads, kv_heads, head_dim, q_stride, out_stride, units, 0};
-    const long long jobs = (long long)units * 2 * kv_heads;
+NIB_API int nib_rope_store_int8(const void* args, cudaStream_t stream) {
+    NibAppendInt8 c;
+    memcpy(&c, args, sizeof c);
+    NIB_REQUIRE(c.m >= 0 && c.n_req >= 0 && c.units >= 0 && c.heads > 0 && c.kv_heads > 0 && c.head_dim > 0 && c.page_size > 0 && c.num_pages > 0,
+                "rope_store_int8: bad sizes");
+    NIB_REQUIRE(c.rot >= 0 && c.rot <= c.head_dim && c.rot % 2 == 0, "rope_store_int8: rotated width %d must be even and <= head_dim %d", c.rot, c.head_dim);
+    NIB_REQUIRE(c.rot == 0 || (c.cos_t && c.sin_t && c.table_rows > 0), "rope_store_int8: a rotated width without tables");
+    NIB_REQUIRE(c.dtype == NIB_F32 || c.dtype == NIB_BF16, "rope_store_int8: unknown dtype %d", c.dtype);
+    if (c.m == 0) return 0;
+    AppendArgs a{c.positions, c.q_start, c.ctx_lens, c.cos_t, c.sin_t, c.block_table, (signed char*)c.k_pages, (signed char*)c.v_pages, c.k_scales,
+                 c.v_scales, c.table_rows, c.rot, c.bt_stride, c.bt_width, c.page_size, c.num_pages, c.m, c.n_req, c.heads, c.kv_heads, c.head_dim,
+                 c.q_stride, c.out_stride, c.units, 0};
+    const long long jobs = (long long)c.units * 2 * c.kv_heads;
     NIB_REQUIRE(jobs < (1LL << 31) - KV_WARPS, "rope_store_int8: too many pages for one launch");
     a.kv_blocks = (int)((jobs + KV_WARPS - 1) / KV_WARPS);
-    const int esize = dtype == NIB_F32 ? 4 : 2;
-    const bool wide = (rot / 2) % 4 == 0 && head_dim % 4 == 0 && q_stride % 4 == 0 && ((uintptr_t)qkv) % (4 * esize) == 0 &&
-                      (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15) == 0 && (((uintptr_t)k_pages | (uintptr_t)v_pages) & 3) == 0;
-    if (dtype == NIB_F32) return wide ? launch_append<float, 4>(qkv, q_out, a, stream) : launch_append<float, 1>(qkv, q_out, a, stream);
-    return wide ? launch_append<__nv_bfloat16, 4>(qkv, q_out, a, stream) : launch_append<__nv_bfloat16, 1>(qkv, q_out, a, stream);
+    const int esize = c.dtype == NIB_F32 ? 4 : 2;
+    const bool wide = (c.rot / 2) % 4 == 0 && c.head_dim % 4 == 0 && c.q_stride % 4 == 0 && ((uintptr_t)c.qkv) % (4 * esize) == 0 &&
+                      (((uintptr_t)c.cos_t | (uintptr_t)c.sin_t) & 15) == 0 && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 3) == 0;
+    if (c.dtype == NIB_F32) return wide ? launch_append<float, 4>(c.qkv, c.q_out, a, stream) : launch_append<float, 1>(c.qkv, c.q_out, a, stream);
+    return wide ? launch_append<__nv_bfloat16, 4>(c.qkv, c.q_out, a, stream) : launch_append<__nv_bfloat16, 1>(c.qkv, c.q_out, a, stream);
 }
 
 // out = codes * scale for ``blocks`` blocks of ``per_block`` codes each.

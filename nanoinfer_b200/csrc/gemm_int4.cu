@@ -278,24 +278,30 @@ bool fits(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || gr
 
 }  // namespace
 
-// 1 if the product of few tokens takes these operands: at most 64 tokens, rows of 16-byte aligned activations; a gated product's halves
-// are whole row tiles.
-NIB_API int nib_gemm_int4_supported(const void* x, int tokens, int n, int k, int ldx, int group, int dual) {
-    return tokens <= 64 && fits(n, k, group) && ldx % 8 == 0 && ((uintptr_t)x & 15) == 0 && (!dual || n % 16 == 0);
-}
+// The arguments of a product, one block of memory.
+struct NibGemmInt4 {
+    const void* x; const void* w; const void* scales; const float* bias; void* out;
+    int tokens, n, k, group, ldx, ldo, epi, sms;        // sms: SMs of the device
+    float alpha, limit, shift;                          // the constants of EPI_GLU
+    int pad;
+};
 
-// out[tokens, n] from the packed weights of n rows (of 2 n rows, gate then up, for the gated epilogues). sms: SMs of the device.
-NIB_API int nib_gemm_int4(const void* x, const void* w, const void* scales, const float* bias, void* out, int tokens, int n, int k, int group,
-                          int ldx, int ldo, int epi, const float* glu, int sms, cudaStream_t stream) {
+// out[tokens, n] from the packed weights of n rows (of 2 n rows, gate then up, for the gated epilogues). -1, and nothing done, where
+// another product has to take these operands: more than 64 tokens, rows that do not begin on 16 bytes, a gated product whose halves
+// are not whole row tiles.
+NIB_API int nib_gemm_int4(const void* args, cudaStream_t stream) {
+    NibGemmInt4 c;
+    memcpy(&c, args, sizeof c);
+    const int tokens = c.tokens, n = c.n, k = c.k, group = c.group, epi = c.epi, sms = c.sms;
     const bool dual = epi_dual(epi);
-    NIB_REQUIRE(tokens >= 0 && nib_gemm_int4_supported(x, tokens, n, k, ldx, group, dual), "gemm_int4: %d tokens, %d x %d weights in groups of %d are not supported", tokens, n, k, group);
+    NIB_REQUIRE(tokens >= 0 && sms > 0 && fits(n, k, group), "gemm_int4: %d tokens, %d x %d weights in groups of %d are not supported", tokens, n, k, group);
     NIB_REQUIRE(epi == EPI_STORE || epi == EPI_ADD || epi == EPI_F32 || dual, "gemm_int4: unknown epilogue %d", epi);
-    NIB_REQUIRE(epi != EPI_GLU || glu, "gemm_int4: the gated product with constants needs them");
-    NIB_REQUIRE((((uintptr_t)w) & 15) == 0 && (((uintptr_t)scales) & 3) == 0, "gemm_int4: weights must be 16-byte aligned");
+    NIB_REQUIRE((((uintptr_t)c.w) & 15) == 0 && (((uintptr_t)c.scales) & 3) == 0, "gemm_int4: weights must be 16-byte aligned");
+    if (tokens > 64 || c.ldx % 8 != 0 || ((uintptr_t)c.x & 15) != 0 || (dual && n % 16 != 0)) return -1;
     if (tokens == 0) return 0;
     const int out_tiles = ceil_div(n, 16);
-    Args a{(const __nv_bfloat16*)x, (const uint4*)w, (const unsigned*)scales, bias, out, tokens, n, k, ldx, ldo, epi, dual ? 2 * out_tiles : out_tiles,
-           ceil_div(k, 64), group == 32 ? 5 : group == 64 ? 6 : 7, k / group, 1, glu ? NibGlu{glu[0], glu[1], glu[2]} : NibGlu{0.f, 0.f, 0.f}};
+    Args a{(const __nv_bfloat16*)c.x, (const uint4*)c.w, (const unsigned*)c.scales, c.bias, c.out, tokens, n, k, c.ldx, c.ldo, epi,
+           dual ? 2 * out_tiles : out_tiles, ceil_div(k, 64), group == 32 ? 5 : group == 64 ? 6 : 7, k / group, 1, NibGlu{c.alpha, c.limit, c.shift}};
     // Two row tiles a warp share the activations' loads; one where two would leave SMs without work.
     const bool two = dual || (tokens <= 32 && out_tiles >= 2 * WARPS * sms);
     const int units = dual || !two ? out_tiles : ceil_div(out_tiles, 2);

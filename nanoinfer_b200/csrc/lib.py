@@ -27,7 +27,17 @@ _DT = {torch.float32: 0, torch.bfloat16: 1}
 _EPI = {"store": 0, "add": 1, "f32": 2, "swiglu": 3, "glu": 5, "geglu": 6}
 _ADD = _EPI["add"]
 _DUAL = (3, 5, 6)       # the gated epilogues: two accumulators, gate rows and up rows
+# The arguments of calls that take them as one block of memory (NibAppendInt8, NibAttendInt8, NibGemmInt4)
+_APPEND_INT8, _ATTEND_INT8, _GEMM_INT4 = struct.Struct("=12Q16i"), struct.Struct("=10Q12ifi"), struct.Struct("=5Q8i3fi")
 _LAYOUT = {"interleaved": 0, "half": 1}     # which elements of a rotated vector make a pair
+
+
+# The current stream's handle. Torch's own look-up of it makes a stream object, which costs as much as a launch.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _current_stream() -> int:
+    return _raw_stream(torch.cuda.current_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _ptr(t: Optional[torch.Tensor]) -> c_void_p:
@@ -147,7 +157,7 @@ class Kernels:
                      "nib_decay_state_scan", "nib_decay_state_chunks_supported",
                      "nib_gemm_stream", "nib_gemm_stream_supported", "nib_gemm_stream_error", "nib_sample_rows", "nib_sample_rows_most",
                      "nib_rope_store_int8", "nib_unpack_int8", "nib_gather_int8", "nib_attention_int8_decode", "nib_attention_int8_decode_kind",
-                     "nib_gemm_int4", "nib_gemm_int4_supported", "nib_unpack_int4"):
+                     "nib_gemm_int4", "nib_unpack_int4"):
             getattr(self._lib, name).restype = c_int
         self.sample_rows_most = int(self._lib.nib_sample_rows_most())      # rows whose parameters a launch takes by value
         self._lib.nib_grouped_state_scratch.restype = self._lib.nib_decay_state_scratch.restype = c_longlong
@@ -217,7 +227,7 @@ class Kernels:
     def _stream(self) -> c_void_p:
         if self._bound_stream is not None:
             return self._bound_stream
-        return c_void_p(torch.cuda.current_stream().cuda_stream)
+        return c_void_p(_current_stream())
 
     def stream_scope(self):
         """Within the scope the kernels launch on the stream that is current at its start, looked up once: a
@@ -506,7 +516,7 @@ class Kernels:
             raise KernelError(f"linear_swiglu: no gated form with '{act}'" + (" and constants" if glu is not None else ""))
         epi = "geglu" if act == "gelu_tanh" else ("swiglu" if glu is None else "glu")
         if isinstance(w_gate_up, Int4Matrix):
-            self._linear_int4("linear_swiglu", a, w_gate_up, None, out, epi, _glu(glu))
+            self._linear_int4("linear_swiglu", a, w_gate_up, None, out, epi, glu)
             return
         if not isinstance(a, LazyNorm):
             _need(a, None, "swiglu a")
@@ -524,11 +534,18 @@ class Kernels:
         left by a second product."""
         if isinstance(a, LazyNorm):
             a = self._resolve(a, a.shape[0] <= 16)
-        self._rows_here(a, None, f"{what} a"); self._rows_here(out, None, f"{what} out"); _here(w.packed, torch.uint8, f"{what} w")
-        dual = _EPI[mode] in _DUAL
-        (m, k), n = a.shape, w.shape[0] // 2 if dual else w.shape[0]
-        if a.dtype not in _DT or w.shape[1] != k or (dual and 2 * n != w.shape[0]) or tuple(out.shape) != (m, n):
-            raise KernelError(f"{what}: shapes a{tuple(a.shape)} w{w.shape} out{tuple(out.shape)} do not fit")
+        device = torch.cuda.current_device()
+        for name, t in (("a", a), ("out", out), ("w", w.packed)):
+            if t.get_device() != device:
+                _here(t, None, f"{what} {name}", contiguous=False)
+        epi = _EPI[mode]
+        dual = epi in _DUAL
+        n = w.shape[0] // 2 if dual else w.shape[0]
+        if a.dim() != 2 or out.dim() != 2 or a.stride(1) != 1 or out.stride(1) != 1:
+            raise KernelError(f"{what}: rows must be dense")
+        m, k = a.shape
+        if a.dtype not in _DT or w.shape[1] != k or (dual and 2 * n != w.shape[0]) or out.shape != (m, n):
+            raise KernelError(f"{what}: shapes {a.dtype} a{tuple(a.shape)} w{w.shape} out{tuple(out.shape)} do not fit")
         if out.dtype != (torch.float32 if mode in ("add", "f32") else a.dtype):
             raise KernelError(f"{what}[{mode}]: out is {out.dtype}")
         if bias32 is not None:
@@ -537,18 +554,20 @@ class Kernels:
                 raise KernelError(f"{what}: {bias32.numel()} biases for {n} columns")
         if m == 0:
             return
-        if a.dtype == torch.bfloat16 and self._lib.nib_gemm_int4_supported(_ptr(a), c_int(m), c_int(n), c_int(k), c_int(a.stride(0)), c_int(w.group),
-                                                                          c_int(1 if dual else 0)) == 1:
+        if m <= 64 and a.dtype == torch.bfloat16:
             if not self.weights_ahead:
                 self._lib.nib_pdl_skip_next()
-            self._check(self._lib.nib_gemm_int4(_ptr(a), _ptr(w.packed), _ptr(w.scales), _ptr(bias32), _ptr(out), c_int(m), c_int(n), c_int(k),
-                                                c_int(w.group), c_int(a.stride(0)), c_int(out.stride(0)), c_int(_EPI[mode]), glu, c_int(self.sm_count),
-                                                self._stream()), "linear (4-bit weights)")
-            return
+            alpha, limit, shift = (0.0, 0.0, 0.0) if glu is None else glu
+            args = _GEMM_INT4.pack(a.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), 0 if bias32 is None else bias32.data_ptr(), out.data_ptr(), m, n, k,
+                                   w.group, a.stride(0), out.stride(0), epi, self.sm_count, alpha, limit, shift, 0)
+            rc = self._lib.nib_gemm_int4(args, self._stream())
+            if rc >= 0:
+                self._check(rc, "linear (4-bit weights)")
+                return
         plain = torch.empty(w.shape, dtype=a.dtype, device=a.device)
         self._unpack_int4(w, plain, 0)
         self._lib.nib_pdl_skip_next()           # the product may not read its weights ahead of the kernel that writes them
-        self._gemm(a, plain, bias32, out, m, n, k, _EPI[mode], glu)
+        self._gemm(a, plain, bias32, out, m, n, k, epi, _glu(glu))
         if a.dtype == torch.bfloat16 and mode in ("add", "f32") and not w.bf16_exact:
             self._unpack_int4(w, plain, 1)
             self._lib.nib_pdl_skip_next()
@@ -742,30 +761,31 @@ class Kernels:
                     c_int(heads), c_int(kv_heads), c_int(head_dim), c_float(scale), c_int(window), self._stream()),
                     "attention prefill")
 
-    # ---- the 8-bit cache of keys and values (cache_int8.cu) ----------------------------------------------------------------
+    # ---- the 8-bit cache of keys and values (cache_int8.cu, attention_int8.cu) ----------------------------------------------
     @staticmethod
-    def _cache_int8(what, kv_heads, page_size, head_dim, block_table, k_pages, v_pages, k_scales, v_scales) -> None:
-        """Refuses pools, scales or a block table that the kernels of the 8-bit cache cannot take."""
-        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-            _here(t, torch.int8, f"{what} {name}")
-            if tuple(t.shape[1:]) != (kv_heads, page_size, head_dim) or t.shape[0] != k_pages.shape[0] or t.shape[0] == 0:
-                raise KernelError(f"{what}: {name} {tuple(t.shape)} do not fit kv_heads/page_size/head_dim")
-        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-            _here(t, torch.float32, f"{what} {name}")
-            if t.numel() != k_pages.shape[0] * kv_heads:
-                raise KernelError(f"{what}: {name} {tuple(t.shape)} do not fit a scale for each page and kv head")
-        _here(block_table, torch.int32, f"{what} block_table", contiguous=False)
+    def _cache_int8(what, qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales) -> int:
+        """Refuses pools, scales, a block table or a step that the kernels of the 8-bit cache cannot take, or tensors of another device
+        than the current one; returns the number of the step's requests."""
+        device = torch.cuda.current_device()
+        for name, t, dtype in (("k_pages", k_pages, torch.int8), ("v_pages", v_pages, torch.int8), ("k_scales", k_scales, torch.float32),
+                               ("v_scales", v_scales, torch.float32), ("positions", ctx.positions, torch.int32), ("req_index", ctx.req_index, torch.int32),
+                               ("q_start", ctx.q_start, torch.int32), ("ctx_lens", ctx.ctx_lens, torch.int32)):
+            if t.get_device() != device or t.dtype != dtype or not t.is_contiguous():
+                _here(t, dtype, f"{what} {name}")
+        pages = k_pages.shape[0]
+        if pages == 0 or k_pages.shape != (pages, kv_heads, page_size, head_dim) or v_pages.shape != k_pages.shape:
+            raise KernelError(f"{what}: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} do not fit kv_heads/page_size/head_dim")
+        if k_scales.numel() != pages * kv_heads or v_scales.numel() != pages * kv_heads:
+            raise KernelError(f"{what}: scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}: one for each page and kv head")
+        if qkv.get_device() != device or block_table.get_device() != device or block_table.dtype != torch.int32:
+            _here(qkv, None, f"{what} qkv"); _here(block_table, torch.int32, f"{what} block_table", contiguous=False)
+        if qkv.dtype not in _DT or qkv.dim() != 2 or qkv.stride(1) != 1:
+            raise KernelError(f"{what}: dense rows of bfloat16 or float32, not {qkv.dtype} {tuple(qkv.shape)}")
         if block_table.dim() != 2 or block_table.stride(1) != 1:
             raise KernelError(f"{what}: block_table rows must be dense")
-
-    @staticmethod
-    def _step_requests(what, ctx, m, block_table) -> int:
-        """The number of requests of a step's context whose lengths fit ``m`` rows and the table."""
-        for name in ("positions", "req_index", "q_start", "ctx_lens"):
-            _here(getattr(ctx, name), torch.int32, f"{what} {name}")
-        n_req = len(ctx.host.q_lens)
-        if sum(ctx.host.q_lens) != m or ctx.positions.numel() < m or ctx.req_index.numel() < m or ctx.q_start.numel() != n_req + 1 or ctx.ctx_lens.numel() != n_req \
-                or block_table.shape[0] < n_req:
+        m, n_req = qkv.shape[0], len(ctx.host.q_lens)
+        if sum(ctx.host.q_lens) != m or ctx.positions.numel() < m or ctx.req_index.numel() < m or ctx.q_start.numel() != n_req + 1 \
+                or ctx.ctx_lens.numel() != n_req or block_table.shape[0] < n_req:
             raise KernelError(f"{what}: the step's lengths do not fit {m} rows and {block_table.shape[0]} rows of the block table")
         return n_req
 
@@ -779,69 +799,68 @@ class Kernels:
         the rounding to a larger scale, if a new token needs one; a page that the step begins anew forgets its old scale. A
         token whose key or value is not finite, or whose position the tables of ``rotary`` do not hold, makes its block's scale NaN.
         No two requests may append to the same page."""
-        self._cache_int8("rope_store_int8", kv_heads, page_size, head_dim, block_table, k_pages, v_pages, k_scales, v_scales)
-        self._rows_here(qkv, None, "rope_store_int8 qkv"); self._rows_here(q_out, qkv.dtype, "rope_store_int8 q_out")
-        m = qkv.shape[0]
-        if qkv.dtype not in _DT:
-            raise KernelError(f"rope_store_int8: rows of {qkv.dtype}")
-        if qkv.shape[1] != (heads + 2 * kv_heads) * head_dim or tuple(q_out.shape) != (m, heads * head_dim):
+        n_req = self._cache_int8("rope_store_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales)
+        m, device = qkv.shape[0], qkv.get_device()
+        if qkv.shape[1] != (heads + 2 * kv_heads) * head_dim or q_out.shape != (m, heads * head_dim):
             raise KernelError("rope_store_int8: widths do not fit the head counts")
-        n_req = self._step_requests("rope_store_int8", ctx, m, block_table)
-        cos = sin = None
-        rot = 0
+        if q_out.get_device() != device or q_out.dtype != qkv.dtype or q_out.stride(1) != 1:
+            raise KernelError(f"rope_store_int8: q_out is {q_out.dtype} on {q_out.device}, {qkv.dtype} in dense rows on {qkv.device} is wanted")
+        cos = sin = rot = rows = 0
         if rotary is not None:
-            cos, sin, rot = rotary
-            _here(cos, torch.float32, "cos"); _here(sin, torch.float32, "sin")
-            if cos.shape[1] != rot // 2 or sin.shape != cos.shape:
-                raise KernelError("rope_store_int8: table width must be rot/2")
+            cos_t, sin_t, rot = rotary
+            if cos_t.get_device() != device or sin_t.get_device() != device or cos_t.dtype != torch.float32 or sin_t.dtype != torch.float32 \
+                    or not cos_t.is_contiguous() or not sin_t.is_contiguous() or cos_t.dim() != 2 or cos_t.shape[1] != rot // 2 or sin_t.shape != cos_t.shape:
+                raise KernelError("rope_store_int8: the tables are dense float32 [positions, rot/2] on the device of the rows")
+            cos, sin, rows = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0]
         units = sum((n + page_size - 2) // page_size + 1 for n in ctx.host.q_lens)
-        self._check(self._lib.nib_rope_store_int8(
-            _ptr(qkv), c_int(qkv.stride(0)), _ptr(q_out), c_int(q_out.stride(0)), _ptr(ctx.positions), _ptr(ctx.q_start), _ptr(ctx.ctx_lens),
-            c_int(n_req), c_int(units), _ptr(cos), _ptr(sin), c_int(0 if cos is None else cos.shape[0]), c_int(rot), _ptr(block_table),
-            c_int(block_table.stride(0)), c_int(block_table.shape[1]), c_int(page_size), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales),
-            _ptr(v_scales), c_int(k_pages.shape[0]), c_int(m), c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(_DT[qkv.dtype]),
-            self._stream()), "rope_store (8-bit cache)")
+        args = _APPEND_INT8.pack(
+            qkv.data_ptr(), q_out.data_ptr(), ctx.positions.data_ptr(), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), cos, sin, block_table.data_ptr(),
+            k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), qkv.stride(0), q_out.stride(0), n_req, units, rows, rot,
+            block_table.stride(0), block_table.shape[1], page_size, k_pages.shape[0], m, heads, kv_heads, head_dim, _DT[qkv.dtype], 0)
+        self._check(self._lib.nib_rope_store_int8(args, self._stream()), "rope_store (8-bit cache)")
 
     def unpack_int8(self, pages, scales, out):
         """out = what the codes of a pool stand for: ``pages`` int8 [pages, kv_heads, page_size, head_dim], ``scales`` a float for each
         page and kv head, ``out`` of the pool's shape in bfloat16 or float32 (both hold the values exactly)."""
-        _here(pages, torch.int8, "unpack_int8 pages"); _here(scales, torch.float32, "unpack_int8 scales"); _here(out, None, "unpack_int8 out")
+        device = torch.cuda.current_device()
+        for name, t, dtype in (("pages", pages, torch.int8), ("scales", scales, torch.float32), ("out", out, out.dtype)):
+            if t.get_device() != device or t.dtype != dtype or not t.is_contiguous():
+                _here(t, dtype, f"unpack_int8 {name}")
         if pages.dim() != 4 or scales.numel() != pages.shape[0] * pages.shape[1] or out.shape != pages.shape or out.dtype not in _DT:
             raise KernelError(f"unpack_int8: pages {tuple(pages.shape)}, scales {tuple(scales.shape)} and {out.dtype} {tuple(out.shape)} do not fit")
         if pages.numel() == 0:
             return
-        self._check(self._lib.nib_unpack_int8(_ptr(pages), _ptr(scales), _ptr(out), c_longlong(scales.numel()), c_int(pages.shape[2] * pages.shape[3]),
-                                              c_int(_DT[out.dtype]), self._stream()), "unpack (8-bit cache)")
+        self._check(self._lib.nib_unpack_int8(_ptr(pages), _ptr(scales), _ptr(out), c_longlong(scales.numel()), pages.shape[2] * pages.shape[3],
+                                              _DT[out.dtype], self._stream()), "unpack (8-bit cache)")
 
     def attention_int8(self, qkv, out, heads, kv_heads, head_dim, scale, window, ctx, block_table, page_size, k_pages, v_pages, k_scales, v_scales):
         """``attention`` over the 8-bit cache that ``rope_store_int8`` fills: the rotated queries are the first columns of the rows of
         ``qkv``, the step's own keys and values are in the pages already."""
-        self._cache_int8("attention_int8", kv_heads, page_size, head_dim, block_table, k_pages, v_pages, k_scales, v_scales)
-        self._rows_here(qkv, None, "attention_int8 qkv"); _here(out, qkv.dtype, "attention_int8 out")
-        m = qkv.shape[0]
-        if qkv.dtype not in _DT:
-            raise KernelError(f"attention_int8: rows of {qkv.dtype}")
-        if heads <= 0 or heads % kv_heads or qkv.shape[1] < heads * head_dim or tuple(out.shape) != (m, heads * head_dim) or window < 0:
+        n_req = self._cache_int8("attention_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales)
+        m, dtype = qkv.shape[0], _DT[qkv.dtype]
+        if heads <= 0 or heads % kv_heads or qkv.shape[1] < heads * head_dim or out.shape != (m, heads * head_dim) or window < 0:
             raise KernelError("attention_int8: widths do not fit the head counts")
-        n_req = self._step_requests("attention_int8", ctx, m, block_table)
+        if out.get_device() != qkv.get_device() or out.dtype != qkv.dtype or not out.is_contiguous():
+            _here(out, qkv.dtype, "attention_int8 out")
         if m == 0:
             return
-        pages = (c_int(page_size), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), c_int(k_pages.shape[0]))
         n_dec, q_lens = 0, ctx.host.q_lens
-        kind = self._lib.nib_attention_int8_decode_kind(c_int(heads), c_int(kv_heads), c_int(head_dim), c_int(page_size), c_int(_DT[qkv.dtype]))
+        kind = self._lib.nib_attention_int8_decode_kind(heads, kv_heads, head_dim, page_size, dtype)
         while kind >= 0 and n_dec < n_req and q_lens[n_dec] == 1:
             n_dec += 1
         if n_dec:
             splits = self._decode_int8_splits(n_dec, kv_heads, max(ctx.host.ctx_lens[:n_dec]), window, kind, head_dim)
-            parts, part_o, part_ml = splits // 8, None, None
+            parts, part_o, part_ml = splits // 8, 0, 0
             if parts > 1:
-                part_o = torch.empty(n_dec * heads * parts * head_dim, dtype=torch.float32, device=qkv.device)
-                part_ml = torch.empty(n_dec * heads * parts * 2, dtype=torch.float32, device=qkv.device)
+                scratch = torch.empty(n_dec * heads * parts * (head_dim + 2), dtype=torch.float32, device=qkv.device)
+                part_o = scratch.data_ptr()
+                part_ml = part_o + 4 * n_dec * heads * parts * head_dim
                 self.launches += 1
-            self._check(self._lib.nib_attention_int8_decode(
-                _ptr(qkv), c_int(qkv.stride(0)), _ptr(out), _ptr(ctx.ctx_lens), _ptr(block_table), c_int(block_table.stride(0)),
-                c_int(block_table.shape[1]), *pages, c_int(n_dec), c_int(heads), c_int(kv_heads), c_int(head_dim), c_float(scale), c_int(window),
-                c_int(splits), _ptr(part_o), _ptr(part_ml), c_int(_DT[qkv.dtype]), self._stream()), "attention decode (8-bit cache)")
+            args = _ATTEND_INT8.pack(
+                qkv.data_ptr(), out.data_ptr(), ctx.ctx_lens.data_ptr(), block_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, qkv.stride(0), block_table.stride(0), block_table.shape[1], page_size,
+                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, splits, dtype, scale, 0)
+            self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
         if n_dec == n_req:
             return
         # The other requests' pages are read back once, in the order of their positions, and the prompt kernels run on them: a portion
@@ -851,10 +870,10 @@ class Kernels:
         values = torch.empty_like(keys)
         table = torch.empty((n_req, width), dtype=torch.int32, device=qkv.device)
         self._check(self._lib.nib_gather_int8(
-            pages[1], pages[2], pages[3], pages[4], _ptr(keys), _ptr(values), c_void_p(table.data_ptr() + 4 * n_dec * width),
+            _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(keys), _ptr(values), c_void_p(table.data_ptr() + 4 * n_dec * width),
             c_void_p(ctx.q_start.data_ptr() + 4 * n_dec), c_void_p(ctx.ctx_lens.data_ptr() + 4 * n_dec), c_int(n_rest),
             c_void_p(block_table.data_ptr() + 4 * n_dec * block_table.stride(0)), c_int(block_table.stride(0)), c_int(block_table.shape[1]),
-            pages[0], pages[5], c_int(kv_heads), c_int(head_dim), c_int(width), c_int(window), c_int(_DT[qkv.dtype]), self._stream()),
+            c_int(page_size), c_int(k_pages.shape[0]), c_int(kv_heads), c_int(head_dim), c_int(width), c_int(window), c_int(dtype), self._stream()),
             "gather (8-bit cache)")
         self._lib.nib_pdl_skip_next()       # the attention reads its table and earlier pages before its wait: here they are the kernel's before it
         self.attention(qkv, out, heads, kv_heads, head_dim, scale, window, ctx, table, 64, keys, values, first=n_dec)
@@ -935,13 +954,6 @@ class Kernels:
         return max(1, min(-(-tiles // 2), most, 64))
 
     # ---- row-wise and element-wise kernels that several designs share (pointwise.cu) -------------
-    @staticmethod
-    def _rows_here(t, dtype, what):
-        """``_rows`` of the current device."""
-        _here(t, dtype, what, contiguous=False)
-        if t.dim() != 2 or t.stride(1) != 1:
-            raise KernelError(f"{what}: rows must be dense")
-
     @staticmethod
     def _rows(t, dtype, what):
         """A matrix whose rows are dense but may lie apart (a slice of the columns of a wider one)."""
