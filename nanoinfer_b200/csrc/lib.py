@@ -28,7 +28,7 @@ _EPI = {"store": 0, "add": 1, "f32": 2, "swiglu": 3, "glu": 5, "geglu": 6}
 _ADD = _EPI["add"]
 _DUAL = (3, 5, 6)       # the gated epilogues: two accumulators, gate rows and up rows
 # The arguments of calls that take them as one block of memory (NibAppendInt8, NibAttendInt8, NibGemmInt4)
-_APPEND_INT8, _ATTEND_INT8, _GEMM_INT4 = struct.Struct("=12Q16i"), struct.Struct("=10Q12ifi"), struct.Struct("=5Q8i3fi")
+_APPEND_INT8, _ATTEND_INT8, _GEMM_INT4 = struct.Struct("=12Q16i"), struct.Struct("=10Q14ifi"), struct.Struct("=5Q8i3fi")
 _LAYOUT = {"interleaved": 0, "half": 1}     # which elements of a rotated vector make a pair
 
 
@@ -849,9 +849,9 @@ class Kernels:
         while kind >= 0 and n_dec < n_req and q_lens[n_dec] == 1:
             n_dec += 1
         if n_dec:
-            splits = self._decode_int8_splits(n_dec, kv_heads, max(ctx.host.ctx_lens[:n_dec]), window, kind, head_dim)
-            parts, part_o, part_ml = splits // 8, 0, 0
-            if parts > 1:
+            ctas, span, parts = self._decode_int8_split(n_dec, kv_heads, max(ctx.host.ctx_lens[:n_dec]), window, kind, head_dim)
+            part_o = part_ml = 0
+            if span:
                 scratch = torch.empty(n_dec * heads * parts * (head_dim + 2), dtype=torch.float32, device=qkv.device)
                 part_o = scratch.data_ptr()
                 part_ml = part_o + 4 * n_dec * heads * parts * head_dim
@@ -859,7 +859,7 @@ class Kernels:
             args = _ATTEND_INT8.pack(
                 qkv.data_ptr(), out.data_ptr(), ctx.ctx_lens.data_ptr(), block_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                 k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, qkv.stride(0), block_table.stride(0), block_table.shape[1], page_size,
-                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, splits, dtype, scale, 0)
+                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, ctas, span, parts, dtype, scale, 0)
             self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
         if n_dec == n_req:
             return
@@ -878,14 +878,22 @@ class Kernels:
         self._lib.nib_pdl_skip_next()       # the attention reads its table and earlier pages before its wait: here they are the kernel's before it
         self.attention(qkv, out, heads, kv_heads, head_dim, scale, window, ctx, table, 64, keys, values, first=n_dec)
 
-    def _decode_int8_splits(self, n_tokens: int, kv_heads: int, max_ctx: int, window: int, kind: int, head_dim: int) -> int:
-        """Into how many CTAs the keys of a decoding token are split over the 8-bit cache."""
-        if self.options.fixed_decode_splits:
-            return _cluster_splits(self.options.fixed_decode_splits)
-        keys = min(max_ctx, window) if window > 0 else max_ctx
-        cta_keys = 32 if kind == 0 else 256 if head_dim == 64 else 128          # a step of every warp
-        want = -(-2 * self.sm_count // max(1, n_tokens * kv_heads))
-        return _cluster_splits(max(1, min(want, -(-keys // cta_keys), 64)))
+    def _decode_int8_split(self, n_tokens: int, kv_heads: int, max_ctx: int, window: int, kind: int, head_dim: int):
+        """How the keys of decoding tokens over the 8-bit cache are cut: (CTAs of a cluster that share a row's keys, 0, 0), or (1, keys of a
+        span, the most spans of a row)."""
+        keys = max(1, min(max_ctx, window) if window > 0 else max_ctx)
+        units = max(1, n_tokens * kv_heads)
+        step = 32 if kind == 0 or head_dim == 64 else 16
+        cta_keys = step if kind == 0 else 4 * step          # a step of every warp
+        fixed = self.options.fixed_decode_splits
+        if not fixed and units * keys > 8 * 3 * self.sm_count * 256:
+            span = 512
+        elif fixed > 8:
+            span = -(-keys // (fixed * 32)) * 32
+        else:
+            want = fixed or min(8, -(-keys // cta_keys), max(1, 3 * self.sm_count // units))
+            return _cluster_splits(want), 0, 0
+        return 1, span, -(-keys // span) + 1        # (steps lie on absolute multiples: a window may touch one more)
 
     def attention_tc_error(self) -> int:
         """The error word of the tcgen05 attention's bounded waits (0 = none); synchronises and clears it."""
