@@ -10,10 +10,10 @@
 // count lie between 2^-125 and 2^106 (the 20 is what centres them).
 //
 // Two kernels. The one on the tensor cores takes heads of 64 and 128, at most 16 query heads a kv head and pages of a multiple of
-// 8 tokens; the general one takes any shape and 32-bit rows. The keys of a (token, kv head) are cut in one of two ways. Few rows: among
-// the CTAs of a cluster, which merge their partial (max, sum, output) through distributed shared memory and store the row. Many, or
-// long ones: into spans of equal length, a CTA each, whatever the contexts' lengths, merged in order by a second kernel (clusters of
-// eight find room on 15 places of the GPU at a time, and contexts of different lengths would keep SMs waiting).
+// 8 tokens; the general one takes any shape and 32-bit rows. The keys are dealt out in one of two ways. Few rows: those of a (token, kv
+// head) among the CTAs of a cluster, which merge their partial (max, sum, output) through distributed shared memory and store the row.
+// Many, or long ones: the chunks of all rows, in order, in equal shares to as many CTAs as find room at a time, whatever the lengths
+// are; a row that lies within one CTA's share is stored, the others' parts are merged in order by a second kernel.
 #include "attention_common.cuh"
 #include "pipeline.cuh"
 #include <cuda_fp16.h>
@@ -27,9 +27,9 @@ constexpr float LIFT = 20.f, UNLIFT = 0x1p-20f, RELIFT = 0x1p20f;
 
 struct Args {
     const int* ctx_lens; const int* block_table; const signed char* k_pages; const signed char* v_pages;
-    const float* k_scales; const float* v_scales; float* part_o; float* part_ml;
-    int q_stride, bt_stride, bt_width, page_size, shift, num_pages, heads, kv_heads, n_rep, head_dim, window;
-    int csize, span, parts;         // CTAs of a cluster and span 0; or 1, the keys of a span and the most spans a row has
+    const float* k_scales; const float* v_scales; float* part_o; float* part_ml;        // [2 * shares][n_rep][head_dim], [2 * shares][n_rep][2]
+    int q_stride, bt_stride, bt_width, page_size, shift, num_pages, n_tokens, heads, kv_heads, n_rep, head_dim, window;
+    int csize, shares;              // CTAs of a cluster and 0 shares, or the CTAs that all chunks are dealt to
     float scale;
 };
 
@@ -39,34 +39,102 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
-// The keys lo..p of a token, and of those the steps of ``step`` keys (aligned to absolute multiples) that are this CTA's.
-struct Range { int lo, p, begin, end; };
-__device__ __forceinline__ Range range_of(const Args& a, int token, int step) {
-    Range r;
-    r.p = a.ctx_lens[token] - 1;                            // the token's own position; -1: a padding row
-    r.lo = a.window > 0 ? max(0, r.p - a.window + 1) : 0;
-    const int first = r.lo / step, n = r.p >= 0 ? r.p / step - first + 1 : 0;
-    const int per = a.span ? a.span / step : (n + a.csize - 1) / a.csize;
-    r.begin = first + blockIdx.x * per;
-    r.end = min(first + n, r.begin + per);
-    return r;
+// The root of 2^(m - to), the factor of what is relative to m on the way to a larger reference. A sum is multiplied with it twice:
+// where scales differ by as much as they may, the factor itself is below 32 bits' range and the sum times it is not.
+__device__ __forceinline__ float half_factor(float m, float to) { return m == -INFINITY ? 0.f : exp2_ftz(0.5f * (m - to)); }
+
+// The keys lo..p of a token (p -1: a padding row) and the chunks of CH keys, aligned to absolute multiples, that hold them.
+template <int CH> struct Keys {
+    int lo, p, first, n;
+    __device__ __forceinline__ Keys(const Args& a, int token) {
+        p = __ldg(a.ctx_lens + token) - 1;
+        lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
+        first = lo / CH;
+        n = p >= 0 ? p / CH - first + 1 : 0;
+    }
+};
+
+// All rows' chunks in order: token by token, a token's kv heads one behind the other. A warp looks its place up together.
+template <int CH> __device__ __forceinline__ int all_chunks(const Args& a, int lane) {
+    int sum = 0;
+    for (int t = lane; t < a.n_tokens; t += 32) sum += Keys<CH>(a, t).n;
+    return __reduce_add_sync(0xffffffffu, sum) * a.kv_heads;
+}
+// The token whose chunks hold number ``at``, and the number of its first.
+template <int CH> __device__ __forceinline__ int token_at(const Args& a, int at, int& token_first, int lane) {
+    int base = 0;
+    for (int t0 = 0; t0 < a.n_tokens; t0 += 32) {
+        const int n = t0 + lane < a.n_tokens ? Keys<CH>(a, t0 + lane).n * a.kv_heads : 0;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const unsigned mine = __ballot_sync(0xffffffffu, at < base + sum);
+        if (mine) {
+            const int src = __ffs(mine) - 1;
+            token_first = base + __shfl_sync(0xffffffffu, sum - n, src);
+            return t0 + src;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    token_first = base;
+    return a.n_tokens;
 }
 
-// What a CTA leaves: its output, relative to its own maximum, in cta_o [n_rep][hd], its (max, sum) in cta_ml. With spans it is stored
-// for the kernel behind; in a cluster this CTA finishes its slice of the outputs. All threads take part.
-template <typename T>
-__device__ __forceinline__ void finish(const float* cta_o, const float* cta_ml, const Args& a, int hd, T* __restrict__ out, int threads) {
-    const size_t th0 = (size_t)blockIdx.y * a.heads + (size_t)blockIdx.z * a.n_rep;
-    const int total = a.n_rep * hd;
-    if (a.span) {
-        for (int i = threadIdx.x; i < total; i += threads) {
-            const int row = i / hd, d = i - row * hd;
-            a.part_o[((th0 + row) * a.parts + blockIdx.x) * hd + d] = cta_o[i];
+// A CTA's work, piece by piece: chunks begin..end of one (token, kv head), and the place of what they leave: -1 the output itself (or
+// the cluster's), else a part.
+template <int CH> struct Pieces {
+    int token, kvh, lo, p, begin, end, part;
+    int at, stop, per;
+    __device__ __forceinline__ bool first(const Args& a, int lane) {
+        if (a.shares == 0) {
+            token = blockIdx.y; kvh = blockIdx.z;
+            const Keys<CH> k(a, token);
+            lo = k.lo; p = k.p; part = -1;
+            const int share = (k.n + a.csize - 1) / a.csize;
+            begin = k.first + blockIdx.x * share;
+            end = min(k.first + k.n, begin + share);
+            at = stop = per = 0;
+            return true;
         }
-        for (int i = threadIdx.x; i < 2 * a.n_rep; i += threads) a.part_ml[((th0 + (i >> 1)) * a.parts + blockIdx.x) * 2 + (i & 1)] = cta_ml[i];
+        const int all = all_chunks<CH>(a, lane);
+        per = max(1, (all + a.shares - 1) / a.shares);
+        at = min(all, (int)blockIdx.x * per);
+        stop = min(all, at + per);
+        return look(a, lane);
+    }
+    __device__ __forceinline__ bool next(const Args& a, int lane) { return a.shares != 0 && look(a, lane); }
+private:
+    __device__ __forceinline__ bool look(const Args& a, int lane) {
+        if (at >= stop) return false;
+        int token_first;
+        token = token_at<CH>(a, at, token_first, lane);
+        const Keys<CH> k(a, token);
+        lo = k.lo; p = k.p;
+        kvh = (at - token_first) / k.n;
+        const int idx = at - token_first - kvh * k.n, n = min(k.n - idx, stop - at);
+        begin = k.first + idx;
+        end = begin + n;
+        part = n == k.n ? -1 : 2 * (int)blockIdx.x + (idx == 0 ? 1 : 0);
+        at += n;
+        return true;
+    }
+};
+
+// What a CTA leaves of a piece: its output, relative to its own maximum, in cta_o [n_rep][hd], its (max, sum) in cta_ml. All threads
+// take part, and all are behind a barrier.
+template <typename T>
+__device__ __forceinline__ void finish(const float* cta_o, const float* cta_ml, const Args& a, int token, int kvh, int part, int hd, T* __restrict__ out, int threads) {
+    const size_t th0 = (size_t)token * a.heads + (size_t)kvh * a.n_rep;
+    const int total = a.n_rep * hd;
+    if (part >= 0) {
+        for (int i = threadIdx.x; i < total; i += threads) a.part_o[(size_t)part * total + i] = cta_o[i];
+        for (int i = threadIdx.x; i < 2 * a.n_rep; i += threads) a.part_ml[(size_t)part * 2 * a.n_rep + i] = cta_ml[i];
         return;
     }
-    if (a.csize > 1) cluster_sync(); else __syncthreads();
+    if (a.csize > 1) cluster_sync();
     const int rank = a.csize > 1 ? (int)cluster_rank() : 0;
     const int slice = (total + a.csize - 1) / a.csize, end = min(total, (rank + 1) * slice);
     for (int i = rank * slice + threadIdx.x; i < end; i += threads) {
@@ -87,9 +155,9 @@ __device__ __forceinline__ void finish(const float* cta_o, const float* cta_ml, 
             for (int r = 0; r < 8; ++r) m_all = fmaxf(m_all, mr[r]);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                const float f = (mr[r] == -INFINITY) ? 0.f : exp2_ftz(mr[r] - m_all);
-                l_all += lr[r] * f;
-                acc += orr[r] * f;
+                const float f = half_factor(mr[r], m_all);
+                l_all += lr[r] * f * f;
+                acc += orr[r] * (f * f);
             }
         } else {
             l_all = cta_ml[row * 2 + 1];
@@ -100,38 +168,56 @@ __device__ __forceinline__ void finish(const float* cta_o, const float* cta_ml, 
     if (a.csize > 1) cluster_sync();        // nobody leaves while a peer may still read its shared memory
 }
 
-// Merges the spans of one (token, head), in order. grid: (heads, tokens). step: as the kernel before cut the keys.
-template <typename T>
-__global__ void __launch_bounds__(128)
-merge_int8_kernel(T* __restrict__ out, const Args a, int step) {
+// Merges the parts of the rows that lie in more than one share, in order, and stores the rows that see nothing. grid: (kv heads, tokens).
+template <typename T, int CH>
+__global__ void __launch_bounds__(256)
+merge_int8_kernel(T* __restrict__ out, const Args a) {
     pdl_wait();
     pdl_launch_dependents();
-    const int p = a.ctx_lens[blockIdx.y] - 1, lo = a.window > 0 ? max(0, p - a.window + 1) : 0, hd = a.head_dim;
-    const int steps = p >= 0 ? p / step - lo / step + 1 : 0, per = a.span / step;
-    const int parts = min(a.parts, (steps + per - 1) / per);
-    const size_t th = (size_t)blockIdx.y * a.heads + blockIdx.x;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + th * a.parts;
-    const float* po = a.part_o + th * a.parts * hd;
-    float m = -INFINITY;
-    for (int s = 0; s < parts; ++s) m = fmaxf(m, ml[s].x);
-    for (int d = threadIdx.x; d < hd; d += 128) {
-        float l = 0.f, acc = 0.f;
+    const int token = blockIdx.y, kvh = blockIdx.x, lane = threadIdx.x & 31, hd = a.head_dim;
+    const Keys<CH> k(a, token);
+    const int total = a.n_rep * hd;
+    T* rows = out + ((size_t)token * a.heads + (size_t)kvh * a.n_rep) * hd;
+    if (k.n == 0) {
+        for (int i = threadIdx.x; i < total; i += 256) Elem<T>::store(rows + i, 0.f);
+        return;
+    }
+    const int per = max(1, (all_chunks<CH>(a, lane) + a.shares - 1) / a.shares);
+    int before = 0;
+    for (int t = lane; t < token; t += 32) before += Keys<CH>(a, t).n;
+    const int begin = __reduce_add_sync(0xffffffffu, before) * a.kv_heads + kvh * k.n;
+    const int b0 = begin / per, parts = (begin + k.n - 1) / per - b0 + 1;
+    if (parts == 1) return;
+    for (int i = threadIdx.x; i < total; i += 256) {
+        const int row = i / hd;
+        auto place = [&](int s) { return (size_t)(s == 0 ? 2 * b0 + 1 : 2 * (b0 + s)); };
+        float m = -INFINITY, l = 0.f, acc = 0.f;
         for (int s0 = 0; s0 < parts; s0 += 8) {
             float v[8];
             float2 x[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const int s = min(s0 + u, parts - 1);
-                v[u] = po[(size_t)s * hd + d];
-                x[u] = ml[s];
+                const size_t at = place(min(s0 + u, parts - 1));
+                v[u] = a.part_o[at * total + i];
+                x[u] = *reinterpret_cast<const float2*>(a.part_ml + (at * a.n_rep + row) * 2);
             }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
+            const float f0 = half_factor(m, top);
+            l = l * f0 * f0;
+            acc *= f0 * f0;
+            m = top;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float f = s0 + u >= parts || x[u].x == -INFINITY ? 0.f : exp2_ftz(x[u].x - m);
-                if (s0 + u < parts) { l += x[u].y * f; acc += v[u] * f; }
+                if (s0 + u < parts) {
+                    const float f = half_factor(x[u].x, m);
+                    l += x[u].y * f * f;
+                    acc += v[u] * (f * f);
+                }
             }
         }
-        Elem<T>::store(out + th * hd + d, l == 0.f ? 0.f : acc / l * RELIFT);
+        Elem<T>::store(rows + i, l == 0.f ? 0.f : acc / l * RELIFT);
     }
 }
 
@@ -163,278 +249,314 @@ __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
     return *reinterpret_cast<const unsigned*>(&v);
 }
 
-// The codes of KU * 16 keys as a warp holds them: thread (g, t) has 16-byte pieces t, t + 4 of the key rows g and g + 8, and the
-// dims g * HD/8 .. of the value rows 2t, 2t + 1, 2t + 8, 2t + 9: every row of 64 or 128 bytes is read whole, by one instruction,
-// straight into the registers that the tensor core is fed from.
-template <int HD, int KU> struct Codes {
-    uint4 k[KU][2][HD / 64];
-    unsigned v[KU][4][HD / 32];
-    float ks[KU][2], vs[KU][2];         // of the rows 0..7 and 8..15
+template <int BYTES> __device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_async_or_zero(unsigned dst, const void* src, bool valid) {       // 4 bytes
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(unsigned at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(unsigned at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
+constexpr int STAGES = 3;           // steps of a warp on their way or being used
+
+template <int HD, int NH> struct Mma {
+    static constexpr int KU = HD == 64 ? 2 : 1, STEP = KU * 16, CHUNK = STEP * WARPS;
+    static constexpr int STAGE = STEP * HD * 2 + 64;        // keys, values, and (key, value) scales of every 8 keys
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int ROWS = NH * 8, MS = HD + 4;
+    static constexpr int MERGE = (WARPS * ROWS * (MS + 2) + ROWS * (HD + 2)) * 4;
+    static constexpr int BYTES = RING > MERGE ? RING : MERGE;
 };
 
+// A step of a warp is 16 (heads of 128) or 32 keys, 4 KB. Thread (g, t) uses the 16-byte pieces t, t + 4 of the key rows g and g + 8,
+// and the dims g * HD/8 .. of the value rows 2t, 2t + 1, 2t + 8, 2t + 9 of every 16 keys, and copies just these, asynchronously, into
+// places of its own: rows of 64 or 128 bytes are read whole by one instruction, shared memory is read without conflicts, and no
+// thread waits for another's copies.
+//
 // A key code enters the tensor core as the 16-bit number (code + 128) 2^-24, which is the code's byte, its first bit turned over, with
 // zeros before it; what the 128 adds to a score, 128 2^-24 sum of the head's elements, is what the accumulator begins at.
 // WHOLE: pages of a multiple of 16 tokens, so that 16 keys lie in one.
-template <int HD, int NH, int KU, bool WHOLE>
-__global__ void __launch_bounds__(WARPS * 32)
+template <int HD, int NH, bool WHOLE>
+__global__ void __launch_bounds__(WARPS * 32, NH == 1 ? 4 : 2)
 attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat16* __restrict__ out, const Args a) {
-    constexpr int STEP = KU * 16, MS = HD + 4, ROWS = NH * 8;
-    extern __shared__ __align__(16) float smem[];
-    const int token = blockIdx.y, kvh = blockIdx.z;
+    using C = Mma<HD, NH>;
+    constexpr int KU = C::KU, STEP = C::STEP, MS = C::MS, ROWS = C::ROWS, H = WHOLE ? 1 : 2, IDS = KU * H, ID_KEYS = 16 / H;
+    constexpr int V_AT = STEP * HD, S_AT = 2 * STEP * HD;
+    extern __shared__ __align__(16) unsigned char mma_smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const unsigned ring = smem_u32(mma_smem) + warp * STAGES * C::STAGE;
     pdl_wait();
     pdl_launch_dependents();
-    const Range range = range_of(a, token, STEP);
-    const int p = range.p, lo = range.lo, end = range.end;
-    if (a.span && range.begin >= end) return;               // (a shorter context than the longest one)
-    const int* bt = a.block_table + (size_t)token * a.bt_stride;
-    const long long page_bytes = (long long)a.kv_heads * a.page_size * HD;
-    const signed char* k_lane = a.k_pages + (size_t)kvh * a.page_size * HD + g * HD + t * 16;
-    const signed char* v_lane = a.v_pages + (size_t)kvh * a.page_size * HD + 2 * t * HD + g * (HD / 8);
+    Pieces<C::CHUNK> piece;
+    for (bool more = piece.first(a, lane); more; more = piece.next(a, lane)) {
+        const int token = piece.token, kvh = piece.kvh, p = piece.p, lo = piece.lo;
+        const int* bt = a.block_table + (size_t)token * a.bt_stride;
+        const long long page_bytes = (long long)a.kv_heads * a.page_size * HD;
+        const signed char* k_lane = a.k_pages + (size_t)kvh * a.page_size * HD + g * HD + t * 16;
+        const signed char* v_lane = a.v_pages + (size_t)kvh * a.page_size * HD + 2 * t * HD + g * (HD / 8);
 
-    // A page that the request does not hold is read as the pool's first with scales of 0: nothing leaves the pool.
-    auto load = [&](Codes<HD, KU>& c, int step) {
+        // The warp takes a step of every chunk. Lane i looks up the pages of its i-th step from here, 32 at a time.
+        int ids[IDS];
+        auto look_up = [&](int chunk) {
 #pragma unroll
-        for (int ku = 0; ku < KU; ++ku) {
-            int slot = 0, page = 0;
+            for (int i = 0; i < IDS; ++i) {
+                const int key = (chunk + lane) * C::CHUNK + warp * STEP + i * ID_KEYS;
+                int slot;
+                ids[i] = chunk + lane < piece.end && key <= p && key + ID_KEYS > lo ? page_at(a, bt, key, slot) : -1;
+            }
+        };
+        // A page that the request does not hold is read as the pool's first with scales of 0: nothing leaves the pool.
+        auto send = [&](int chunk, int stage) {
+            const unsigned dst = ring + stage * C::STAGE;
+            const int from = (chunk - piece.begin) & 31;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int key = step * STEP + ku * 16 + h * 8;
-                if (!WHOLE || h == 0) page = (key <= p && key + (WHOLE ? 16 : 8) > lo) ? page_at(a, bt, key, slot) : -1;
+            for (int i = 0; i < IDS; ++i) {
+                const int key = chunk * C::CHUNK + warp * STEP + i * ID_KEYS;
+                const int page = __shfl_sync(0xffffffffu, ids[i], from);
                 const bool held = page >= 0;
-                const int at_page = held ? page : 0, at_slot = (held ? slot : 0) + (WHOLE ? h * 8 : 0);
-                const long long at = at_page * page_bytes + at_slot * HD;
-                if (!WHOLE || h == 0) {
-                    const size_t block = (size_t)at_page * a.kv_heads + kvh;
-                    c.ks[ku][h] = __ldg(a.k_scales + block);
-                    c.vs[ku][h] = __ldg(a.v_scales + block);
-                    if (!held) c.ks[ku][h] = c.vs[ku][h] = 0.f;
-                } else {
-                    c.ks[ku][h] = c.ks[ku][0];
-                    c.vs[ku][h] = c.vs[ku][0];
+                const int slot = !held ? 0 : a.shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
+                const long long at = max(page, 0) * page_bytes + slot * HD;
+                if (lane < 2) {
+                    const size_t block = (size_t)max(page, 0) * a.kv_heads + kvh;
+                    copy_async_or_zero(dst + S_AT + i * 8 + lane * 4, (lane ? a.v_scales : a.k_scales) + block, held);
                 }
 #pragma unroll
-                for (int i = 0; i < HD / 64; ++i) c.k[ku][h][i] = __ldg(reinterpret_cast<const uint4*>(k_lane + at + i * 64));
+                for (int h = 0; h < 2 / H; ++h) {
+                    const int part = i * (2 / H) + h;               // 8 keys
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if constexpr (HD == 64) {
-                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(v_lane + at + j * HD));
-                        c.v[ku][2 * h + j][0] = x.x; c.v[ku][2 * h + j][1] = x.y;
-                    } else {
-                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(v_lane + at + j * HD));
-                        c.v[ku][2 * h + j][0] = x.x; c.v[ku][2 * h + j][1] = x.y;
-                        c.v[ku][2 * h + j][2] = x.z; c.v[ku][2 * h + j][3] = x.w;
-                    }
+                    for (int j = 0; j < HD / 64; ++j) copy_async<16>(dst + (part * (HD / 64) + j) * 512 + lane * 16, k_lane + at + h * 8 * HD + j * 64);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        copy_async<HD / 8>(dst + V_AT + (part * 2 + j) * (32 * HD / 8) + lane * (HD / 8), v_lane + at + (h * 8 + j) * HD);
                 }
             }
+        };
+        look_up(piece.begin);
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) {
+            if (piece.begin + i < piece.end) send(piece.begin + i, i);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
-    };
-    Codes<HD, KU> c[2];
-    int step = range.begin + warp;
-    if (step < end) load(c[0], step);
 
-    // Q^T as the column operand, its dims in the order in which the key rows' pieces hold them. A head is scaled by a power of two so
-    // that its largest element lies in 2^12 .. 2^13: 16-bit floats then hold every element that counts exactly.
-    unsigned qb[HD / 16][NH][2];
-    float factor[NH][2], bias[NH][2];
-#pragma unroll
-    for (int nh = 0; nh < NH; ++nh) {
-        const int head = nh * 8 + g;
-        const __nv_bfloat16* qp = q_rows + (size_t)token * a.q_stride + (size_t)(kvh * a.n_rep + head) * HD + t * 16;
-        unsigned raw[HD / 16][2], top = 0;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                raw[kk][j] = head < a.n_rep ? *reinterpret_cast<const unsigned*>(qp + (kk >> 2) * 64 + (kk & 3) * 4 + 2 * j) : 0u;
-                top = max(top, max(raw[kk][j] & 0x7fffu, (raw[kk][j] >> 16) & 0x7fffu));
-            }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the exponent field of the largest element: 2^(139 - e) takes it to 2^12 (in two factors: the power may leave the range)
-        const int e = (int)(top >> 7), up = (e == 0 || e == 255) ? 0 : 139 - e;
-        const float f1 = __uint_as_float((unsigned)(127 + up / 2) << 23), f2 = __uint_as_float((unsigned)(127 + up - up / 2) << 23);
-        float sum = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                qb[kk][nh][j] = pack_f16(__uint_as_float(raw[kk][j] << 16) * f1 * f2, __uint_as_float(raw[kk][j] & 0xffff0000u) * f1 * f2);
-                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&qb[kk][nh][j]));
-                sum += x.x + x.y;
-            }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        // 2^24 / 2^up, in factors that stay in range
-        const float mine = a.scale * LOG2E * __uint_as_float((unsigned)(127 - up / 2) << 23) * __uint_as_float((unsigned)(127 - (up - up / 2)) << 23) * 0x1p24f;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {           // of the heads 2t, 2t + 1
-            factor[nh][q] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * q);
-            bias[nh][q] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * q) * (-128.f * 0x1p-24f);
-        }
-    }
-
-    float o[HD / 16][NH][4], m_ref[NH][2], l_part[NH][2];
-#pragma unroll
-    for (int nh = 0; nh < NH; ++nh) {
-        m_ref[nh][0] = m_ref[nh][1] = -INFINITY;
-        l_part[nh][0] = l_part[nh][1] = 0.f;
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) o[d][nh][0] = o[d][nh][1] = o[d][nh][2] = o[d][nh][3] = 0.f;
-    }
-
-    auto compute = [&](const Codes<HD, KU>& c, int step) {
-        float s[KU][NH][4];
-        // S^T = K Q^T
-#pragma unroll
-        for (int ku = 0; ku < KU; ++ku) {
-#pragma unroll
-            for (int nh = 0; nh < NH; ++nh) { s[ku][nh][0] = s[ku][nh][2] = bias[nh][0]; s[ku][nh][1] = s[ku][nh][3] = bias[nh][1]; }
-#pragma unroll
-            for (int i = 0; i < HD / 64; ++i) {
-                const unsigned w0[4] = {c.k[ku][0][i].x, c.k[ku][0][i].y, c.k[ku][0][i].z, c.k[ku][0][i].w};
-                const unsigned w1[4] = {c.k[ku][1][i].x, c.k[ku][1][i].y, c.k[ku][1][i].z, c.k[ku][1][i].w};
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const unsigned u0 = w0[b] ^ 0x80808080u, u1 = w1[b] ^ 0x80808080u;
-                    const unsigned a0 = __byte_perm(u0, 0, 0x4140), a1 = __byte_perm(u1, 0, 0x4140), a2 = __byte_perm(u0, 0, 0x4342), a3 = __byte_perm(u1, 0, 0x4342);
-#pragma unroll
-                    for (int nh = 0; nh < NH; ++nh) mma_f16(s[ku][nh], a0, a1, a2, a3, qb[i * 4 + b][nh][0], qb[i * 4 + b][nh][1]);
-                }
-            }
-        }
-        // element e of a tile: key g + 8 * (e / 2), head 2t + (e & 1)
-        const int key0 = step * STEP + g;
-        const bool edge = step * STEP < lo || step * STEP + STEP - 1 > p;
-        float lv[KU][2], vs[KU][2];
-#pragma unroll
-        for (int ku = 0; ku < KU; ++ku)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                lv[ku][h] = WHOLE && h == 1 ? lv[ku][0] : reference_log2(c.vs[ku][h]);
-                vs[ku][h] = WHOLE && h == 1 ? vs[ku][0] : c.vs[ku][h] * UNLIFT;
-            }
+        // Q^T as the column operand, its dims in the order in which the key rows' pieces hold them. A head is scaled by a power of two
+        // so that its largest element lies in 2^12 .. 2^13: 16-bit floats then hold every element that counts exactly.
+        unsigned qb[HD / 16][NH][2];
+        float factor[NH][2], bias[NH][2];
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
-            float top[2] = {-INFINITY, -INFINITY};
+            const int head = nh * 8 + g;
+            const __nv_bfloat16* qp = q_rows + (size_t)token * a.q_stride + (size_t)(kvh * a.n_rep + head) * HD + t * 16;
+            unsigned raw[HD / 16][2], top = 0;
 #pragma unroll
-            for (int ku = 0; ku < KU; ++ku)
+            for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = s[ku][nh][e] * (factor[nh][e & 1] * c.ks[ku][e >> 1]);
-                    if (edge) {
-                        const int key = key0 + ku * 16 + 8 * (e >> 1);
-                        if (key < lo || key > p) v = -INFINITY;
-                    }
-                    s[ku][nh][e] = v;
-                    top[e & 1] = fmaxf(top[e & 1], v + lv[ku][e >> 1]);
+                for (int j = 0; j < 2; ++j) {
+                    raw[kk][j] = head < a.n_rep ? *reinterpret_cast<const unsigned*>(qp + (kk >> 2) * 64 + (kk & 3) * 4 + 2 * j) : 0u;
+                    top = max(top, max(raw[kk][j] & 0x7fffu, (raw[kk][j] >> 16) & 0x7fffu));
                 }
-            // the reference moves only where a key is 2^6 above it: p stays far inside 16 bits meanwhile
-            if (__any_sync(0xffffffffu, top[0] > m_ref[nh][0] + 6.f || top[1] > m_ref[nh][1] + 6.f)) {
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the exponent field e of the largest element: 2^(139 - e) takes it to 2^12 (in two factors: the power may leave the range)
+            const int e = (int)(top >> 7), up = (e == 0 || e == 255) ? 0 : 139 - e;
+            const float f1 = __uint_as_float((unsigned)(127 + up / 2) << 23), f2 = __uint_as_float((unsigned)(127 + up - up / 2) << 23);
+            float sum = 0.f;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 4));
-                    top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 8));
-                    top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 16));
-                    const float m_new = fmaxf(m_ref[nh][q], top[q]);
-                    const float corr = (m_ref[nh][q] == -INFINITY) ? 0.f : exp2_ftz(m_ref[nh][q] - m_new);
-                    m_ref[nh][q] = m_new;
-                    l_part[nh][q] *= corr;
+            for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
-                    for (int d = 0; d < HD / 16; ++d) { o[d][nh][q] *= corr; o[d][nh][2 + q] *= corr; }
+                for (int j = 0; j < 2; ++j) {
+                    qb[kk][nh][j] = pack_f16(__uint_as_float(raw[kk][j] << 16) * f1 * f2, __uint_as_float(raw[kk][j] & 0xffff0000u) * f1 * f2);
+                    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&qb[kk][nh][j]));
+                    sum += x.x + x.y;
+                }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            // 2^24 / 2^up, in factors that stay in range
+            const float mine = a.scale * LOG2E * __uint_as_float((unsigned)(127 - up / 2) << 23) * __uint_as_float((unsigned)(127 - (up - up / 2)) << 23) * 0x1p24f;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {           // of the heads 2t, 2t + 1
+                factor[nh][q] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * q);
+                bias[nh][q] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * q) * (-128.f * 0x1p-24f);
+            }
+        }
+
+        float o[HD / 16][NH][4], m_ref[NH][2], l_part[NH][2];
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+            m_ref[nh][0] = m_ref[nh][1] = -INFINITY;
+            l_part[nh][0] = l_part[nh][1] = 0.f;
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) o[d][nh][0] = o[d][nh][1] = o[d][nh][2] = o[d][nh][3] = 0.f;
+        }
+
+        int stage = 0, ahead = STAGES - 1;
+#pragma unroll 1
+        for (int chunk = piece.begin; chunk < piece.end; ++chunk) {
+            if (((chunk + STAGES - 1 - piece.begin) & 31) == 0) look_up(chunk + STAGES - 1);
+            if (chunk + STAGES - 1 < piece.end) send(chunk + STAGES - 1, ahead);
+            asm volatile("cp.async.commit_group;\ncp.async.wait_group %0;\n" ::"n"(STAGES - 1) : "memory");
+            __syncwarp();                           // (the scales are two lanes' copies)
+            const unsigned src = ring + stage * C::STAGE;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
+            float2 sc[IDS];
+#pragma unroll
+            for (int i = 0; i < IDS; ++i) {
+                const uint2 u = lds8(src + S_AT + i * 8);
+                sc[i] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+            }
+            float s[KU][NH][4];
+            // S^T = K Q^T
+#pragma unroll
+            for (int ku = 0; ku < KU; ++ku) {
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) { s[ku][nh][0] = s[ku][nh][2] = bias[nh][0]; s[ku][nh][1] = s[ku][nh][3] = bias[nh][1]; }
+#pragma unroll
+                for (int i = 0; i < HD / 64; ++i) {
+                    const uint4 r0 = lds16(src + ((ku * 2) * (HD / 64) + i) * 512 + lane * 16), r1 = lds16(src + ((ku * 2 + 1) * (HD / 64) + i) * 512 + lane * 16);
+                    const unsigned w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const unsigned u0 = w0[b] ^ 0x80808080u, u1 = w1[b] ^ 0x80808080u;
+                        const unsigned a0 = __byte_perm(u0, 0, 0x4140), a1 = __byte_perm(u1, 0, 0x4140), a2 = __byte_perm(u0, 0, 0x4342), a3 = __byte_perm(u1, 0, 0x4342);
+#pragma unroll
+                        for (int nh = 0; nh < NH; ++nh) mma_f16(s[ku][nh], a0, a1, a2, a3, qb[i * 4 + b][nh][0], qb[i * 4 + b][nh][1]);
+                    }
                 }
             }
+            // element e of a tile: key g + 8 * (e / 2), head 2t + (e & 1)
+            const int k0 = chunk * C::CHUNK + warp * STEP;
+            const bool edge = k0 < lo || k0 + STEP - 1 > p;
+            float lv[IDS], vs[IDS];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const float m_use = (m_ref[nh][q] == -INFINITY) ? 0.f : m_ref[nh][q] - LIFT;       // nothing visible yet: 2^(-inf - 0) = 0
+            for (int i = 0; i < IDS; ++i) { lv[i] = reference_log2(sc[i].y); vs[i] = sc[i].y * UNLIFT; }
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh) {
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int ku = 0; ku < KU; ++ku)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float w = exp2_ftz(s[ku][nh][2 * h + q] - m_use);
-                        l_part[nh][q] += w;
-                        float pv = w * vs[ku][h];
-                        if (edge && w == 0.f) pv = 0.f;             // (a hidden key's block may be undefined)
-                        s[ku][nh][2 * h + q] = pv;
+                    for (int e = 0; e < 4; ++e) {
+                        const int id = WHOLE ? ku : ku * 2 + (e >> 1);
+                        float v = s[ku][nh][e] * (factor[nh][e & 1] * sc[id].x);
+                        if (edge) {
+                            const int key = k0 + g + ku * 16 + 8 * (e >> 1);
+                            if (key < lo || key > p) v = -INFINITY;
+                        }
+                        s[ku][nh][e] = v;
+                        top[e & 1] = fmaxf(top[e & 1], v + lv[id]);
                     }
-            }
-        }
-        // O^T += V^T P^T
+                // the reference moves only where a key is 2^6 above it: p stays far inside 16 bits meanwhile
+                if (__any_sync(0xffffffffu, top[0] > m_ref[nh][0] + 6.f || top[1] > m_ref[nh][1] + 6.f)) {
 #pragma unroll
-        for (int ku = 0; ku < KU; ++ku) {
-            unsigned pb[NH][2];
+                    for (int q = 0; q < 2; ++q) {
+                        top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 4));
+                        top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 8));
+                        top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 16));
+                        const float m_new = fmaxf(m_ref[nh][q], top[q]);
+                        const float f = half_factor(m_ref[nh][q], m_new), corr = f * f;
+                        m_ref[nh][q] = m_new;
+                        l_part[nh][q] = l_part[nh][q] * f * f;
 #pragma unroll
-            for (int nh = 0; nh < NH; ++nh) {
-                pb[nh][0] = movmatrix_trans(pack_f16(s[ku][nh][0], s[ku][nh][1]));
-                pb[nh][1] = movmatrix_trans(pack_f16(s[ku][nh][2], s[ku][nh][3]));
-            }
+                        for (int d = 0; d < HD / 16; ++d) { o[d][nh][q] *= corr; o[d][nh][2 + q] *= corr; }
+                    }
+                }
 #pragma unroll
-            for (int w = 0; w < HD / 32; ++w) {             // four dims: two row tiles of V^T
-                const unsigned x0 = c.v[ku][0][w] ^ 0x80808080u, x1 = c.v[ku][1][w] ^ 0x80808080u;
-                const unsigned x2 = c.v[ku][2][w] ^ 0x80808080u, x3 = c.v[ku][3][w] ^ 0x80808080u;
-                const unsigned lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);      // dims 0, 1 and 2, 3 of two keys
-                const unsigned lo23 = __byte_perm(x2, x3, 0x5140), hi23 = __byte_perm(x2, x3, 0x7362);
-                const unsigned d0a = two_codes(lo01, 0x4140), d1a = two_codes(lo01, 0x4342), d0b = two_codes(lo23, 0x4140), d1b = two_codes(lo23, 0x4342);
-                const unsigned d2a = two_codes(hi01, 0x4140), d3a = two_codes(hi01, 0x4342), d2b = two_codes(hi23, 0x4140), d3b = two_codes(hi23, 0x4342);
+                for (int q = 0; q < 2; ++q) {
+                    const float m_use = (m_ref[nh][q] == -INFINITY) ? 0.f : m_ref[nh][q] - LIFT;       // nothing visible yet: 2^(-inf - 0) = 0
 #pragma unroll
-                for (int nh = 0; nh < NH; ++nh) {
-                    mma_f16(o[2 * w][nh], d0a, d1a, d0b, d1b, pb[nh][0], pb[nh][1]);
-                    mma_f16(o[2 * w + 1][nh], d2a, d3a, d2b, d3b, pb[nh][0], pb[nh][1]);
+                    for (int ku = 0; ku < KU; ++ku)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float w = exp2_ftz(s[ku][nh][2 * h + q] - m_use);
+                            l_part[nh][q] += w;
+                            float pv = w * vs[WHOLE ? ku : ku * 2 + h];
+                            if (edge && w == 0.f) pv = 0.f;             // (a hidden key's block may be undefined)
+                            s[ku][nh][2 * h + q] = pv;
+                        }
                 }
             }
-        }
-    };
-
-    while (step < end) {
+            // O^T += V^T P^T
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            if (step < end) {
-                if (step + WARPS < end) load(c[b ^ 1], step + WARPS);
-                compute(c[b], step);
-                step += WARPS;
+            for (int ku = 0; ku < KU; ++ku) {
+                unsigned pb[NH][2], v[4][HD / 32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned at = src + V_AT + (ku * 4 + j) * (32 * HD / 8) + lane * (HD / 8);
+                    if constexpr (HD == 64) { const uint2 u = lds8(at); v[j][0] = u.x; v[j][1] = u.y; }
+                    else { const uint4 u = lds16(at); v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w; }
+                }
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) {
+                    pb[nh][0] = movmatrix_trans(pack_f16(s[ku][nh][0], s[ku][nh][1]));
+                    pb[nh][1] = movmatrix_trans(pack_f16(s[ku][nh][2], s[ku][nh][3]));
+                }
+#pragma unroll
+                for (int w = 0; w < HD / 32; ++w) {             // four dims: two row tiles of V^T
+                    const unsigned x0 = v[0][w] ^ 0x80808080u, x1 = v[1][w] ^ 0x80808080u;
+                    const unsigned x2 = v[2][w] ^ 0x80808080u, x3 = v[3][w] ^ 0x80808080u;
+                    const unsigned lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);      // dims 0, 1 and 2, 3 of two keys
+                    const unsigned lo23 = __byte_perm(x2, x3, 0x5140), hi23 = __byte_perm(x2, x3, 0x7362);
+                    const unsigned d0a = two_codes(lo01, 0x4140), d1a = two_codes(lo01, 0x4342), d0b = two_codes(lo23, 0x4140), d1b = two_codes(lo23, 0x4342);
+                    const unsigned d2a = two_codes(hi01, 0x4140), d3a = two_codes(hi01, 0x4342), d2b = two_codes(hi23, 0x4140), d3b = two_codes(hi23, 0x4342);
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh) {
+                        mma_f16(o[2 * w][nh], d0a, d1a, d0b, d1b, pb[nh][0], pb[nh][1]);
+                        mma_f16(o[2 * w + 1][nh], d2a, d3a, d2b, d3b, pb[nh][0], pb[nh][1]);
+                    }
+                }
             }
+            __syncwarp();                           // the scales' places are free
         }
-    }
+        __syncthreads();                            // every warp is through with its copies: their room is used for the merge
 
-    // ---- merge the warps through shared memory
-    float* sm_o = smem;                                     // [WARPS][ROWS][MS]
-    float* sm_ml = sm_o + WARPS * ROWS * MS;                // [WARPS][ROWS][2]
-    float* cta_o = sm_ml + WARPS * ROWS * 2;                // [ROWS][HD]
-    float* cta_ml = cta_o + ROWS * HD;                      // [ROWS][2]
+        float* sm_o = reinterpret_cast<float*>(mma_smem);           // [WARPS][ROWS][MS]
+        float* sm_ml = sm_o + WARPS * ROWS * MS;                // [WARPS][ROWS][2]
+        float* cta_o = sm_ml + WARPS * ROWS * 2;                // [ROWS][HD]
+        float* cta_ml = cta_o + ROWS * HD;                      // [ROWS][2]
 #pragma unroll
-    for (int nh = 0; nh < NH; ++nh)
+        for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int row = warp * ROWS + nh * 8 + 2 * t + q;
-            float l = l_part[nh][q];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            for (int q = 0; q < 2; ++q) {
+                const int row = warp * ROWS + nh * 8 + 2 * t + q;
+                float l = l_part[nh][q];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d)           // row g of tile d is the dim g * HD/8 + 2d, row g + 8 the one behind it
-                *reinterpret_cast<float2*>(sm_o + row * MS + g * (HD / 8) + 2 * d) = make_float2(o[d][nh][q], o[d][nh][2 + q]);
-            if (g == 0) { sm_ml[row * 2] = m_ref[nh][q]; sm_ml[row * 2 + 1] = l; }
+                for (int d = 0; d < HD / 16; ++d)           // row g of tile d is the dim g * HD/8 + 2d, row g + 8 the one behind it
+                    *reinterpret_cast<float2*>(sm_o + row * MS + g * (HD / 8) + 2 * d) = make_float2(o[d][nh][q], o[d][nh][2 + q]);
+                if (g == 0) { sm_ml[row * 2] = m_ref[nh][q]; sm_ml[row * 2 + 1] = l; }
+            }
+        __syncthreads();
+        for (int i = tid; i < a.n_rep * HD; i += WARPS * 32) {
+            const int row = i / HD, d = i - row * HD;
+            float mw[WARPS], m_row = -INFINITY, acc = 0.f, l_row = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) { mw[w] = sm_ml[(w * ROWS + row) * 2]; m_row = fmaxf(m_row, mw[w]); }
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = half_factor(mw[w], m_row);
+                acc += sm_o[(w * ROWS + row) * MS + d] * (f * f);
+                l_row += sm_ml[(w * ROWS + row) * 2 + 1] * f * f;
+            }
+            cta_o[i] = acc;
+            if (d == 0) { cta_ml[row * 2] = m_row; cta_ml[row * 2 + 1] = l_row; }
         }
-    __syncthreads();
-    for (int i = tid; i < a.n_rep * HD; i += WARPS * 32) {
-        const int row = i / HD, d = i - row * HD;
-        float mw[WARPS], m_row = -INFINITY, acc = 0.f, l_row = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) { mw[w] = sm_ml[(w * ROWS + row) * 2]; m_row = fmaxf(m_row, mw[w]); }
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float f = (mw[w] == -INFINITY) ? 0.f : exp2_ftz(mw[w] - m_row);
-            acc += sm_o[(w * ROWS + row) * MS + d] * f;
-            l_row += sm_ml[(w * ROWS + row) * 2 + 1] * f;
-        }
-        cta_o[i] = acc;
-        if (d == 0) { cta_ml[row * 2] = m_row; cta_ml[row * 2 + 1] = l_row; }
+        __syncthreads();
+        finish(cta_o, cta_ml, a, token, kvh, piece.part, HD, out, WARPS * 32);
+        if (a.shares) __syncthreads();              // the next piece's copies go where this one's results are
     }
-    if (a.span) __syncthreads();
-    finish(cta_o, cta_ml, a, HD, out, WARPS * 32);
 }
-
-template <int HD, int NH> constexpr int mma_smem() { return (WARPS * NH * 8 * (HD + 4 + 2) + NH * 8 * (HD + 2)) * 4; }
 
 // ------------------------------------------------------------------------------------------ any shape
 // Tiles of 32 keys, as 32-bit values in shared memory: a thread has one (query head, key) of the scores at a time, then one
@@ -445,7 +567,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(GEN_THREADS)
 attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, const Args a) {
     extern __shared__ __align__(16) float smem[];
-    const int hd = a.head_dim, n_rep = a.n_rep, token = blockIdx.y, kvh = blockIdx.z, tid = threadIdx.x;
+    const int hd = a.head_dim, n_rep = a.n_rep, tid = threadIdx.x;
     const int ks_stride = VEC ? hd + 4 : hd | 1;        // (a warp's threads read 32 rows at the same column)
     float* kt = smem;                           // [GT][ks_stride]
     float* vt = kt + GT * ks_stride;            // [GT][hd]
@@ -458,16 +580,16 @@ attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, con
     __shared__ long long from[GT];              // where a key's codes are; -1: nowhere
     pdl_wait();
     pdl_launch_dependents();
-    const Range range = range_of(a, token, GT);
-    const int p = range.p, lo = range.lo;
-    if (a.span && range.begin >= range.end) return;
+    Pieces<GT> piece;
+    for (bool more = piece.first(a, tid & 31); more; more = piece.next(a, tid & 31)) {
+    const int token = piece.token, kvh = piece.kvh, p = piece.p, lo = piece.lo;
     const int* bt = a.block_table + (size_t)token * a.bt_stride;
     for (int i = tid; i < n_rep * hd; i += GEN_THREADS) {
         q[i] = Elem<T>::load(q_rows + (size_t)token * a.q_stride + (size_t)kvh * n_rep * hd + i) * (a.scale * LOG2E);
         cta_o[i] = 0.f;
     }
     for (int i = tid; i < n_rep; i += GEN_THREADS) { cta_ml[2 * i] = -INFINITY; cta_ml[2 * i + 1] = 0.f; }
-    for (int tile = range.begin; tile < range.end; ++tile) {
+    for (int tile = piece.begin; tile < piece.end; ++tile) {
         __syncthreads();
         if (tid < GT) {
             const int key = tile * GT + tid;
@@ -529,10 +651,10 @@ attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, con
             const float sum = warp_sum(e);
             __syncwarp();
             if (row == 0) {
-                const float c = m_old == -INFINITY ? 0.f : exp2f(m_old - m_new);
-                corr[h] = c;
+                const float f = half_factor(m_old, m_new);
+                corr[h] = f * f;
                 cta_ml[2 * h] = m_new;
-                cta_ml[2 * h + 1] = cta_ml[2 * h + 1] * c + sum;
+                cta_ml[2 * h + 1] = cta_ml[2 * h + 1] * f * f + sum;
             }
             w[i] = e == 0.f ? 0.f : e * (vs[row] * UNLIFT);
         }
@@ -546,16 +668,18 @@ attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, con
         }
     }
     __syncthreads();
-    finish(cta_o, cta_ml, a, hd, out, GEN_THREADS);
+    finish(cta_o, cta_ml, a, token, kvh, piece.part, hd, out, GEN_THREADS);
+    if (a.shares) __syncthreads();
+    }
 }
 
 long long any_smem(int n_rep, int hd) { return 4LL * (2LL * n_rep * hd + GT * (2LL * hd + 4) + n_rep * (GT + 3LL)); }
 constexpr long long MAX_SMEM = 226 * 1024;         // (and what a CTA has besides)
 
-template <typename T>
-int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int n_tokens, int step, int threads, long long smem, const void* q, void* out, cudaStream_t stream) {
+template <typename T, int CH>
+int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int threads, long long smem, const void* q, void* out, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.span ? a.parts : a.csize, n_tokens, a.kv_heads);
+    cfg.gridDim = a.shares ? dim3(a.shares) : dim3(a.csize, a.n_tokens, a.kv_heads);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
@@ -576,7 +700,7 @@ int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int n_tokens,
     cfg.attrs = attr;
     cfg.numAttrs = n;
     NIB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const T*)q, (T*)out, a));
-    if (a.span) NIB_CUDA(launch_pdl(merge_int8_kernel<T>, dim3(a.heads, n_tokens), dim3(128), (size_t)0, stream, (T*)out, a, step));
+    if (a.shares) NIB_CUDA(launch_pdl(merge_int8_kernel<T, CH>, dim3(a.kv_heads, a.n_tokens), dim3(256), (size_t)0, stream, (T*)out, a));
     return 0;
 }
 
@@ -593,13 +717,13 @@ NIB_API int nib_attention_int8_decode_kind(int heads, int kv_heads, int head_dim
 struct NibAttendInt8 {
     const void* q; void* out; const int* ctx_lens; const int* block_table; const void* k_pages; const void* v_pages; const float* k_scales;
     const float* v_scales; float* part_o; float* part_ml;
-    int q_stride, bt_stride, bt_width, page_size, num_pages, n_tokens, heads, kv_heads, head_dim, window, ctas, span, parts, dtype;
-    float scale; int pad;
+    int q_stride, bt_stride, bt_width, page_size, num_pages, n_tokens, heads, kv_heads, head_dim, window, ctas, shares, dtype, pad;
+    float scale; int pad2;
 };
 
 // Attention of n_tokens single tokens (token i is request i, at position ctx_lens[i] - 1) whose keys and values are in the pages.
-// ``span`` 0: the keys of a (token, kv head) are cut among ``ctas`` CTAs (1, 2, 4 or 8). Else a CTA takes ``span`` keys (a multiple of
-// 32) and a row has at most ``parts`` of them: part_o [tokens * heads * parts * head_dim], part_ml [tokens * heads * parts * 2].
+// ``shares`` 0: the keys of a (token, kv head) are cut among ``ctas`` CTAs (1, 2, 4 or 8). Else all rows' keys are dealt to that many
+// CTAs: part_o [2 * shares * heads/kv_heads * head_dim], part_ml [2 * shares * heads/kv_heads * 2].
 NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     NibAttendInt8 c;
     memcpy(&c, args, sizeof c);
@@ -610,8 +734,8 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "attention (8-bit cache): unknown dtype %d", dtype);
     const int kind = nib_attention_int8_decode_kind(heads, kv_heads, head_dim, page_size, dtype);
     NIB_REQUIRE(kind >= 0, "attention (8-bit cache): %d/%d heads of %d are not supported", heads, kv_heads, head_dim);
-    if (c.span) {
-        NIB_REQUIRE(c.ctas == 1 && c.span > 0 && c.span % 32 == 0 && c.parts > 0 && c.part_o && c.part_ml, "attention (8-bit cache): spans of a multiple of 32 keys, and scratch memory for them");
+    if (c.shares) {
+        NIB_REQUIRE(c.ctas == 1 && c.shares > 0 && c.part_o && c.part_ml, "attention (8-bit cache): shares need scratch memory");
     } else {
         NIB_REQUIRE(c.ctas == 1 || c.ctas == 2 || c.ctas == 4 || c.ctas == 8, "attention (8-bit cache): 1, 2, 4 or 8 CTAs share a row's keys, not %d", c.ctas);
     }
@@ -620,23 +744,24 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     int shift = -1;
     if ((page_size & (page_size - 1)) == 0) for (shift = 0; (1 << shift) < page_size;) ++shift;
     const Args a{c.ctx_lens, c.block_table, (const signed char*)c.k_pages, (const signed char*)c.v_pages, c.k_scales, c.v_scales, c.part_o, c.part_ml,
-                 c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, heads, kv_heads, heads / kv_heads, head_dim, c.window, c.ctas, c.span, c.parts, c.scale};
+                 c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, n_tokens, heads, kv_heads, heads / kv_heads, head_dim, c.window, c.ctas, c.shares, c.scale};
     int rc;
     if (kind == 1) {
         NIB_REQUIRE((((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0, "attention (8-bit cache): the pools must be 16-byte aligned");
-#define CALL(KERNEL, T, STEP, THREADS, SMEM, MOST)                                                                              \
+#define CALL(KERNEL, T, CH, THREADS, SMEM, MOST)                                                                                \
     do {                                                                                                                        \
         static const cudaError_t set = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MOST));  \
         NIB_CUDA(set);                                                                                                          \
-        rc = launch_rows<T>(KERNEL, a, n_tokens, STEP, THREADS, SMEM, q, out, stream);                                          \
+        rc = launch_rows<T, CH>(KERNEL, a, THREADS, SMEM, q, out, stream);                                                      \
     } while (0)
-#define MMA(HD, NH, KU)                                                                                                                              \
-    do {                                                                                                                                             \
-        if (page_size % 16 == 0) CALL((attention_int8_mma_kernel<HD, NH, KU, true>), __nv_bfloat16, KU * 16, WARPS * 32, (mma_smem<HD, NH>()), (mma_smem<HD, NH>())); \
-        else CALL((attention_int8_mma_kernel<HD, NH, KU, false>), __nv_bfloat16, KU * 16, WARPS * 32, (mma_smem<HD, NH>()), (mma_smem<HD, NH>()));      \
+#define MMA(HD, NH, WHOLE)                                                                                                      \
+    CALL((attention_int8_mma_kernel<HD, NH, WHOLE>), __nv_bfloat16, (Mma<HD, NH>::CHUNK), WARPS * 32, (Mma<HD, NH>::BYTES), (Mma<HD, NH>::BYTES))
+#define HEADS(NH)                                                                                       \
+    do {                                                                                                \
+        if (page_size % 16 == 0) { if (head_dim == 64) MMA(64, NH, true); else MMA(128, NH, true); }    \
+        else { if (head_dim == 64) MMA(64, NH, false); else MMA(128, NH, false); }                      \
     } while (0)
-        if (a.n_rep <= 8) { if (head_dim == 64) MMA(64, 1, 2); else MMA(128, 1, 1); }
-        else { if (head_dim == 64) MMA(64, 2, 2); else MMA(128, 2, 1); }
+        if (a.n_rep <= 8) HEADS(1); else HEADS(2);
     } else {
         const bool vec = head_dim % 16 == 0 && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0;
 #define ANY(T, VEC) CALL((attention_int8_any_kernel<T, VEC>), T, GT, GEN_THREADS, any_smem(a.n_rep, head_dim), MAX_SMEM)
@@ -644,6 +769,7 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
         else { if (vec) ANY(__nv_bfloat16, true); else ANY(__nv_bfloat16, false); }
 #undef ANY
     }
+#undef HEADS
 #undef MMA
 #undef CALL
     return rc;

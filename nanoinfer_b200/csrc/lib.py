@@ -849,17 +849,18 @@ class Kernels:
         while kind >= 0 and n_dec < n_req and q_lens[n_dec] == 1:
             n_dec += 1
         if n_dec:
-            ctas, span, parts = self._decode_int8_split(n_dec, kv_heads, max(ctx.host.ctx_lens[:n_dec]), window, kind, head_dim)
+            ctas, shares = self._decode_int8_split(n_dec, kv_heads, max(ctx.host.ctx_lens[:n_dec]), window, kind, head_dim)
             part_o = part_ml = 0
-            if span:
-                scratch = torch.empty(n_dec * heads * parts * (head_dim + 2), dtype=torch.float32, device=qkv.device)
+            if shares:
+                rows = 2 * shares * (heads // kv_heads)
+                scratch = torch.empty(rows * (head_dim + 2), dtype=torch.float32, device=qkv.device)
                 part_o = scratch.data_ptr()
-                part_ml = part_o + 4 * n_dec * heads * parts * head_dim
+                part_ml = part_o + 4 * rows * head_dim
                 self.launches += 1
             args = _ATTEND_INT8.pack(
                 qkv.data_ptr(), out.data_ptr(), ctx.ctx_lens.data_ptr(), block_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                 k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, qkv.stride(0), block_table.stride(0), block_table.shape[1], page_size,
-                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, ctas, span, parts, dtype, scale, 0)
+                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 0, scale, 0)
             self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
         if n_dec == n_req:
             return
@@ -879,21 +880,16 @@ class Kernels:
         self.attention(qkv, out, heads, kv_heads, head_dim, scale, window, ctx, table, 64, keys, values, first=n_dec)
 
     def _decode_int8_split(self, n_tokens: int, kv_heads: int, max_ctx: int, window: int, kind: int, head_dim: int):
-        """How the keys of decoding tokens over the 8-bit cache are cut: (CTAs of a cluster that share a row's keys, 0, 0), or (1, keys of a
-        span, the most spans of a row)."""
+        """How the keys of decoding tokens over the 8-bit cache are cut: (CTAs of a cluster that share a row's keys, 0), or (1, the CTAs that
+        all rows' keys are dealt to)."""
         keys = max(1, min(max_ctx, window) if window > 0 else max_ctx)
         units = max(1, n_tokens * kv_heads)
-        step = 32 if kind == 0 or head_dim == 64 else 16
-        cta_keys = step if kind == 0 else 4 * step          # a step of every warp
+        chunk = 32 if kind == 0 else 128 if head_dim == 64 else 64
+        chunks = -(-keys // chunk)
         fixed = self.options.fixed_decode_splits
-        if not fixed and units * keys > 8 * 3 * self.sm_count * 256:
-            span = 512
-        elif fixed > 8:
-            span = -(-keys // (fixed * 32)) * 32
-        else:
-            want = fixed or min(8, -(-keys // cta_keys), max(1, 3 * self.sm_count // units))
-            return _cluster_splits(want), 0, 0
-        return 1, span, -(-keys // span) + 1        # (steps lie on absolute multiples: a window may touch one more)
+        if fixed > 8 or (not fixed and units * chunks > 4 * self.sm_count):
+            return 1, min(4 * self.sm_count, units * (fixed or chunks))
+        return _cluster_splits(fixed or min(8, chunks, max(1, 4 * self.sm_count // units))), 0
 
     def attention_tc_error(self) -> int:
         """The error word of the tcgen05 attention's bounded waits (0 = none); synchronises and clears it."""
