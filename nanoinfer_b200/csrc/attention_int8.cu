@@ -168,48 +168,46 @@ __device__ __forceinline__ void finish(const float* cta_o, const float* cta_ml, 
     if (a.csize > 1) cluster_sync();        // nobody leaves while a peer may still read its shared memory
 }
 
-// Merges the parts of the rows that lie in more than one share, in order, and stores the rows that see nothing. grid: (kv heads, tokens).
+// Merges the parts of the rows that lie in more than one share, in order, and stores the rows that see nothing. grid: (heads, tokens).
+constexpr int MERGE_THREADS = 128;
+
 template <typename T, int CH>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(MERGE_THREADS)
 merge_int8_kernel(T* __restrict__ out, const Args a) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int token = blockIdx.y, kvh = blockIdx.x, lane = threadIdx.x & 31, hd = a.head_dim;
-    const Keys<CH> k(a, token);
-    const int total = a.n_rep * hd;
-    T* rows = out + ((size_t)token * a.heads + (size_t)kvh * a.n_rep) * hd;
-    if (k.n == 0) {
-        for (int i = threadIdx.x; i < total; i += 256) Elem<T>::store(rows + i, 0.f);
-        return;
+    const int token = blockIdx.y, head = blockIdx.x, kvh = head / a.n_rep, row = head - kvh * a.n_rep, lane = threadIdx.x & 31, hd = a.head_dim;
+    int all = 0, before = 0;                        // chunks of a kv head
+    for (int t = lane; t < a.n_tokens; t += 32) {
+        const int n = Keys<CH>(a, t).n;
+        all += n;
+        if (t < token) before += n;
     }
-    const int per = max(1, (all_chunks<CH>(a, lane) + a.shares - 1) / a.shares);
-    int before = 0;
-    for (int t = lane; t < token; t += 32) before += Keys<CH>(a, t).n;
-    const int begin = __reduce_add_sync(0xffffffffu, before) * a.kv_heads + kvh * k.n;
-    const int b0 = begin / per, parts = (begin + k.n - 1) / per - b0 + 1;
+    all = __reduce_add_sync(0xffffffffu, all) * a.kv_heads;
+    const int n = Keys<CH>(a, token).n, begin = __reduce_add_sync(0xffffffffu, before) * a.kv_heads + kvh * n;
+    const int per = max(1, (all + a.shares - 1) / a.shares), b0 = begin / per, parts = n ? (begin + n - 1) / per - b0 + 1 : 0;
+    pdl_wait();             // (the lengths are the step's inputs)
+    pdl_launch_dependents();
     if (parts == 1) return;
-    for (int i = threadIdx.x; i < total; i += 256) {
-        const int row = i / hd;
-        auto place = [&](int s) { return (size_t)(s == 0 ? 2 * b0 + 1 : 2 * (b0 + s)); };
+    for (int d = threadIdx.x; d < hd; d += MERGE_THREADS) {
         float m = -INFINITY, l = 0.f, acc = 0.f;
-        for (int s0 = 0; s0 < parts; s0 += 8) {
-            float v[8];
-            float2 x[8];
+        for (int s0 = 0; s0 < parts; s0 += 16) {
+            float v[16];
+            float2 x[16];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const size_t at = place(min(s0 + u, parts - 1));
-                v[u] = a.part_o[at * total + i];
-                x[u] = *reinterpret_cast<const float2*>(a.part_ml + (at * a.n_rep + row) * 2);
+            for (int u = 0; u < 16; ++u) {
+                const int s = min(s0 + u, parts - 1);
+                const size_t at = (size_t)(s == 0 ? 2 * b0 + 1 : 2 * (b0 + s)) * a.n_rep + row;
+                v[u] = a.part_o[at * hd + d];
+                x[u] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
             }
             float top = m;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
+            for (int u = 0; u < 16; ++u) top = fmaxf(top, x[u].x);
             const float f0 = half_factor(m, top);
             l = l * f0 * f0;
             acc *= f0 * f0;
             m = top;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
+            for (int u = 0; u < 16; ++u) {
                 if (s0 + u < parts) {
                     const float f = half_factor(x[u].x, m);
                     l += x[u].y * f * f;
@@ -217,7 +215,7 @@ merge_int8_kernel(T* __restrict__ out, const Args a) {
                 }
             }
         }
-        Elem<T>::store(rows + i, l == 0.f ? 0.f : acc / l * RELIFT);
+        Elem<T>::store(out + ((size_t)token * a.heads + head) * hd + d, l == 0.f ? 0.f : acc / l * RELIFT);
     }
 }
 
@@ -274,9 +272,23 @@ template <int HD, int NH> struct Mma {
     static constexpr int STAGE = STEP * HD * 2 + 64;        // keys, values, and (key, value) scales of every 8 keys
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int ROWS = NH * 8, MS = HD + 4;
-    static constexpr int MERGE = (WARPS * ROWS * (MS + 2) + ROWS * (HD + 2)) * 4;
-    static constexpr int BYTES = RING > MERGE ? RING : MERGE;
+    static constexpr int MERGE = WARPS * ROWS * (MS + 2) * 4;
+    static constexpr int OWN = RING > MERGE ? RING : MERGE;
+    static constexpr int BYTES = OWN + ROWS * HD * 4 + 8 * ROWS * 8 + 128;      // and what the cluster's CTAs send: slices of outputs, (max, sum)
+    static_assert(OWN % 16 == 0, "the slices are stored 16 bytes at a time");
 };
+
+__device__ __forceinline__ void st_peer_f32x4(unsigned addr, const float4& v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_peer_f32x2(unsigned addr, const float2& v) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};\n" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
+}
+__device__ __forceinline__ void store_row4(__nv_bfloat16* out, const float4& acc, float l) {
+    const float f = l == 0.f ? 0.f : RELIFT / l;            // a row that sees nothing is zero, an undefined one NaN
+    const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x * f, acc.y * f), b = __floats2bfloat162_rn(acc.z * f, acc.w * f);
+    *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
 
 // A step of a warp is 16 (heads of 128) or 32 keys, 4 KB. Thread (g, t) uses the 16-byte pieces t, t + 4 of the key rows g and g + 8,
 // and the dims g * HD/8 .. of the value rows 2t, 2t + 1, 2t + 8, 2t + 9 of every 16 keys, and copies just these, asynchronously, into
@@ -295,26 +307,40 @@ attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat1
     extern __shared__ __align__(16) unsigned char mma_smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const unsigned ring = smem_u32(mma_smem) + warp * STAGES * C::STAGE;
+    if (a.csize > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");       // this CTA is there: its peers may send
+    Pieces<C::CHUNK> piece;
+    // The warp takes a step of every chunk. Lane i looks up the pages of its i-th step from here, 32 at a time.
+    int ids[IDS];
+    auto look_up = [&](int chunk) {
+        const int* bt = a.block_table + (size_t)piece.token * a.bt_stride;
+#pragma unroll
+        for (int i = 0; i < IDS; ++i) {
+            const int key = (chunk + lane) * C::CHUNK + warp * STEP + i * ID_KEYS;
+            int slot;
+            ids[i] = chunk + lane < piece.end && key <= piece.p && key + ID_KEYS > piece.lo ? page_at(a, bt, key, slot) : -1;
+        }
+    };
+    bool more = piece.first(a, lane);
+    if (more) look_up(piece.begin);         // lengths and tables are the step's inputs; queries, keys, values and scales are kernels' results
     pdl_wait();
     pdl_launch_dependents();
-    Pieces<C::CHUNK> piece;
-    for (bool more = piece.first(a, lane); more; more = piece.next(a, lane)) {
+    while (more) {
         const int token = piece.token, kvh = piece.kvh, p = piece.p, lo = piece.lo;
-        const int* bt = a.block_table + (size_t)token * a.bt_stride;
+        unsigned raw[HD / 16][NH][2];           // the queries, as they are stored
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+            const int head = nh * 8 + g;
+            const __nv_bfloat16* qp = q_rows + (size_t)token * a.q_stride + (size_t)(kvh * a.n_rep + head) * HD + t * 16;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    raw[kk][nh][j] = head < a.n_rep ? *reinterpret_cast<const unsigned*>(qp + (kk >> 2) * 64 + (kk & 3) * 4 + 2 * j) : 0u;
+        }
         const long long page_bytes = (long long)a.kv_heads * a.page_size * HD;
         const signed char* k_lane = a.k_pages + (size_t)kvh * a.page_size * HD + g * HD + t * 16;
         const signed char* v_lane = a.v_pages + (size_t)kvh * a.page_size * HD + 2 * t * HD + g * (HD / 8);
 
-        // The warp takes a step of every chunk. Lane i looks up the pages of its i-th step from here, 32 at a time.
-        int ids[IDS];
-        auto look_up = [&](int chunk) {
-#pragma unroll
-            for (int i = 0; i < IDS; ++i) {
-                const int key = (chunk + lane) * C::CHUNK + warp * STEP + i * ID_KEYS;
-                int slot;
-                ids[i] = chunk + lane < piece.end && key <= p && key + ID_KEYS > lo ? page_at(a, bt, key, slot) : -1;
-            }
-        };
         // A page that the request does not hold is read as the pool's first with scales of 0: nothing leaves the pool.
         auto send = [&](int chunk, int stage) {
             const unsigned dst = ring + stage * C::STAGE;
@@ -341,7 +367,6 @@ attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat1
                 }
             }
         };
-        look_up(piece.begin);
 #pragma unroll
         for (int i = 0; i < STAGES - 1; ++i) {
             if (piece.begin + i < piece.end) send(piece.begin + i, i);
@@ -354,16 +379,11 @@ attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat1
         float factor[NH][2], bias[NH][2];
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
-            const int head = nh * 8 + g;
-            const __nv_bfloat16* qp = q_rows + (size_t)token * a.q_stride + (size_t)(kvh * a.n_rep + head) * HD + t * 16;
-            unsigned raw[HD / 16][2], top = 0;
+            unsigned top = 0;
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    raw[kk][j] = head < a.n_rep ? *reinterpret_cast<const unsigned*>(qp + (kk >> 2) * 64 + (kk & 3) * 4 + 2 * j) : 0u;
-                    top = max(top, max(raw[kk][j] & 0x7fffu, (raw[kk][j] >> 16) & 0x7fffu));
-                }
+                for (int j = 0; j < 2; ++j) top = max(top, max(raw[kk][nh][j] & 0x7fffu, (raw[kk][nh][j] >> 16) & 0x7fffu));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // the exponent field e of the largest element: 2^(139 - e) takes it to 2^12 (in two factors: the power may leave the range)
@@ -374,7 +394,7 @@ attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat1
             for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    qb[kk][nh][j] = pack_f16(__uint_as_float(raw[kk][j] << 16) * f1 * f2, __uint_as_float(raw[kk][j] & 0xffff0000u) * f1 * f2);
+                    qb[kk][nh][j] = pack_f16(__uint_as_float(raw[kk][nh][j] << 16) * f1 * f2, __uint_as_float(raw[kk][nh][j] & 0xffff0000u) * f1 * f2);
                     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&qb[kk][nh][j]));
                     sum += x.x + x.y;
                 }
@@ -519,42 +539,96 @@ attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat1
         }
         __syncthreads();                            // every warp is through with its copies: their room is used for the merge
 
+        // ---- the warps' results, relative to their common maximum, and their sums
         float* sm_o = reinterpret_cast<float*>(mma_smem);           // [WARPS][ROWS][MS]
-        float* sm_ml = sm_o + WARPS * ROWS * MS;                // [WARPS][ROWS][2]
-        float* cta_o = sm_ml + WARPS * ROWS * 2;                // [ROWS][HD]
-        float* cta_ml = cta_o + ROWS * HD;                      // [ROWS][2]
+        float2* sm_ml = reinterpret_cast<float2*>(sm_o + WARPS * ROWS * MS);            // [WARPS][ROWS]
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const int row = warp * ROWS + nh * 8 + 2 * t + q;
                 float l = l_part[nh][q];
                 l += __shfl_xor_sync(0xffffffffu, l, 4);
                 l += __shfl_xor_sync(0xffffffffu, l, 8);
                 l += __shfl_xor_sync(0xffffffffu, l, 16);
+                if (g == 0) sm_ml[warp * ROWS + nh * 8 + 2 * t + q] = make_float2(m_ref[nh][q], l);
+            }
+        __syncthreads();
+        auto whole_row = [&](int row) {
+            float2 x[WARPS], all = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) { x[w] = sm_ml[w * ROWS + row]; all.x = fmaxf(all.x, x[w].x); }
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) { const float f = half_factor(x[w].x, all.x); all.y += x[w].y * f * f; }
+            return all;
+        };
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int row = nh * 8 + 2 * t + q;
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_ml[w * ROWS + row].x);
+                const float f0 = half_factor(m_ref[nh][q], top), f = f0 * f0;
 #pragma unroll
                 for (int d = 0; d < HD / 16; ++d)           // row g of tile d is the dim g * HD/8 + 2d, row g + 8 the one behind it
-                    *reinterpret_cast<float2*>(sm_o + row * MS + g * (HD / 8) + 2 * d) = make_float2(o[d][nh][q], o[d][nh][2 + q]);
-                if (g == 0) { sm_ml[row * 2] = m_ref[nh][q]; sm_ml[row * 2 + 1] = l; }
+                    *reinterpret_cast<float2*>(sm_o + (warp * ROWS + row) * MS + g * (HD / 8) + 2 * d) = make_float2(o[d][nh][q] * f, o[d][nh][2 + q] * f);
             }
         __syncthreads();
-        for (int i = tid; i < a.n_rep * HD; i += WARPS * 32) {
-            const int row = i / HD, d = i - row * HD;
-            float mw[WARPS], m_row = -INFINITY, acc = 0.f, l_row = 0.f;
+        const int quads = a.n_rep * (HD / 4);
+        auto sum_of = [&](int i) {
+            const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
+            float4 s = *reinterpret_cast<const float4*>(sm_o + row * MS + d);
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) { mw[w] = sm_ml[(w * ROWS + row) * 2]; m_row = fmaxf(m_row, mw[w]); }
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float f = half_factor(mw[w], m_row);
-                acc += sm_o[(w * ROWS + row) * MS + d] * (f * f);
-                l_row += sm_ml[(w * ROWS + row) * 2 + 1] * f * f;
+            for (int w = 1; w < WARPS; ++w) {
+                const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + row) * MS + d);
+                s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
             }
-            cta_o[i] = acc;
-            if (d == 0) { cta_ml[row * 2] = m_row; cta_ml[row * 2 + 1] = l_row; }
+            return s;
+        };
+        __nv_bfloat16* rows = out + ((size_t)token * a.heads + (size_t)kvh * a.n_rep) * HD;
+        if (piece.part >= 0) {
+            float4* to = reinterpret_cast<float4*>(a.part_o) + (size_t)piece.part * quads;
+            for (int i = tid; i < quads; i += WARPS * 32) to[i] = sum_of(i);
+            if (tid < a.n_rep) reinterpret_cast<float2*>(a.part_ml)[(size_t)piece.part * a.n_rep + tid] = whole_row(tid);
+        } else if (a.csize == 1) {
+            for (int i = tid; i < quads; i += WARPS * 32) store_row4(rows + i * 4, sum_of(i), whole_row(i / (HD / 4)).y);
+        } else {
+            // every CTA of the cluster finishes a slice: the others send it theirs, and the (max, sum) of all rows
+            const int rank = (int)cluster_rank(), slice = (quads + a.csize - 1) / a.csize;
+            float4* recv = reinterpret_cast<float4*>(mma_smem + C::OWN);               // [csize][slice]
+            float2* recv_ml = reinterpret_cast<float2*>(mma_smem + C::OWN + ROWS * HD * 4 + 128);         // [csize][n_rep]
+            asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");               // every CTA is there
+            for (int i = tid; i < quads; i += WARPS * 32) {
+                const int to = i / slice;
+                st_peer_f32x4(peer_smem(recv + rank * slice + (i - to * slice), to), sum_of(i));
+            }
+            if (tid < a.n_rep) {
+                const float2 ml = whole_row(tid);
+                for (int r = 0; r < a.csize; ++r) st_peer_f32x2(peer_smem(recv_ml + rank * a.n_rep + tid, r), ml);
+            }
+            cluster_sync();
+            const int end = min(quads, (rank + 1) * slice);
+            for (int i = rank * slice + tid; i < end; i += WARPS * 32) {
+                const int row = i / (HD / 4);
+                float top = -INFINITY, l = 0.f;
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int r = 0; r < a.csize; ++r) top = fmaxf(top, recv_ml[r * a.n_rep + row].x);
+                for (int r = 0; r < a.csize; ++r) {
+                    const float2 ml = recv_ml[r * a.n_rep + row];
+                    const float4 x = recv[r * slice + (i - rank * slice)];
+                    const float f0 = half_factor(ml.x, top), f = f0 * f0;
+                    l += ml.y * f0 * f0;
+                    acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+                }
+                store_row4(rows + i * 4, acc, l);
+            }
         }
-        __syncthreads();
-        finish(cta_o, cta_ml, a, token, kvh, piece.part, HD, out, WARPS * 32);
-        if (a.shares) __syncthreads();              // the next piece's copies go where this one's results are
+        more = piece.next(a, lane);
+        if (more) {
+            __syncthreads();                        // the next piece's copies go where this one's results are
+            look_up(piece.begin);
+        }
     }
 }
 
@@ -700,7 +774,7 @@ int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int threads, 
     cfg.attrs = attr;
     cfg.numAttrs = n;
     NIB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const T*)q, (T*)out, a));
-    if (a.shares) NIB_CUDA(launch_pdl(merge_int8_kernel<T, CH>, dim3(a.kv_heads, a.n_tokens), dim3(256), (size_t)0, stream, (T*)out, a));
+    if (a.shares) NIB_CUDA(launch_pdl(merge_int8_kernel<T, CH>, dim3(a.heads, a.n_tokens), dim3(MERGE_THREADS), (size_t)0, stream, (T*)out, a));
     return 0;
 }
 
@@ -746,8 +820,8 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     const Args a{c.ctx_lens, c.block_table, (const signed char*)c.k_pages, (const signed char*)c.v_pages, c.k_scales, c.v_scales, c.part_o, c.part_ml,
                  c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, n_tokens, heads, kv_heads, heads / kv_heads, head_dim, c.window, c.ctas, c.shares, c.scale};
     int rc;
-    if (kind == 1) {
-        NIB_REQUIRE((((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0, "attention (8-bit cache): the pools must be 16-byte aligned");
+    // (rows and pools that lie off the pieces that a thread reads and writes at a time go to the general kernel)
+    if (kind == 1 && ((uintptr_t)q & 3) == 0 && c.q_stride % 2 == 0 && ((uintptr_t)out & 7) == 0 && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0) {
 #define CALL(KERNEL, T, CH, THREADS, SMEM, MOST)                                                                                \
     do {                                                                                                                        \
         static const cudaError_t set = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MOST));  \
