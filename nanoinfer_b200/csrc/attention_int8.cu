@@ -169,11 +169,13 @@ __device__ __forceinline__ void finish(const float* cta_o, const float* cta_ml, 
 }
 
 // Merges the parts of the rows that lie in more than one share, in order, and stores the rows that see nothing. grid: (heads, tokens).
-constexpr int MERGE_THREADS = 128;
+// More than eight parts are taken in turns by as many threads as there are for an element, whose sums meet in shared memory.
+constexpr int MERGE_THREADS = 256;         // the most; half of them where the rows alone fill the SMs (64 x 14 rows of 64: 15.2 us with the attention, 17.5)
 
 template <typename T, int CH>
 __global__ void __launch_bounds__(MERGE_THREADS)
 merge_int8_kernel(T* __restrict__ out, const Args a) {
+    __shared__ float s_acc[MERGE_THREADS], s_m[MERGE_THREADS], s_l[MERGE_THREADS];
     const int token = blockIdx.y, head = blockIdx.x, kvh = head / a.n_rep, row = head - kvh * a.n_rep, lane = threadIdx.x & 31, hd = a.head_dim;
     int all = 0, before = 0;                        // chunks of a kv head
     for (int t = lane; t < a.n_tokens; t += 32) {
@@ -187,35 +189,59 @@ merge_int8_kernel(T* __restrict__ out, const Args a) {
     pdl_wait();             // (the lengths are the step's inputs)
     pdl_launch_dependents();
     if (parts == 1) return;
-    for (int d = threadIdx.x; d < hd; d += MERGE_THREADS) {
+    const int threads = blockDim.x;
+    const int turns = parts <= 8 ? 1 : max(1, threads / hd);
+    for (int d0 = 0; d0 < hd; d0 += threads) {
+        const int turn = turns > 1 ? threadIdx.x / hd : 0, d = turns > 1 ? threadIdx.x - turn * hd : d0 + threadIdx.x;
         float m = -INFINITY, l = 0.f, acc = 0.f;
-        for (int s0 = 0; s0 < parts; s0 += 16) {
-            float v[16];
-            float2 x[16];
+        if (turn < turns && d < hd) {
+            for (int s0 = turn; s0 < parts; s0 += 8 * turns) {
+                float v[8];
+                float2 x[8];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) {
-                const int s = min(s0 + u, parts - 1);
-                const size_t at = (size_t)(s == 0 ? 2 * b0 + 1 : 2 * (b0 + s)) * a.n_rep + row;
-                v[u] = a.part_o[at * hd + d];
-                x[u] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-            }
-            float top = m;
+                for (int u = 0; u < 8; ++u) {
+                    const int s = s0 + u * turns;
+                    v[u] = 0.f;
+                    x[u] = make_float2(-INFINITY, 0.f);
+                    if (s < parts) {
+                        const size_t at = (size_t)(s == 0 ? 2 * b0 + 1 : 2 * (b0 + s)) * a.n_rep + row;
+                        v[u] = a.part_o[at * hd + d];
+                        x[u] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+                    }
+                }
+                float top = m;
 #pragma unroll
-            for (int u = 0; u < 16; ++u) top = fmaxf(top, x[u].x);
-            const float f0 = half_factor(m, top);
-            l = l * f0 * f0;
-            acc *= f0 * f0;
-            m = top;
+                for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
+                const float f0 = half_factor(m, top);
+                l = l * f0 * f0;
+                acc *= f0 * f0;
+                m = top;
 #pragma unroll
-            for (int u = 0; u < 16; ++u) {
-                if (s0 + u < parts) {
-                    const float f = half_factor(x[u].x, m);
-                    l += x[u].y * f * f;
-                    acc += v[u] * (f * f);
+                for (int u = 0; u < 8; ++u) {
+                    if (s0 + u * turns < parts) {
+                        const float f = half_factor(x[u].x, m);
+                        l += x[u].y * f * f;
+                        acc += v[u] * (f * f);
+                    }
                 }
             }
         }
-        Elem<T>::store(out + ((size_t)token * a.heads + head) * hd + d, l == 0.f ? 0.f : acc / l * RELIFT);
+        if (turns > 1) {
+            s_acc[threadIdx.x] = acc; s_m[threadIdx.x] = m; s_l[threadIdx.x] = l;
+            __syncthreads();
+            if (turn != 0) return;
+            float top = m;
+            for (int u = 1; u < turns; ++u) top = fmaxf(top, s_m[u * hd + d]);
+            const float f0 = half_factor(m, top);
+            l = l * f0 * f0;
+            acc *= f0 * f0;
+            for (int u = 1; u < turns; ++u) {
+                const float f = half_factor(s_m[u * hd + d], top);
+                l += s_l[u * hd + d] * f * f;
+                acc += s_acc[u * hd + d] * (f * f);
+            }
+        }
+        if (d < hd) Elem<T>::store(out + ((size_t)token * a.heads + head) * hd + d, l == 0.f ? 0.f : acc / l * RELIFT);
     }
 }
 
@@ -774,7 +800,7 @@ int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int threads, 
     cfg.attrs = attr;
     cfg.numAttrs = n;
     NIB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const T*)q, (T*)out, a));
-    if (a.shares) NIB_CUDA(launch_pdl(merge_int8_kernel<T, CH>, dim3(a.heads, a.n_tokens), dim3(MERGE_THREADS), (size_t)0, stream, (T*)out, a));
+    if (a.shares) NIB_CUDA(launch_pdl(merge_int8_kernel<T, CH>, dim3(a.heads, a.n_tokens), dim3(a.heads * a.n_tokens <= 2 * 148 ? MERGE_THREADS : MERGE_THREADS / 2), (size_t)0, stream, (T*)out, a));
     return 0;
 }
 

@@ -884,12 +884,15 @@ class Kernels:
         all rows' keys are dealt to)."""
         keys = max(1, min(max_ctx, window) if window > 0 else max_ctx)
         units = max(1, n_tokens * kv_heads)
-        chunk = 32 if kind == 0 else 128 if head_dim == 64 else 64
-        chunks = -(-keys // chunk)
+        chunk = 32 if kind == 0 else 128 if head_dim == 64 else 64          # keys that a CTA takes at a time
+        chunks, room = -(-keys // chunk), 4 * self.sm_count                 # (four CTAs find room on an SM)
         fixed = self.options.fixed_decode_splits
-        if fixed > 8 or (not fixed and units * chunks > 4 * self.sm_count):
-            return 1, min(4 * self.sm_count, units * (fixed or chunks))
-        return _cluster_splits(fixed or min(8, chunks, max(1, 4 * self.sm_count // units))), 0
+        if fixed:
+            return (_cluster_splits(fixed), 0) if fixed <= 8 else (1, min(room, units * fixed))
+        ctas = _cluster_splits(max(1, min(8, chunks, room // 2 // units)))
+        if chunks <= ctas * (1 if kind == 0 else 16):
+            return ctas, 0
+        return 1, min(room, units * min(chunks, 64))        # (a row's parts are one kernel's sum)
 
     def attention_tc_error(self) -> int:
         """The error word of the tcgen05 attention's bounded waits (0 = none); synchronises and clears it."""
