@@ -11,7 +11,16 @@
 //
 // The scale multiplies a group's 32-bit sum, not its weights: the products are exact, and a group costs one multiply-add for each
 // result instead of one multiplication for each weight.
+//
+// What bounds a product of many weights is the instructions that make a code a number: 11 for eight codes as above, 65 for a tile and
+// its row tile, where memory delivers a tile to an SM every 22 cycles. So there (F16) a code is fed as it lies in its word: in the low
+// bits of a 16-bit float it is code * 2^-24 (a number below the normal ones, which the tensor core multiplies exactly), four bits
+// further up 16 times that, and one shift reaches the word's other half: 5 instructions. The activations are 16-bit floats too,
+// scaled by a power of two for each token so that the largest lies in 2^13 .. 2^14 (every element that counts is exact), and the 8 of
+// (code - 8) leaves a group's sum as 8 times the sum of the group's activations, where the sum begins. A small kernel before makes
+// the scaled activations, those sums and the factors, which small products cannot wait for.
 #include "common.cuh"
+#include <cuda_fp16.h>
 
 namespace {
 
@@ -22,11 +31,21 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const unsigned (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 // Weights are read once: they are not to push the activations out of L1.
 __device__ __forceinline__ uint4 ldg16_stream(const uint4* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
+}
+// The four fragments of a word as they lie there: 16-bit floats code * 2^-24, the rows g + 8 (fragments 1 and 3) 16 times that.
+__device__ __forceinline__ void codes_of(unsigned w, unsigned (&a)[4]) {
+    const unsigned u = w >> 8;
+    a[0] = w & 0x000f000fu; a[1] = w & 0x00f000f0u; a[2] = u & 0x000f000fu; a[3] = u & 0x00f000f0u;
 }
 // The four fragments of a word: nibble pairs as bfloat16 numbers code - 8.
 __device__ __forceinline__ void weights_of(unsigned w, unsigned (&a)[4]) {
@@ -41,13 +60,62 @@ __device__ __forceinline__ void weights_of(unsigned w, unsigned (&a)[4]) {
 
 struct Args {
     const __nv_bfloat16* x; const uint4* w; const unsigned* scales; const float* bias; void* out;
+    const float* sums; const float* factors;        // F16: -8 * 2^-24 * the sums of the activations [k / 64 or 32][64 tokens], a factor for each token
     int tokens, n_out, k, ldx, ldo, epi, row_tiles, k_tiles, group_shift, groups, ksplit;      // group_shift: log2(group)
     NibGlu glu;
 };
 
+// The activations of F16: a CTA a token. x16 [tokens][k] = x * 2^e, sums as Args has them, factors = 2^24 / 2^e. step: 64 or 32.
+constexpr int PREP_THREADS = 512;
+__global__ void __launch_bounds__(PREP_THREADS)
+prepare_f16_kernel(const __nv_bfloat16* __restrict__ x, int ldx, __half* __restrict__ x16, float* __restrict__ sums, float* __restrict__ factors, int k, int step) {
+    __shared__ unsigned s_top[PREP_THREADS / 32];
+    const int token = blockIdx.x, lane = threadIdx.x & 31;
+    const uint4* row = reinterpret_cast<const uint4*>(x + (size_t)token * ldx);
+    pdl_launch_dependents();        // (the product sends for its weights meanwhile)
+    pdl_wait();
+    unsigned top = 0;
+    for (int i = threadIdx.x; i < k / 8; i += PREP_THREADS) {
+        const uint4 u = row[i];
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7fffu, (w[j] >> 16) & 0x7fffu));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) s_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PREP_THREADS / 32; ++i) top = max(top, s_top[i]);
+    // the exponent field e of the largest element: 2^(140 - e) takes it to 2^13 (in two factors: the power may leave the range)
+    const int e = (int)(top >> 7), up = (e == 0 || e == 255) ? 0 : 140 - e;
+    const float f1 = __uint_as_float((unsigned)(127 + up / 2) << 23), f2 = __uint_as_float((unsigned)(127 + up - up / 2) << 23);
+    if (threadIdx.x == 0)
+        factors[token] = 0x1p24f * __uint_as_float((unsigned)(127 - up / 2) << 23) * __uint_as_float((unsigned)(127 - (up - up / 2)) << 23);
+    const int lanes = step / 8;                     // that hold a step between them
+    for (int i0 = 0; i0 < k / 8; i0 += PREP_THREADS) {
+        const int i = i0 + threadIdx.x;
+        float sum = 0.f;
+        if (i < k / 8) {
+            const uint4 u = row[i];
+            const unsigned w[4] = {u.x, u.y, u.z, u.w};
+            unsigned r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * f1 * f2, __uint_as_float(w[j] & 0xffff0000u) * f1 * f2);
+                const float2 v = __half22float2(h);
+                sum += v.x + v.y;
+                r[j] = *reinterpret_cast<const unsigned*>(&h);
+            }
+            reinterpret_cast<uint4*>(x16 + (size_t)token * k)[i] = make_uint4(r[0], r[1], r[2], r[3]);
+        }
+        for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (i < k / 8 && (i & (lanes - 1)) == 0) sums[(size_t)(i / lanes) * 64 + token] = sum * (-8.f * 0x1p-24f);
+    }
+}
+
 // R row tiles a warp, which share the activations they multiply with (two of one matrix, or with DUAL a gate's and an up's); NT tiles
 // of 8 tokens; D tiles of weights on their way at any time. ``ksplit`` warps of a CTA share a row unit's K and are summed in order.
-template <int NT, int R, bool DUAL, bool G32, int D>
+template <int NT, int R, bool DUAL, bool G32, bool F16, int D>
 __global__ void __launch_bounds__(WARPS * 32)
 gemm_int4_kernel(const Args a) {
     extern __shared__ float part[];             // [WARPS][R][NT][4][32] where K is split
@@ -87,7 +155,7 @@ gemm_int4_kernel(const Args a) {
     pdl_wait();                                 // weights are nobody's output; the activations are
     const __nv_bfloat16* xp[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) xp[n] = n * 8 + g < a.tokens ? a.x + (size_t)(n * 8 + g) * a.ldx + 8 * t : nullptr;
+    for (int n = 0; n < NT; ++n) xp[n] = n * 8 + g < a.tokens ? a.x + (size_t)(n * 8 + g) * a.ldx + 8 * t : nullptr;        // (16 bits either way)
 
     float acc[R][NT][4];
 #pragma unroll
@@ -117,19 +185,26 @@ gemm_int4_kernel(const Args a) {
             for (int b = 0; b < 2; ++b) {
                 if (G32 || b == 0) {
 #pragma unroll
-                    for (int r = 0; r < R; ++r)
+                    for (int n = 0; n < NT; ++n) {
+                        float2 c = make_float2(0.f, 0.f);
+                        if (F16) c = __ldg(reinterpret_cast<const float2*>(a.sums + (size_t)min(G32 ? 2 * kt + b : kt, a.k / (G32 ? 32 : 64) - 1) * 64 + n * 8 + 2 * t));
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) s[r][n][0] = s[r][n][1] = s[r][n][2] = s[r][n][3] = 0.f;
+                        for (int r = 0; r < R; ++r) { s[r][n][0] = c.x; s[r][n][1] = c.y; s[r][n][2] = 16.f * c.x; s[r][n][3] = 16.f * c.y; }
+                    }
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     unsigned f[4];
-                    weights_of(b == 0 ? w[d][r].x : w[d][r].z, f);
+                    auto multiply = [&](unsigned word, bool second) {
+                        if (F16) codes_of(word, f); else weights_of(word, f);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_bf16(s[r][n], f, x[n][b].x, x[n][b].y);
-                    weights_of(b == 0 ? w[d][r].y : w[d][r].w, f);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_bf16(s[r][n], f, x[n][b].z, x[n][b].w);
+                        for (int n = 0; n < NT; ++n) {
+                            const unsigned b0 = second ? x[n][b].z : x[n][b].x, b1 = second ? x[n][b].w : x[n][b].y;
+                            if (F16) mma_f16(s[r][n], f, b0, b1); else mma_bf16(s[r][n], f, b0, b1);
+                        }
+                    };
+                    multiply(b == 0 ? w[d][r].x : w[d][r].z, false);
+                    multiply(b == 0 ? w[d][r].y : w[d][r].w, true);
                 }
                 if (G32 || b == 1) {
 #pragma unroll
@@ -143,7 +218,16 @@ gemm_int4_kernel(const Args a) {
     }
 
     // ---- the results of token tile n: element e is row g + 8 * (e / 2), token n * 8 + 2t + (e & 1)
-    auto emit = [&](const float (&v)[R][4], int n) {
+    auto emit = [&](float (&v)[R][4], int n) {
+        if (F16) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int tok = n * 8 + 2 * t + j;
+                const float f = tok < a.tokens ? __ldg(a.factors + tok) : 0.f;
+#pragma unroll
+                for (int r = 0; r < R; ++r) { v[r][j] *= f; v[r][2 + j] *= f * 0.0625f; }
+            }
+        }
 #pragma unroll
         for (int r = 0; r < (DUAL ? 1 : R); ++r)
 #pragma unroll
@@ -255,23 +339,23 @@ unpack_int4_kernel(const uint4* __restrict__ w, const unsigned* __restrict__ sca
     }
 }
 
-template <int NT, int R, bool DUAL, bool G32>
+template <int NT, int R, bool DUAL, bool G32, bool F16>
 int launch(const Args& a, int blocks, cudaStream_t stream) {
     constexpr int D = NT <= 2 ? 4 : 2;
     const size_t smem = a.ksplit > 1 ? (size_t)WARPS * R * NT * 4 * 32 * 4 : 0;
-    static const cudaError_t set = cudaFuncSetAttribute(gemm_int4_kernel<NT, R, DUAL, G32, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    static const cudaError_t set = cudaFuncSetAttribute(gemm_int4_kernel<NT, R, DUAL, G32, F16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                         WARPS * R * NT * 4 * 32 * 4);
     NIB_CUDA(set);
-    NIB_CUDA(launch_pdl(gemm_int4_kernel<NT, R, DUAL, G32, D>, dim3(blocks), dim3(WARPS * 32), smem, stream, a));
+    NIB_CUDA(launch_pdl(gemm_int4_kernel<NT, R, DUAL, G32, F16, D>, dim3(blocks), dim3(WARPS * 32), smem, stream, a));
     return 0;
 }
 
-template <int R, bool DUAL, bool G32>
+template <int R, bool DUAL, bool G32, bool F16>
 int by_tokens(const Args& a, int blocks, cudaStream_t stream) {
-    if (a.tokens <= 8) return launch<1, R, DUAL, G32>(a, blocks, stream);
-    if (a.tokens <= 16) return launch<2, R, DUAL, G32>(a, blocks, stream);
-    if (a.tokens <= 32) return launch<4, R, DUAL, G32>(a, blocks, stream);
-    return launch<8, R, DUAL, G32>(a, blocks, stream);
+    if (a.tokens <= 8) return launch<1, R, DUAL, G32, F16>(a, blocks, stream);
+    if (a.tokens <= 16) return launch<2, R, DUAL, G32, F16>(a, blocks, stream);
+    if (a.tokens <= 32) return launch<4, R, DUAL, G32, F16>(a, blocks, stream);
+    return launch<8, R, DUAL, G32, F16>(a, blocks, stream);
 }
 
 bool fits(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0; }
@@ -281,10 +365,17 @@ bool fits(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || gr
 // The arguments of a product, one block of memory.
 struct NibGemmInt4 {
     const void* x; const void* w; const void* scales; const float* bias; void* out;
+    void* scratch;                                      // nib_gemm_int4_scratch bytes, 16-byte aligned
     int tokens, n, k, group, ldx, ldo, epi, sms;        // sms: SMs of the device
     float alpha, limit, shift;                          // the constants of EPI_GLU
     int pad;
 };
+
+// Whether a product's activations are prepared as 16-bit floats, and the scratch bytes that takes (0: not).
+static long long f16_scratch(int tokens, int n, int k, bool dual) {
+    return (long long)(dual ? 2 : 1) * n * k / 2 >= (4 << 20) ? (long long)tokens * k * 2 + (long long)ceil_div(k, 32) * 64 * 4 + 256 : 0;
+}
+NIB_API long long nib_gemm_int4_scratch(int tokens, int n, int k, int dual) { return tokens > 64 ? 0 : f16_scratch(tokens, n, k, dual != 0); }
 
 // out[tokens, n] from the packed weights of n rows (of 2 n rows, gate then up, for the gated epilogues). -1, and nothing done, where
 // another product has to take these operands: more than 64 tokens, rows that do not begin on 16 bytes, a gated product whose halves
@@ -300,18 +391,31 @@ NIB_API int nib_gemm_int4(const void* args, cudaStream_t stream) {
     if (tokens > 64 || c.ldx % 8 != 0 || ((uintptr_t)c.x & 15) != 0 || (dual && n % 16 != 0)) return -1;
     if (tokens == 0) return 0;
     const int out_tiles = ceil_div(n, 16);
-    Args a{(const __nv_bfloat16*)c.x, (const uint4*)c.w, (const unsigned*)c.scales, c.bias, c.out, tokens, n, k, c.ldx, c.ldo, epi,
+    const bool g32 = group == 32, f16 = c.scratch != nullptr && f16_scratch(tokens, n, k, dual) > 0;
+    Args a{(const __nv_bfloat16*)c.x, (const uint4*)c.w, (const unsigned*)c.scales, c.bias, c.out, nullptr, nullptr, tokens, n, k, c.ldx, c.ldo, epi,
            dual ? 2 * out_tiles : out_tiles, ceil_div(k, 64), group == 32 ? 5 : group == 64 ? 6 : 7, k / group, 1, NibGlu{c.alpha, c.limit, c.shift}};
+    if (f16) {
+        float* sums = (float*)c.scratch;
+        float* factors = sums + (size_t)ceil_div(k, 32) * 64;
+        __half* x16 = (__half*)(factors + 64);
+        NIB_CUDA(launch_pdl(prepare_f16_kernel, dim3(tokens), dim3(PREP_THREADS), (size_t)0, stream, (const __nv_bfloat16*)c.x, c.ldx, x16, sums, factors, k, g32 ? 32 : 64));
+        a.x = (const __nv_bfloat16*)x16;
+        a.ldx = k;
+        a.sums = sums;
+        a.factors = factors;
+    }
     // Two row tiles a warp share the activations' loads; one where two would leave SMs without work.
     const bool two = dual || (tokens <= 32 && out_tiles >= 2 * WARPS * sms);
     const int units = dual || !two ? out_tiles : ceil_div(out_tiles, 2);
     // As many warps share a unit's K as it takes to have 16 warps an SM, while each has a tile.
     while (a.ksplit < WARPS && (long long)units * a.ksplit < 16LL * sms && a.k_tiles >= 2 * a.ksplit) a.ksplit *= 2;
     const int blocks = ceil_div((long long)units * a.ksplit, WARPS);
-    const bool g32 = group == 32;
-    if (dual) return g32 ? by_tokens<2, true, true>(a, blocks, stream) : by_tokens<2, true, false>(a, blocks, stream);
-    if (two) return g32 ? by_tokens<2, false, true>(a, blocks, stream) : by_tokens<2, false, false>(a, blocks, stream);
-    return g32 ? by_tokens<1, false, true>(a, blocks, stream) : by_tokens<1, false, false>(a, blocks, stream);
+#define CALL(R, DUAL)                                                                                                                                  \
+    (f16 ? (g32 ? by_tokens<R, DUAL, true, true>(a, blocks, stream) : by_tokens<R, DUAL, false, true>(a, blocks, stream))                               \
+         : (g32 ? by_tokens<R, DUAL, true, false>(a, blocks, stream) : by_tokens<R, DUAL, false, false>(a, blocks, stream)))
+    if (dual) return CALL(2, true);
+    return two ? CALL(2, false) : CALL(1, false);
+#undef CALL
 }
 
 // The weights of n rows as bfloat16 or 32-bit numbers [n, k]; part 1: what the rounding to bfloat16 leaves.

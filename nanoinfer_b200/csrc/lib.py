@@ -28,7 +28,7 @@ _EPI = {"store": 0, "add": 1, "f32": 2, "swiglu": 3, "glu": 5, "geglu": 6}
 _ADD = _EPI["add"]
 _DUAL = (3, 5, 6)       # the gated epilogues: two accumulators, gate rows and up rows
 # The arguments of calls that take them as one block of memory (NibAppendInt8, NibAttendInt8, NibGemmInt4)
-_APPEND_INT8, _ATTEND_INT8, _GEMM_INT4 = struct.Struct("=12Q16i"), struct.Struct("=10Q14ifi"), struct.Struct("=5Q8i3fi")
+_APPEND_INT8, _ATTEND_INT8, _GEMM_INT4 = struct.Struct("=12Q16i"), struct.Struct("=10Q14ifi"), struct.Struct("=6Q8i3fi")
 _LAYOUT = {"interleaved": 0, "half": 1}     # which elements of a rotated vector make a pair
 
 
@@ -160,6 +160,7 @@ class Kernels:
                      "nib_gemm_int4", "nib_unpack_int4"):
             getattr(self._lib, name).restype = c_int
         self.sample_rows_most = int(self._lib.nib_sample_rows_most())      # rows whose parameters a launch takes by value
+        self._lib.nib_gemm_int4_scratch.restype = c_longlong
         self._lib.nib_grouped_state_scratch.restype = self._lib.nib_decay_state_scratch.restype = c_longlong
 
     # ---- plumbing ---------------------------------------------------------------------------
@@ -558,10 +559,13 @@ class Kernels:
             if not self.weights_ahead:
                 self._lib.nib_pdl_skip_next()
             alpha, limit, shift = (0.0, 0.0, 0.0) if glu is None else glu
-            args = _GEMM_INT4.pack(a.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), 0 if bias32 is None else bias32.data_ptr(), out.data_ptr(), m, n, k,
-                                   w.group, a.stride(0), out.stride(0), epi, self.sm_count, alpha, limit, shift, 0)
+            scratch = self._lib.nib_gemm_int4_scratch(m, n, k, 1 if dual else 0)
+            room = torch.empty(scratch, dtype=torch.uint8, device=a.device) if scratch else None
+            args = _GEMM_INT4.pack(a.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), 0 if bias32 is None else bias32.data_ptr(), out.data_ptr(),
+                                   0 if room is None else room.data_ptr(), m, n, k, w.group, a.stride(0), out.stride(0), epi, self.sm_count, alpha, limit, shift, 0)
             rc = self._lib.nib_gemm_int4(args, self._stream())
             if rc >= 0:
+                self.launches += 1 if scratch else 0
                 self._check(rc, "linear (4-bit weights)")
                 return
         plain = torch.empty(w.shape, dtype=a.dtype, device=a.device)
