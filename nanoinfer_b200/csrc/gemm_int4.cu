@@ -19,8 +19,11 @@
 // scaled by a power of two for each token so that the largest lies in 2^13 .. 2^14 (every element that counts is exact), and the 8 of
 // (code - 8) leaves a group's sum as 8 times the sum of the group's activations, where the sum begins. A small kernel before makes
 // the scaled activations, those sums and the factors, which small products cannot wait for.
-#include "common.cuh"
+#include "pipeline.cuh"
 #include <cuda_fp16.h>
+#include <cmath>
+
+using namespace nibp;
 
 namespace {
 
@@ -36,12 +39,31 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const unsigned (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Weights are read once: they are not to push the activations out of L1.
-__device__ __forceinline__ uint4 ldg16_stream(const uint4* p) {
+__device__ __forceinline__ void copy16_once(unsigned dst, const void* src) {          // (past L1: weights are read once)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(unsigned dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4_or_zero(unsigned dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(unsigned at) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ unsigned lds4(unsigned at) {
+    unsigned v;
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 lds8f(unsigned at) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
 // The four fragments of a word as they lie there: 16-bit floats code * 2^-24, the rows g + 8 (fragments 1 and 3) 16 times that.
 __device__ __forceinline__ void codes_of(unsigned w, unsigned (&a)[4]) {
     const unsigned u = w >> 8;
@@ -61,7 +83,7 @@ __device__ __forceinline__ void weights_of(unsigned w, unsigned (&a)[4]) {
 struct Args {
     const __nv_bfloat16* x; const uint4* w; const unsigned* scales; const float* bias; void* out;
     const float* sums; const float* factors;        // F16: -8 * 2^-24 * the sums of the activations [k / 64 or 32][64 tokens], a factor for each token
-    int tokens, n_out, k, ldx, ldo, epi, row_tiles, k_tiles, group_shift, groups, ksplit;      // group_shift: log2(group)
+    int tokens, n_out, k, ldx, ldo, epi, row_tiles, k_tiles, group_shift, groups, ksplit, csize;      // group_shift: log2(group)
     NibGlu glu;
 };
 
@@ -113,49 +135,94 @@ prepare_f16_kernel(const __nv_bfloat16* __restrict__ x, int ldx, __half* __restr
     }
 }
 
-// R row tiles a warp, which share the activations they multiply with (two of one matrix, or with DUAL a gate's and an up's); NT tiles
-// of 8 tokens; D tiles of weights on their way at any time. ``ksplit`` warps of a CTA share a row unit's K and are summed in order.
-template <int NT, int R, bool DUAL, bool G32, bool F16, int D>
+// A stage of a warp's ring in shared memory: R tiles of weights and the activations of 64 k of NT * 8 tokens, every lane's own 16-byte
+// pieces (what a lane uses it has copied itself), and the scales and sums of G groups.
+template <int NT, int R, bool G32, bool F16> struct Ring {
+    static constexpr int G = G32 ? 2 : 1;
+    static constexpr int X_AT = R * 512, S_AT = X_AT + NT * 1024, C_AT = S_AT + R * G * 32;
+    static constexpr int STAGE = C_AT + (F16 ? G * NT * 32 : 0);
+    static constexpr int SPLIT = NT <= 2 ? 4 : 1;           // CTAs that may share K
+    static constexpr int SENT = SPLIT > 1 ? SPLIT * R * NT * 512 : 0;       // what they send to the first of them
+    static constexpr int FIT = (108 * 1024 - SENT) / WARPS / STAGE, D = FIT < 2 ? 2 : FIT > 8 ? 8 : FIT;      // two CTAs an SM
+    static constexpr int RING = WARPS * D * STAGE, PART = WARPS * R * NT * 4 * 32 * 4;
+    static constexpr int OWN = RING > PART ? RING : PART, BYTES = OWN + SENT;
+    static_assert(OWN % 16 == 0, "results are sent 16 bytes at a time");
+};
+
+__device__ __forceinline__ void st_peer_f32x4(unsigned addr, const float4& v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+// R row tiles a warp, which share the activations they multiply with (with DUAL half of them a gate's and half an up's); NT tiles of 8
+// tokens. ``ksplit`` warps of a CTA share a row unit's K and are summed in order; where all eight do, up to four CTAs of a cluster may
+// share it further, and the first of them sums what the others send it, in order.
+template <int NT, int R, bool DUAL, bool G32, bool F16>
 __global__ void __launch_bounds__(WARPS * 32)
 gemm_int4_kernel(const Args a) {
-    extern __shared__ float part[];             // [WARPS][R][NT][4][32] where K is split
+    using C = Ring<NT, R, G32, F16>;
+    constexpr int D = C::D, G = C::G, OUT = DUAL ? R / 2 : R;              // row tiles of the result
+    extern __shared__ __align__(16) float part[];             // the rings; then [WARPS][R][NT][4][32] where K is split
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int unit = blockIdx.x * (WARPS / a.ksplit) + warp / a.ksplit, kpart = warp % a.ksplit;
+    const int rank = a.csize > 1 ? (int)cluster_rank() : 0;
+    if (a.csize > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");       // this CTA is there: its peers may send
+    const int unit = (blockIdx.x / a.csize) * (WARPS / a.ksplit) + warp / a.ksplit, kpart = warp % a.ksplit;
     const int out_tiles = (a.n_out + 15) / 16;
-    const int rt0 = DUAL ? unit : unit * R;                                 // first row tile of the unit
+    const int rt0 = unit * OUT;                                             // first row tile of the unit's results
     const bool live = rt0 < out_tiles;
-    const int per = (a.k_tiles + a.ksplit - 1) / a.ksplit;
-    const int begin = live ? min(a.k_tiles, kpart * per) : 0, end = live ? min(a.k_tiles, begin + per) : 0;
+    const int per = (a.k_tiles + a.ksplit * a.csize - 1) / (a.ksplit * a.csize);
+    const int begin = live ? min(a.k_tiles, (rank * a.ksplit + kpart) * per) : 0, end = live ? min(a.k_tiles, begin + per) : 0;
     const uint4* wp[R];
-    const unsigned* sp[R];
+    size_t scale_row[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int rt = min(DUAL ? rt0 + r * out_tiles : rt0 + r, a.row_tiles - 1);      // (a tile behind the last is computed and not stored)
+        // (a tile behind the last is computed and not stored)
+        const int rt = min(DUAL ? min(rt0 + r / 2, out_tiles - 1) + (r & 1) * out_tiles : rt0 + r, a.row_tiles - 1);
         wp[r] = a.w + (size_t)rt * a.k_tiles * 32 + lane;
-        sp[r] = a.scales + (size_t)rt * a.groups * 8 + g;
+        scale_row[r] = (size_t)rt * a.groups;
     }
-    pdl_launch_dependents();
-    uint4 w[D][R];
-    unsigned sc[D][R][G32 ? 2 : 1];
-    auto load = [&](int d, int kt) {
+    const unsigned ring = (unsigned)__cvta_generic_to_shared(part) + warp * D * C::STAGE;
+    const int groups = a.groups;
+    auto send_weights = [&](int kt, unsigned dst) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            w[d][r] = ldg16_stream(wp[r] + (size_t)kt * 32);
-            if (G32) {
-                sc[d][r][0] = __ldg(sp[r] + (size_t)(2 * kt) * 8);
-                sc[d][r][G32 ? 1 : 0] = 2 * kt + 1 < a.groups ? __ldg(sp[r] + (size_t)(2 * kt + 1) * 8) : 0u;
-            } else {
-                sc[d][r][0] = __ldg(sp[r] + (size_t)((kt << 6) >> a.group_shift) * 8);
+            copy16_once(dst + r * 512 + lane * 16, wp[r] + (size_t)kt * 32);
+#pragma unroll
+            for (int b = 0; b < G; ++b) {
+                const int at = G32 ? 2 * kt + b : (kt << 6) >> a.group_shift;
+                if (lane < 8) copy4_or_zero(dst + C::S_AT + (r * G + b) * 32 + lane * 4, a.scales + (scale_row[r] + min(at, groups - 1)) * 8 + lane, at < groups);
             }
         }
     };
+    const __nv_bfloat16* xp[NT];            // (16 bits either way)
 #pragma unroll
-    for (int d = 0; d < D; ++d)
-        if (begin + d < end) load(d, begin + d);
-    pdl_wait();                                 // weights are nobody's output; the activations are
-    const __nv_bfloat16* xp[NT];
+    for (int n = 0; n < NT; ++n) xp[n] = a.x + (size_t)min(n * 8 + g, a.tokens - 1) * a.ldx + 8 * t;
+    auto send_activations = [&](int kt, unsigned dst) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) xp[n] = n * 8 + g < a.tokens ? a.x + (size_t)(n * 8 + g) * a.ldx + 8 * t : nullptr;        // (16 bits either way)
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const bool valid = n * 8 + g < a.tokens && kt * 64 + b * 32 < a.k;
+                copy16_or_zero(dst + C::X_AT + (n * 2 + b) * 512 + lane * 16, xp[n] + (valid ? kt * 64 + b * 32 : 0), valid);
+            }
+        if (F16) {
+#pragma unroll
+            for (int b = 0; b < G; ++b) {
+                const int at = G32 ? 2 * kt + b : kt;
+                for (int i = lane; i < NT * 8; i += 32) copy4_or_zero(dst + C::C_AT + (b * NT * 8 + i) * 4, a.sums + (size_t)at * 64 + i, i < a.tokens && at * (G32 ? 32 : 64) < a.k);
+            }
+        }
+    };
+    pdl_launch_dependents();
+    // weights are nobody's output: the first stages' are sent for before the wait, the activations behind it
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+        if (begin + d < end) send_weights(begin + d, ring + d * C::STAGE);
+    pdl_wait();
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d) {
+        if (begin + d < end) send_activations(begin + d, ring + d * C::STAGE);
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
 
     float acc[R][NT][4];
 #pragma unroll
@@ -167,54 +234,55 @@ gemm_int4_kernel(const Args a) {
         to[0] = fmaf(s[0], s0, to[0]); to[1] = fmaf(s[1], s0, to[1]);
         to[2] = fmaf(s[2], s1, to[2]); to[3] = fmaf(s[3], s1, to[3]);
     };
-    for (int base = begin; base < end; base += D) {
+    unsigned src = ring, dst = ring + (D - 1) * C::STAGE;
+    const unsigned ring_end = ring + D * C::STAGE;
+#pragma unroll 1
+    for (int kt = begin; kt < end; ++kt) {
+        if (kt + D - 1 < end) { send_weights(kt + D - 1, dst); send_activations(kt + D - 1, dst); }
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group %0;\n" ::"n"(D - 1) : "memory");
+        __syncwarp();               // (scales and sums are other lanes' copies)
+        float s[R][NT][4];
 #pragma unroll
-        for (int d = 0; d < D; ++d) {
-            const int kt = base + d;
-            if (kt >= end) break;
-            uint4 x[NT][2];
+        for (int b = 0; b < 2; ++b) {
+            if (G32 || b == 0) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                    const float2 c = F16 ? lds8f(src + C::C_AT + (G32 ? b * NT * 32 : 0) + n * 32 + t * 8) : make_float2(0.f, 0.f);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    x[n][b] = make_uint4(0u, 0u, 0u, 0u);
-                    if (xp[n] != nullptr && kt * 64 + b * 32 < a.k) x[n][b] = *reinterpret_cast<const uint4*>(xp[n] + kt * 64 + b * 32);
-                }
-            float s[R][NT][4];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                if (G32 || b == 0) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float2 c = make_float2(0.f, 0.f);
-                        if (F16) c = __ldg(reinterpret_cast<const float2*>(a.sums + (size_t)min(G32 ? 2 * kt + b : kt, a.k / (G32 ? 32 : 64) - 1) * 64 + n * 8 + 2 * t));
-#pragma unroll
-                        for (int r = 0; r < R; ++r) { s[r][n][0] = c.x; s[r][n][1] = c.y; s[r][n][2] = 16.f * c.x; s[r][n][3] = 16.f * c.y; }
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    unsigned f[4];
-                    auto multiply = [&](unsigned word, bool second) {
-                        if (F16) codes_of(word, f); else weights_of(word, f);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const unsigned b0 = second ? x[n][b].z : x[n][b].x, b1 = second ? x[n][b].w : x[n][b].y;
-                            if (F16) mma_f16(s[r][n], f, b0, b1); else mma_bf16(s[r][n], f, b0, b1);
-                        }
-                    };
-                    multiply(b == 0 ? w[d][r].x : w[d][r].z, false);
-                    multiply(b == 0 ? w[d][r].y : w[d][r].w, true);
-                }
-                if (G32 || b == 1) {
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) add(acc[r][n], s[r][n], sc[d][r][G32 ? b : 0]);
+                    for (int r = 0; r < R; ++r) { s[r][n][0] = c.x; s[r][n][1] = c.y; s[r][n][2] = 16.f * c.x; s[r][n][3] = 16.f * c.y; }
                 }
             }
-            if (kt + D < end) load(d, kt + D);
+            uint4 x[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[n] = lds16(src + C::X_AT + (n * 2 + b) * 512 + lane * 16);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const unsigned at = src + r * 512 + lane * 16 + b * 8;
+                const float2 words = lds8f(at);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    unsigned f[4];
+                    const unsigned word = __float_as_uint(h == 0 ? words.x : words.y);
+                    if (F16) codes_of(word, f); else weights_of(word, f);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const unsigned b0 = h == 0 ? x[n].x : x[n].z, b1 = h == 0 ? x[n].y : x[n].w;
+                        if (F16) mma_f16(s[r][n], f, b0, b1); else mma_bf16(s[r][n], f, b0, b1);
+                    }
+                }
+            }
+            if (G32 || b == 1) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const unsigned scale = lds4(src + C::S_AT + (r * G + (G32 ? b : 0)) * 32 + g * 4);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) add(acc[r][n], s[r][n], scale);
+                }
+            }
         }
+        __syncwarp();               // the shared places are free
+        src = src + C::STAGE == ring_end ? ring : src + C::STAGE;
+        dst = dst + C::STAGE == ring_end ? ring : dst + C::STAGE;
     }
 
     // ---- the results of token tile n: element e is row g + 8 * (e / 2), token n * 8 + 2t + (e & 1)
@@ -229,14 +297,14 @@ gemm_int4_kernel(const Args a) {
             }
         }
 #pragma unroll
-        for (int r = 0; r < (DUAL ? 1 : R); ++r)
+        for (int r = 0; r < OUT; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int f = (rt0 + r) * 16 + g + 8 * (e >> 1), tok = n * 8 + 2 * t + (e & 1);
                 if (f >= a.n_out || tok >= a.tokens) continue;
                 const size_t at = (size_t)tok * a.ldo + f;
                 if (DUAL) {
-                    const float gate = v[0][e], up = v[R - 1][e];
+                    const float gate = v[DUAL ? 2 * r : 0][e], up = v[DUAL ? 2 * r + 1 : 0][e];
                     const float y = a.epi == EPI_GEGLU ? nib_geglu_fast(gate, up)
                                   : a.epi == EPI_GLU ? nib_glu_fast(a.glu, gate, up) : __fdividef(gate, 1.0f + __expf(-gate)) * up;
                     static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
@@ -261,6 +329,7 @@ gemm_int4_kernel(const Args a) {
         }
         return;
     }
+    __syncthreads();                // every warp is through with its ring
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -268,18 +337,46 @@ gemm_int4_kernel(const Args a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) part[(((warp * R + r) * NT + n) * 4 + e) * 32 + lane] = acc[r][n][e];
     __syncthreads();
-    if (!live) return;
     const int first = warp - kpart;             // the unit's first warp
+    auto sum_of = [&](int r, int n) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < a.ksplit; ++p) {
+            const float* at = part + (((first + p) * R + r) * NT + n) * 128 + lane;
+            v.x += at[0]; v.y += at[32]; v.z += at[64]; v.w += at[96];
+        }
+        return v;
+    };
+    if constexpr (C::SPLIT > 1) {
+        if (a.csize > 1) {          // (all eight warps share one unit)
+            float4* sent = reinterpret_cast<float4*>(reinterpret_cast<unsigned char*>(part) + C::OWN);         // [csize][R * NT][32]
+            asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");           // every CTA is there
+            for (int i = warp; i < R * NT; i += WARPS) st_peer_f32x4(peer_smem(sent + (rank * R * NT + i) * 32 + lane, 0), sum_of(i / NT, i % NT));
+            cluster_sync();
+            if (rank != 0) return;
+            for (int n = warp; n < NT; n += WARPS) {
+                float v[R][4];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int p = 0; p < a.csize; ++p) {
+                        const float4 x = sent[(p * R * NT + r * NT + n) * 32 + lane];
+                        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+                    }
+                    v[r][0] = sum.x; v[r][1] = sum.y; v[r][2] = sum.z; v[r][3] = sum.w;
+                }
+                emit(v, n);
+            }
+            return;
+        }
+    }
+    if (!live) return;
     for (int n = kpart; n < NT; n += a.ksplit) {
         float v[R][4];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float sum = 0.f;
-                for (int p = 0; p < a.ksplit; ++p) sum += part[((((first + p) * R + r) * NT + n) * 4 + e) * 32 + lane];
-                v[r][e] = sum;
-            }
+        for (int r = 0; r < R; ++r) {
+            const float4 sum = sum_of(r, n);
+            v[r][0] = sum.x; v[r][1] = sum.y; v[r][2] = sum.z; v[r][3] = sum.w;
+        }
         emit(v, n);
     }
 }
@@ -341,12 +438,31 @@ unpack_int4_kernel(const uint4* __restrict__ w, const unsigned* __restrict__ sca
 
 template <int NT, int R, bool DUAL, bool G32, bool F16>
 int launch(const Args& a, int blocks, cudaStream_t stream) {
-    constexpr int D = NT <= 2 ? 4 : 2;
-    const size_t smem = a.ksplit > 1 ? (size_t)WARPS * R * NT * 4 * 32 * 4 : 0;
-    static const cudaError_t set = cudaFuncSetAttribute(gemm_int4_kernel<NT, R, DUAL, G32, F16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                        WARPS * R * NT * 4 * 32 * 4);
+    constexpr int bytes = Ring<NT, R, G32, F16>::BYTES;
+    static const cudaError_t set = cudaFuncSetAttribute(gemm_int4_kernel<NT, R, DUAL, G32, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     NIB_CUDA(set);
-    NIB_CUDA(launch_pdl(gemm_int4_kernel<NT, R, DUAL, G32, F16, D>, dim3(blocks), dim3(WARPS * 32), smem, stream, a));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = (size_t)bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (a.csize > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = a.csize;
+        attr[n].val.clusterDim.y = 1;
+        attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (nib_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    NIB_CUDA(cudaLaunchKernelEx(&cfg, gemm_int4_kernel<NT, R, DUAL, G32, F16>, a));
     return 0;
 }
 
@@ -354,8 +470,11 @@ template <int R, bool DUAL, bool G32, bool F16>
 int by_tokens(const Args& a, int blocks, cudaStream_t stream) {
     if (a.tokens <= 8) return launch<1, R, DUAL, G32, F16>(a, blocks, stream);
     if (a.tokens <= 16) return launch<2, R, DUAL, G32, F16>(a, blocks, stream);
-    if (a.tokens <= 32) return launch<4, R, DUAL, G32, F16>(a, blocks, stream);
-    return launch<8, R, DUAL, G32, F16>(a, blocks, stream);
+    if constexpr (R <= 2) {
+        if (a.tokens <= 32) return launch<4, R, DUAL, G32, F16>(a, blocks, stream);
+        return launch<8, R, DUAL, G32, F16>(a, blocks, stream);
+    }
+    return 1;       // (four row tiles are up to 16 tokens' choice)
 }
 
 bool fits(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0; }
@@ -373,7 +492,7 @@ struct NibGemmInt4 {
 
 // Whether a product's activations are prepared as 16-bit floats, and the scratch bytes that takes (0: not).
 static long long f16_scratch(int tokens, int n, int k, bool dual) {
-    return (long long)(dual ? 2 : 1) * n * k / 2 >= (4 << 20) ? (long long)tokens * k * 2 + (long long)ceil_div(k, 32) * 64 * 4 + 256 : 0;
+    return (long long)(dual ? 2 : 1) * n * k / 2 >= (48LL << 20) && tokens <= 16 ? (long long)tokens * k * 2 + (long long)ceil_div(k, 32) * 64 * 4 + 256 : 0;
 }
 NIB_API long long nib_gemm_int4_scratch(int tokens, int n, int k, int dual) { return tokens > 64 ? 0 : f16_scratch(tokens, n, k, dual != 0); }
 
@@ -393,7 +512,7 @@ NIB_API int nib_gemm_int4(const void* args, cudaStream_t stream) {
     const int out_tiles = ceil_div(n, 16);
     const bool g32 = group == 32, f16 = c.scratch != nullptr && f16_scratch(tokens, n, k, dual) > 0;
     Args a{(const __nv_bfloat16*)c.x, (const uint4*)c.w, (const unsigned*)c.scales, c.bias, c.out, nullptr, nullptr, tokens, n, k, c.ldx, c.ldo, epi,
-           dual ? 2 * out_tiles : out_tiles, ceil_div(k, 64), group == 32 ? 5 : group == 64 ? 6 : 7, k / group, 1, NibGlu{c.alpha, c.limit, c.shift}};
+           dual ? 2 * out_tiles : out_tiles, ceil_div(k, 64), group == 32 ? 5 : group == 64 ? 6 : 7, k / group, 1, 1, NibGlu{c.alpha, c.limit, c.shift}};
     if (f16) {
         float* sums = (float*)c.scratch;
         float* factors = sums + (size_t)ceil_div(k, 32) * 64;
@@ -404,17 +523,28 @@ NIB_API int nib_gemm_int4(const void* args, cudaStream_t stream) {
         a.sums = sums;
         a.factors = factors;
     }
-    // Two row tiles a warp share the activations' loads; one where two would leave SMs without work.
-    const bool two = dual || (tokens <= 32 && out_tiles >= 2 * WARPS * sms);
-    const int units = dual || !two ? out_tiles : ceil_div(out_tiles, 2);
-    // As many warps share a unit's K as it takes to have 16 warps an SM, while each has a tile.
-    while (a.ksplit < WARPS && (long long)units * a.ksplit < 16LL * sms && a.k_tiles >= 2 * a.ksplit) a.ksplit *= 2;
-    const int blocks = ceil_div((long long)units * a.ksplit, WARPS);
+    // How the work is cut: row tiles a warp (they share the activations' copies), warps of a CTA and CTAs that share K. A tile costs about
+    // 60 instructions and a step of a warp 40 besides; an SM issues some 2.2 a cycle, a warp alone one in four.
+    int rows = dual ? 2 : 1, best_rows = rows;
+    double best = 1e30;
+    for (; rows <= (tokens <= 16 ? 4 : 2); rows *= 2)
+        for (int ks = 1; ks <= WARPS; ks *= 2)
+            for (int cs = 1; cs <= (ks == WARPS && tokens <= 16 ? 4 : 1); ++cs) {
+                if (ks * cs > a.k_tiles) continue;
+                const int per_token_tile = (tokens + 7) / 8 - 1;             // (more tokens: more copies and products)
+                const double step = ceil_div(a.k_tiles, ks * cs) * (rows * (60.0 + 8.0 * per_token_tile) + 40.0 + 12.0 * per_token_tile);
+                const double ctas = (double)ceil_div((long long)ceil_div(a.row_tiles, rows) * ks, WARPS) * cs;
+                const double busy = ceil(ctas / sms) * WARPS * step / 2.2, alone = 4.0 * step;
+                const double cost = (busy > alone ? busy : alone) + (ks > 1 ? 300.0 : 0.0) + (cs > 1 ? 1500.0 : 0.0);
+                if (cost < best) { best = cost; best_rows = rows; a.ksplit = ks; a.csize = cs; }
+            }
+    rows = best_rows;
+    const int blocks = ceil_div((long long)ceil_div(a.row_tiles, rows) * a.ksplit, WARPS) * a.csize;
 #define CALL(R, DUAL)                                                                                                                                  \
     (f16 ? (g32 ? by_tokens<R, DUAL, true, true>(a, blocks, stream) : by_tokens<R, DUAL, false, true>(a, blocks, stream))                               \
          : (g32 ? by_tokens<R, DUAL, true, false>(a, blocks, stream) : by_tokens<R, DUAL, false, false>(a, blocks, stream)))
-    if (dual) return CALL(2, true);
-    return two ? CALL(2, false) : CALL(1, false);
+    if (dual) return rows == 4 ? CALL(4, true) : CALL(2, true);
+    return rows == 4 ? CALL(4, false) : rows == 2 ? CALL(2, false) : CALL(1, false);
 #undef CALL
 }
 
