@@ -89,12 +89,16 @@ class Model:
 def load_model(model_dir: str, dtype: str = "bfloat16", page_size: int = 16, num_pages: int = 0,
                max_cache_tokens: int = 0, max_batch: int = 8, max_tokens_per_step: int = 2048,
                device: str = "cuda:0", cuda_graphs: bool = True,
-               kernel_options: Optional[KernelOptions] = None) -> Model:
+               kernel_options: Optional[KernelOptions] = None, cache_dtype: str = "auto",
+               weight_format: str = "auto", weight_group: int = 64) -> Model:
+    """``cache_dtype`` "int8" keeps keys and values in 8 bits, ``weight_format`` "int4" the matrices of attention and feed-forward in 4
+    (see ``EngineConfig``)."""
     if num_pages <= 0 and max_cache_tokens <= 0:
         max_cache_tokens = 16384
     cfg = EngineConfig(dtype=dtype, page_size=page_size, num_pages=num_pages, max_cache_tokens=max_cache_tokens,
                        max_batch=max_batch, max_tokens_per_step=max_tokens_per_step, device=device,
-                       cuda_graphs=cuda_graphs, kernel_options=kernel_options or KernelOptions())
+                       cuda_graphs=cuda_graphs, kernel_options=kernel_options or KernelOptions(),
+                       cache_dtype=cache_dtype, weight_format=weight_format, weight_group=weight_group)
     return Model(model_dir, cfg)
 
 

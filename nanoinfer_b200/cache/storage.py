@@ -2,7 +2,7 @@
 
 What an entry keeps per token is a list of tensors (``CacheNeed.tensors``: keys and values for attention; a mixer
 may keep keys alone, one latent, or tensors of different widths and dtypes). Layout of one of them:
-``[num_pages, heads, page_size, width]``, so that the ``page_size x width`` tile of one head of one page is
+``[num_pages, heads, page_size, width]`` (a tensor that is kept once for a page: 1 in place of page_size), so that the ``page_size x width`` tile of one head of one page is
 contiguous. The reference keeps
 ``[layers, blocks, n_kv, block_size, head_dim]`` in 32-bit (cpp/src/cuda/cuda_backend.cu:852-871);
 here the element type is the engine's compute dtype.
@@ -54,7 +54,7 @@ class CacheStorage:
             if len({t.name for t in g.tensors}) != len(g.tensors):
                 raise ValueError(f"a cache need names a tensor twice: {[t.name for t in g.tensors]}")
             for e in g.entries:
-                self.pages[e] = {t.name: torch.zeros((num_pages, t.heads, page_size, t.width),
+                self.pages[e] = {t.name: torch.zeros((num_pages, t.heads, 1 if t.per_page else page_size, t.width),
                                                      dtype=t.dtype if t.dtype is not None else dtype, device=device)
                                  for t in g.tensors}
         # One slot more than there can be requests: the padding rows of a captured decode step read and write
@@ -88,8 +88,9 @@ class CacheStorage:
         return out
 
     def bytes_per_token(self) -> int:
+        """Of all entries; what a page keeps once is shared out among its tokens (rounded up)."""
         total = 0
         for per_entry in self.pages.values():
             for t in per_entry.values():
-                total += t.shape[1] * t.shape[3] * t.element_size()
-        return total
+                total += t.shape[1] * t.shape[2] * t.shape[3] * t.element_size()
+        return -(-total // self.page_size)

@@ -21,6 +21,10 @@ def add_model_args(p: argparse.ArgumentParser) -> None:
     p.add_argument("--random-weights", metavar="CONFIG_JSON", default=None,
                    help="write a random-weights model folder from this config.json file and use it")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    p.add_argument("--cache-dtype", default="auto", choices=["auto", "int8"], help="keys and values as --dtype, or in 8 bits")
+    p.add_argument("--weights", dest="weight_format", default="auto", choices=["auto", "int4"],
+                   help="matrices of attention and feed-forward as --dtype, or in 4 bits (quantized when the model is loaded)")
+    p.add_argument("--weight-group", type=int, default=64, choices=[32, 64, 128], help="int4: weights of a row that share a scale")
     p.add_argument("--block-size", "--page-size", dest="page_size", type=int, default=16,
                    help="tokens per cache page")
     p.add_argument("--num-blocks", "--num-pages", dest="num_pages", type=int, default=1024,
@@ -72,7 +76,8 @@ def main(argv=None) -> int:
     from ..sampling.params import SamplingParams
     model_dir = resolve_model_dir(args)
     model = load_model(model_dir, dtype=args.dtype, page_size=args.page_size, num_pages=args.num_pages,
-                       max_batch=1, max_tokens_per_step=args.max_tokens_per_step)
+                       max_batch=1, max_tokens_per_step=args.max_tokens_per_step, cache_dtype=args.cache_dtype,
+                       weight_format=args.weight_format, weight_group=args.weight_group)
     tok = load_tokenizer(model_dir, model.eos_token_id)
     try:
         tok.encode(args.prompt)

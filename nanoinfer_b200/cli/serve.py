@@ -26,7 +26,8 @@ def main(argv=None) -> int:
     from ..engine.scheduler import Request, Scheduler
     model_dir = resolve_model_dir(args)
     model = load_model(model_dir, dtype=args.dtype, page_size=args.page_size, num_pages=args.num_pages,
-                       max_batch=args.max_batch, max_tokens_per_step=args.max_tokens_per_step)
+                       max_batch=args.max_batch, max_tokens_per_step=args.max_tokens_per_step, cache_dtype=args.cache_dtype,
+                       weight_format=args.weight_format, weight_group=args.weight_group)
     tok = load_tokenizer(model_dir, model.eos_token_id)
     sched = Scheduler(model, max_batch=args.max_batch, lookahead=True)
     prompts = {}

@@ -17,6 +17,9 @@ _DTYPES = {"bfloat16": "bfloat16", "bf16": "bfloat16", "float32": "float32", "fp
 @dataclass(frozen=True)
 class EngineConfig:
     dtype: str = "bfloat16"          # "bfloat16": serving kernels; "float32": true 32-bit everywhere
+    cache_dtype: str = "auto"        # keys and values: "auto" as dtype; "int8" codes of 8 bits, a scale for each page and kv head
+    weight_format: str = "auto"      # matrices of attention and feed-forward: "auto" as dtype; "int4" codes of 4 bits, quantized at load
+    weight_group: int = 64           # int4: weights of a row that share a scale (32, 64 or 128)
     page_size: int = 16              # tokens per cache page
     num_pages: int = 0               # pages per cache group; 0 = size from max_cache_tokens
     max_cache_tokens: int = 0        # used when num_pages == 0
@@ -30,6 +33,12 @@ class EngineConfig:
         if self.dtype not in _DTYPES:
             raise ValueError(f"dtype must be one of {sorted(set(_DTYPES))}, got {self.dtype!r}")
         object.__setattr__(self, "dtype", _DTYPES[self.dtype])
+        if self.cache_dtype not in ("auto", "int8"):
+            raise ValueError(f"cache_dtype must be 'auto' or 'int8', got {self.cache_dtype!r}")
+        if self.weight_format not in ("auto", "int4"):
+            raise ValueError(f"weight_format must be 'auto' or 'int4', got {self.weight_format!r}")
+        if self.weight_group not in (32, 64, 128):
+            raise ValueError(f"weight_group must be 32, 64 or 128, got {self.weight_group!r}")
         if self.page_size <= 0:
             raise ValueError("page_size must be > 0")
         if self.max_batch <= 0:

@@ -47,8 +47,16 @@ class Engine:
             ops = load_kernels(engine_config.kernel_options).with_weights_ahead()      # the parts' matrices are parameters
         self.device = torch.device(engine_config.device)
         self.dtype = _TORCH_DTYPE[engine_config.dtype]
-        self.rt = Runtime(self.device, self.dtype, ops)
+        self.rt = Runtime(self.device, self.dtype, ops, engine_config.cache_dtype == "int8",
+                          engine_config.weight_group if engine_config.weight_format == "int4" else 0)
         self.model = DecoderModel(self.plan, tensors, self.rt)
+        if self.rt.cache_int8:
+            other = {type(m).__name__ for m in (self.model.layers[e.layer].mixer for e in self.model.schedule) if not getattr(m, "int8_cache", False) and m.cache_need()}
+            if other or not any(need for need, _, _ in self.model.cache_needs()):
+                raise ValueError(f"cache_dtype 'int8': the model {self.plan.architecture} keeps " + (f"the cache of {sorted(other)}, which has no 8-bit form"
+                                                                                                      if other else "no pages"))
+        if self.rt.weight_group and "int4" not in self.model.weight_breakdown():
+            raise ValueError(f"weight_format 'int4': no part of the model {self.plan.architecture} multiplies with 4-bit weights")
         self.storage = CacheStorage(self.model.cache_needs(), engine_config.resolved_num_pages(),
                                     engine_config.page_size, engine_config.max_batch, self.dtype, self.device)
         self.cache: CacheManager = self.storage.make_manager(engine_config.max_batch)

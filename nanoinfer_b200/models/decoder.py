@@ -13,6 +13,7 @@ import torch
 from ..parts.base import CacheNeed, LayerCache, Runtime, StateNeed, StepContext, normed_input, resolve_pending
 from ..parts.spec import ModelPlan, PartSpec
 from ..registry import get_arrangement, get_part
+from ..weights.int4 import Int4Matrix
 
 
 def _build_part(spec: PartSpec, tensors: Dict[str, torch.Tensor], rt: Runtime):
@@ -83,16 +84,17 @@ class DecoderModel:
         """dtype name -> (tensors, bytes) over the device tensors that the parts were given (a tied head counts once)."""
         out: Dict[str, Tuple[int, int]] = {}
         for t in self._weights:
-            name = str(t.dtype).replace("torch.", "")
+            int4 = isinstance(t, Int4Matrix)
+            name = "int4" if int4 else str(t.dtype).replace("torch.", "")
             n, b = out.get(name, (0, 0))
-            out[name] = (n + 1, b + t.numel() * t.element_size())
+            out[name] = (n + 1, b + (t.nbytes() if int4 else t.numel() * t.element_size()))
         return out
 
     def weight_bytes(self) -> Tuple[int, int]:
         """(bytes the weights take on the device, bytes they would take with every element in 32-bit): the pair
         that the reference reports (cpp/src/model.cpp:298-318)."""
-        actual = sum(t.numel() * t.element_size() for t in self._weights)
-        return actual, sum(t.numel() * 4 for t in self._weights)
+        actual = sum(b for _, b in self.weight_breakdown().values())
+        return actual, sum(4 * (t.shape[0] * t.shape[1] if isinstance(t, Int4Matrix) else t.numel()) for t in self._weights)
 
     # -- one step ------------------------------------------------------------------------------
     def forward(self, ctx: StepContext, caches: List[LayerCache],
@@ -123,16 +125,25 @@ class DecoderModel:
 
 
 class _SharingRuntime(Runtime):
-    """A runtime whose ``matrix`` / ``vector32`` return one device copy per source tensor."""
+    """A runtime whose ``matrix`` / ``weight`` / ``vector32`` return one device copy per source tensor."""
 
     def __init__(self, rt: Runtime, memo, made):
-        super().__init__(rt.device, rt.dtype, rt.ops)
+        super().__init__(rt.device, rt.dtype, rt.ops, rt.cache_int8, rt.weight_group)
         self._memo, self._made = memo, made
 
     def matrix(self, t: torch.Tensor) -> torch.Tensor:
         key = (id(t), "m")
         if key not in self._memo:
             self._memo[key] = (t, Runtime.matrix(self, t))
+            self._made.append(self._memo[key][1])
+        return self._memo[key][1]
+
+    def weight(self, t: torch.Tensor):
+        if not self.weight_group:
+            return self.matrix(t)
+        key = (id(t), "w")
+        if key not in self._memo:
+            self._memo[key] = (t, Runtime.weight(self, t))
             self._made.append(self._memo[key][1])
         return self._memo[key][1]
 

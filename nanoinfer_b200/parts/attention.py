@@ -27,6 +27,7 @@ class GroupedQueryAttention(Mixer):
     (0 = all keys), ``position`` (name of a shared position encoding), ``scale`` (optional).
     tensors: ``q_w k_w v_w o_w`` and, with bias, ``q_b k_b v_b``."""
 
+    int8_cache = True   # keeps its keys and values in 8 bits where the runtime says so
     graph_safe = True   # launches do not depend on which requests are in the batch
     accepts_lazy_norm = True   # its first projection can apply the norm while reading its input
 
@@ -59,16 +60,17 @@ class GroupedQueryAttention(Mixer):
         self.scale = float(p.get("scale", 1.0 / math.sqrt(float(self.head_dim))))
         self.position_name = str(p["position"])
         # One fused projection: rows [q | k | v].
-        self.w_qkv = rt.matrix(torch.cat([tensors["q_w"], tensors["k_w"], tensors["v_w"]], dim=0))
+        self.w_qkv = rt.weight(torch.cat([tensors["q_w"], tensors["k_w"], tensors["v_w"]], dim=0))
         self.b_qkv = None
         if p.get("bias"):
             self.b_qkv = rt.vector32(torch.cat([tensors["q_b"], tensors["k_b"], tensors["v_b"]], dim=0))
-        self.w_o = rt.matrix(tensors["o_w"])
+        self.w_o = rt.weight(tensors["o_w"])
         self.qkv_width = (self.heads + 2 * self.kv_heads) * self.head_dim
         self._rotary = None
 
     def cache_need(self) -> CacheNeed:
-        return CacheNeed.keys_and_values(self.kv_heads, self.head_dim, self.window)
+        need = CacheNeed.keys_and_values_int8 if self.rt.cache_int8 else CacheNeed.keys_and_values
+        return need(self.kv_heads, self.head_dim, self.window)
 
     def bind_positions(self, positions: Dict[str, PositionEncoding]) -> None:
         self._rotary = positions[self.position_name].rotary()
@@ -78,6 +80,9 @@ class GroupedQueryAttention(Mixer):
     def forward(self, h: torch.Tensor, residual32: torch.Tensor, ctx: StepContext, cache: LayerCache) -> None:
         m = h.shape[0]
         qkv = torch.empty((m, self.qkv_width), dtype=self.rt.dtype, device=h.device)
+        if self.rt.cache_int8:
+            self._forward_int8(h, qkv, residual32, ctx, cache)
+            return
         # projection, rotation of q and k, keys (rotated) and values into the pages
         self.ops.qkv_project(h, self.w_qkv, self.b_qkv, qkv, self.heads, self.kv_heads, self.head_dim, ctx.positions,
                              ctx.req_index, self._rotary, cache.block_table, cache.page_size, cache.k_pages,
@@ -85,6 +90,21 @@ class GroupedQueryAttention(Mixer):
         attn = torch.empty((m, self.heads * self.head_dim), dtype=self.rt.dtype, device=h.device)
         self.ops.attention(qkv, attn, self.heads, self.kv_heads, self.head_dim, self.scale, self.window,
                            ctx, cache.block_table, cache.page_size, cache.k_pages, cache.v_pages, own_kv=cache.writes)
+        self.ops.linear(attn, self.w_o, None, residual32, "add")
+
+    def _forward_int8(self, h, qkv: torch.Tensor, residual32: torch.Tensor, ctx: StepContext, cache: LayerCache) -> None:
+        """The same over a cache of 8 bits; a token reads its own key and value as the cache holds them, too."""
+        self.ops.linear(h, self.w_qkv, self.b_qkv, qkv, "store")
+        k_scales, v_scales = cache.pages["k_scale"], cache.pages["v_scale"]
+        attn = torch.empty((h.shape[0], self.heads * self.head_dim), dtype=self.rt.dtype, device=h.device)
+        if cache.writes:
+            self.ops.rope_store_int8(qkv, qkv[:, :self.heads * self.head_dim], self.heads, self.kv_heads, self.head_dim, ctx, self._rotary,
+                                     cache.block_table, cache.page_size, cache.k_pages, cache.v_pages, k_scales, v_scales)
+        else:       # (another entry's cache: the queries alone are rotated; rows of keys and values are nobody's)
+            self.ops.rope_store(qkv, self.heads, self.kv_heads, self.head_dim, ctx.positions, ctx.req_index, self._rotary, None, cache.page_size,
+                                None, None, False)
+        self.ops.attention_int8(qkv, attn, self.heads, self.kv_heads, self.head_dim, self.scale, self.window, ctx, cache.block_table,
+                                cache.page_size, cache.k_pages, cache.v_pages, k_scales, v_scales)
         self.ops.linear(attn, self.w_o, None, residual32, "add")
 
 

@@ -26,6 +26,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from ..weights.int4 import Int4Matrix
 from .spec import PartSpec
 
 
@@ -37,6 +38,12 @@ class Runtime:
     # The kernel library (csrc/lib.py: Kernels). An engine's reads the matrices given to its products ahead of the kernels before them: a
     # part that multiplies with a matrix that a kernel writes takes ``ops.with_weights_ahead(False)`` for it, and more than 16 tokens.
     ops: object
+    cache_int8: bool = False      # attention keeps its keys and values in 8 bits
+    weight_group: int = 0         # ``weight`` makes matrices of 4 bits, this many weights to a scale; 0: it is ``matrix``
+
+    def weight(self, t: torch.Tensor):
+        """A matrix operand that only ``linear``, ``linear_swiglu`` and ``qkv_project`` read: as ``matrix``, or in 4 bits."""
+        return Int4Matrix.quantize(t.to(self.device), self.weight_group) if self.weight_group else self.matrix(t)
 
     def matrix(self, t: torch.Tensor) -> torch.Tensor:
         """A matrix operand: compute dtype, contiguous, on the device."""
@@ -50,11 +57,13 @@ class Runtime:
 @dataclass(frozen=True)
 class PagedTensor:
     """One tensor that a mixer keeps per token in the paged cache: ``heads x width`` elements for every position, laid
-    out per page as ``[heads, page_size, width]``. ``dtype`` None = the engine's compute dtype."""
+    out per page as ``[heads, page_size, width]``, or with ``per_page`` once for a page, as ``[heads, 1, width]``. ``dtype`` None =
+    the engine's compute dtype."""
     name: str
     heads: int
     width: int
     dtype: Optional[torch.dtype] = None
+    per_page: bool = False
 
 
 @dataclass(frozen=True)
@@ -71,6 +80,13 @@ class CacheNeed:
     def keys_and_values(kv_heads: int, head_dim: int, window: int = 0) -> "CacheNeed":
         """The two-tensor case of attention: ``k`` and ``v`` of the same shape in the compute dtype."""
         return CacheNeed((PagedTensor("k", kv_heads, head_dim), PagedTensor("v", kv_heads, head_dim)), window)
+
+    @staticmethod
+    def keys_and_values_int8(kv_heads: int, head_dim: int, window: int = 0) -> "CacheNeed":
+        """Keys and values as codes of 8 bits, and the scales of every page and kv head."""
+        return CacheNeed((PagedTensor("k", kv_heads, head_dim, torch.int8), PagedTensor("v", kv_heads, head_dim, torch.int8),
+                          PagedTensor("k_scale", kv_heads, 1, torch.float32, per_page=True),
+                          PagedTensor("v_scale", kv_heads, 1, torch.float32, per_page=True)), window)
 
     def group_key(self):
         """Entries with equal keys share a cache group (one block table per request)."""
@@ -140,7 +156,7 @@ def resolve_pending(x32: torch.Tensor, ctx: "StepContext") -> None:
 @dataclass
 class LayerCache:
     """The cache of one schedule entry, as its mixer sees it."""
-    pages: Dict[str, torch.Tensor]      # PagedTensor.name -> [num_pages, heads, page_size, width]
+    pages: Dict[str, torch.Tensor]      # PagedTensor.name -> [num_pages, heads, page_size (per_page: 1), width]
     block_table: Optional[torch.Tensor]  # [R, max_pages] int32, -1 where no page is held
     page_size: int
     writes: bool                        # False when this entry reads another entry's cache
@@ -238,6 +254,8 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    int8_cache = False      # whether ``cache_need`` goes by the runtime's ``cache_int8``
+
     def cache_need(self) -> Optional[CacheNeed]:
         return None
 

@@ -47,8 +47,8 @@ class SwiGLU(FeedForward):
         if self.act not in ("silu", "gelu_tanh") or (self.act != "silu" and self.glu is not None):
             raise ValueError(f"unknown activation '{self.act}', or one that takes no constants")
         # One fused operand: rows [gate | up].
-        self.w_gate_up = rt.matrix(torch.cat([tensors["gate_w"], tensors["up_w"]], dim=0))
-        self.w_down = rt.matrix(tensors["down_w"])
+        self.w_gate_up = rt.weight(torch.cat([tensors["gate_w"], tensors["up_w"]], dim=0))
+        self.w_down = rt.weight(tensors["down_w"])
 
     def forward(self, h: torch.Tensor, residual32: torch.Tensor, ctx: StepContext) -> None:
         act = torch.empty((h.shape[0], self.intermediate), dtype=self.rt.dtype, device=h.device)

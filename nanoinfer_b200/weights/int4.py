@@ -65,7 +65,8 @@ class Int4Matrix:
         codes, scales = [], []
         for rows in w.split(max(1, (1 << 24) // k)):            # (a large matrix is not copied whole to 32 bits)
             x = rows.float().reshape(-1, k // group, group)
-            largest = x.abs().amax(dim=2) / 7.0
+            largest = x.abs().amax(dim=2)
+            largest = largest / torch.full_like(largest, 7.0)       # (by a number it is a product with 1/7 on some devices, and another scale)
             if not bool(torch.isfinite(largest).all()):
                 raise ValueError("a matrix with undefined or infinite elements cannot be quantized")
             s = ((largest.view(torch.int32) + 0x7FFFF) & ~0x7FFFF).view(torch.float32)
