@@ -30,6 +30,7 @@ struct Args {
     const float* k_scales; const float* v_scales; float* part_o; float* part_ml;        // [2 * shares][n_rep][head_dim], [2 * shares][n_rep][2]
     int q_stride, bt_stride, bt_width, page_size, shift, num_pages, n_tokens, heads, kv_heads, n_rep, head_dim, window;
     int csize, shares;              // CTAs of a cluster and 0 shares, or the CTAs that all chunks are dealt to
+    int early;                      // pages before the one that a token's own key lies in are no running kernel's results
     float scale;
 };
 
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(MERGE_THREADS)
 merge_int8_kernel(T* __restrict__ out, const Args a) {
     __shared__ float s_acc[MERGE_THREADS], s_m[MERGE_THREADS], s_l[MERGE_THREADS];
     const int token = blockIdx.y, head = blockIdx.x, kvh = head / a.n_rep, row = head - kvh * a.n_rep, lane = threadIdx.x & 31, hd = a.head_dim;
+    pdl_launch_dependents();
     int all = 0, before = 0;                        // chunks of a kv head
     for (int t = lane; t < a.n_tokens; t += 32) {
         const int n = Keys<CH>(a, t).n;
@@ -187,7 +189,6 @@ merge_int8_kernel(T* __restrict__ out, const Args a) {
     const int n = Keys<CH>(a, token).n, begin = __reduce_add_sync(0xffffffffu, before) * a.kv_heads + kvh * n;
     const int per = max(1, (all + a.shares - 1) / a.shares), b0 = begin / per, parts = n ? (begin + n - 1) / per - b0 + 1 : 0;
     pdl_wait();             // (the lengths are the step's inputs)
-    pdl_launch_dependents();
     if (parts == 1) return;
     const int threads = blockDim.x;
     const int turns = parts <= 8 ? 1 : max(1, threads / hd);
@@ -346,9 +347,50 @@ attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat1
             ids[i] = chunk + lane < piece.end && key <= piece.p && key + ID_KEYS > piece.lo ? page_at(a, bt, key, slot) : -1;
         }
     };
+    const long long page_bytes = (long long)a.kv_heads * a.page_size * HD;
+    // A page that the request does not hold is read as the pool's first with scales of 0: nothing leaves the pool.
+    auto send = [&](int chunk, int stage) {
+        const unsigned dst = ring + stage * C::STAGE;
+        const int from = (chunk - piece.begin) & 31;
+        const signed char* k_lane = a.k_pages + (size_t)piece.kvh * a.page_size * HD + g * HD + t * 16;
+        const signed char* v_lane = a.v_pages + (size_t)piece.kvh * a.page_size * HD + 2 * t * HD + g * (HD / 8);
+#pragma unroll
+        for (int i = 0; i < IDS; ++i) {
+            const int key = chunk * C::CHUNK + warp * STEP + i * ID_KEYS;
+            const int page = __shfl_sync(0xffffffffu, ids[i], from);
+            const bool held = page >= 0;
+            const int slot = !held ? 0 : a.shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
+            const long long at = max(page, 0) * page_bytes + slot * HD;
+            if (lane < 2) {
+                const size_t block = (size_t)max(page, 0) * a.kv_heads + piece.kvh;
+                copy_async_or_zero(dst + S_AT + i * 8 + lane * 4, (lane ? a.v_scales : a.k_scales) + block, held);
+            }
+#pragma unroll
+            for (int h = 0; h < 2 / H; ++h) {
+                const int part = i * (2 / H) + h;               // 8 keys
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j) copy_async<16>(dst + (part * (HD / 64) + j) * 512 + lane * 16, k_lane + at + h * 8 * HD + j * 64);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    copy_async<HD / 8>(dst + V_AT + (part * 2 + j) * (32 * HD / 8) + lane * (HD / 8), v_lane + at + (h * 8 + j) * HD);
+            }
+        }
+    };
     bool more = piece.first(a, lane);
     if (more) look_up(piece.begin);         // lengths and tables are the step's inputs; queries, keys, values and scales are kernels' results
+    // Where the caller says so, pages before the one that the token's own key goes to are sent for before the wait.
+    int sent = 0;
+    if (a.early && more) {
+        const int own_page = piece.p >= 0 ? piece.p - piece.p % a.page_size : 0;
+        while (sent < STAGES - 1 && piece.begin + sent < piece.end && (piece.begin + sent + 1) * C::CHUNK <= own_page) {
+            send(piece.begin + sent, sent);
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+            ++sent;
+        }
+    }
     pdl_wait();
+    // (Let in at this kernel's first instruction the one behind takes places that its own CTAs could have: 8 tokens of 4,096 keys in a chain
+    // of such calls 9.4 us instead of 6.6, 64 of 200 to 4,000 24 instead of 16.)
     pdl_launch_dependents();
     while (more) {
         const int token = piece.token, kvh = piece.kvh, p = piece.p, lo = piece.lo;
@@ -363,41 +405,11 @@ attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat1
                 for (int j = 0; j < 2; ++j)
                     raw[kk][nh][j] = head < a.n_rep ? *reinterpret_cast<const unsigned*>(qp + (kk >> 2) * 64 + (kk & 3) * 4 + 2 * j) : 0u;
         }
-        const long long page_bytes = (long long)a.kv_heads * a.page_size * HD;
-        const signed char* k_lane = a.k_pages + (size_t)kvh * a.page_size * HD + g * HD + t * 16;
-        const signed char* v_lane = a.v_pages + (size_t)kvh * a.page_size * HD + 2 * t * HD + g * (HD / 8);
-
-        // A page that the request does not hold is read as the pool's first with scales of 0: nothing leaves the pool.
-        auto send = [&](int chunk, int stage) {
-            const unsigned dst = ring + stage * C::STAGE;
-            const int from = (chunk - piece.begin) & 31;
-#pragma unroll
-            for (int i = 0; i < IDS; ++i) {
-                const int key = chunk * C::CHUNK + warp * STEP + i * ID_KEYS;
-                const int page = __shfl_sync(0xffffffffu, ids[i], from);
-                const bool held = page >= 0;
-                const int slot = !held ? 0 : a.shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
-                const long long at = max(page, 0) * page_bytes + slot * HD;
-                if (lane < 2) {
-                    const size_t block = (size_t)max(page, 0) * a.kv_heads + kvh;
-                    copy_async_or_zero(dst + S_AT + i * 8 + lane * 4, (lane ? a.v_scales : a.k_scales) + block, held);
-                }
-#pragma unroll
-                for (int h = 0; h < 2 / H; ++h) {
-                    const int part = i * (2 / H) + h;               // 8 keys
-#pragma unroll
-                    for (int j = 0; j < HD / 64; ++j) copy_async<16>(dst + (part * (HD / 64) + j) * 512 + lane * 16, k_lane + at + h * 8 * HD + j * 64);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        copy_async<HD / 8>(dst + V_AT + (part * 2 + j) * (32 * HD / 8) + lane * (HD / 8), v_lane + at + (h * 8 + j) * HD);
-                }
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) {
+        for (int i = sent; i < STAGES - 1; ++i) {
             if (piece.begin + i < piece.end) send(piece.begin + i, i);
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
+        sent = 0;
 
         // Q^T as the column operand, its dims in the order in which the key rows' pieces hold them. A head is scaled by a power of two
         // so that its largest element lies in 2^12 .. 2^13: 16-bit floats then hold every element that counts exactly.
@@ -678,10 +690,11 @@ attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, con
     float* cta_ml = corr + n_rep;               // [n_rep][2]
     __shared__ float ks[GT], vs[GT];
     __shared__ long long from[GT];              // where a key's codes are; -1: nowhere
-    pdl_wait();
     pdl_launch_dependents();
     Pieces<GT> piece;
-    for (bool more = piece.first(a, tid & 31); more; more = piece.next(a, tid & 31)) {
+    bool more = piece.first(a, tid & 31);
+    pdl_wait();
+    for (; more; more = piece.next(a, tid & 31)) {
     const int token = piece.token, kvh = piece.kvh, p = piece.p, lo = piece.lo;
     const int* bt = a.block_table + (size_t)token * a.bt_stride;
     for (int i = tid; i < n_rep * hd; i += GEN_THREADS) {
@@ -817,8 +830,8 @@ NIB_API int nib_attention_int8_decode_kind(int heads, int kv_heads, int head_dim
 struct NibAttendInt8 {
     const void* q; void* out; const int* ctx_lens; const int* block_table; const void* k_pages; const void* v_pages; const float* k_scales;
     const float* v_scales; float* part_o; float* part_ml;
-    int q_stride, bt_stride, bt_width, page_size, num_pages, n_tokens, heads, kv_heads, head_dim, window, ctas, shares, dtype, pad;
-    float scale; int pad2;
+    int q_stride, bt_stride, bt_width, page_size, num_pages, n_tokens, heads, kv_heads, head_dim, window, ctas, shares, dtype, early;
+    float scale; int pad;
 };
 
 // Attention of n_tokens single tokens (token i is request i, at position ctx_lens[i] - 1) whose keys and values are in the pages.
@@ -844,7 +857,7 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     int shift = -1;
     if ((page_size & (page_size - 1)) == 0) for (shift = 0; (1 << shift) < page_size;) ++shift;
     const Args a{c.ctx_lens, c.block_table, (const signed char*)c.k_pages, (const signed char*)c.v_pages, c.k_scales, c.v_scales, c.part_o, c.part_ml,
-                 c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, n_tokens, heads, kv_heads, heads / kv_heads, head_dim, c.window, c.ctas, c.shares, c.scale};
+                 c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, n_tokens, heads, kv_heads, heads / kv_heads, head_dim, c.window, c.ctas, c.shares, c.early, c.scale};
     int rc;
     // (rows and pools that lie off the pieces that a thread reads and writes at a time go to the general kernel)
     if (kind == 1 && ((uintptr_t)q & 3) == 0 && c.q_stride % 2 == 0 && ((uintptr_t)out & 7) == 0 && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0) {

@@ -13,8 +13,11 @@
 // scales of any value every growth could add another half step. An element that is not finite makes the block's scale NaN:
 // whoever reads the block sees that it is undefined. Slots behind the last token keep their codes.
 //
-// The rotated key is formed in 64 bits (bfloat16 or float times float is exact there): a code is a rounding to whole steps,
-// and a key that lies between two must not change its side with the order of the products.
+// A code is a rounding to whole steps, and a key that lies between two must not change its side with the order of the rotation's
+// products: an element is formed as the sum of a float and what its rounding left (the products' errors by a fused multiply-add, the
+// sum's by the two-sum), some 48 bits, of which the second part decides ties. (In 64 bits it was twice as slow: conversions.)
+//
+// What bounds it: a decode step's launch and three dependent loads; for a prompt's portion the bytes, queries above all.
 #include "common.cuh"
 
 namespace {
@@ -33,11 +36,11 @@ __device__ __forceinline__ float block_scale(float a) {
 
 // Where a unit of work lies: the tokens of one request in one page. Units are counted request by request; request r has at
 // most (q_len + page_size - 2) / page_size + 1 of them, whatever its position.
-struct Unit { int row, count, slot; long long page; };
+struct Unit { int row, count, slot, pos; long long page; };       // pos: the first token's position
 
 __device__ __forceinline__ Unit find_unit(int u, const int* __restrict__ q_start, const int* __restrict__ ctx_lens, int n_req,
                                           const int* __restrict__ block_table, int bt_stride, int bt_width, int page_size, int num_pages, int lane) {
-    Unit out{0, 0, 0, -1};
+    Unit out{0, 0, 0, 0, -1};
     int base = 0;
     for (int r0 = 0; r0 < n_req; r0 += 32) {
         const int r = r0 + lane;
@@ -63,6 +66,7 @@ __device__ __forceinline__ Unit find_unit(int u, const int* __restrict__ q_start
             out.row = row + (lo - first);
             out.count = hi - lo;
             out.slot = lo - lp * page_size;
+            out.pos = lo;
             out.page = page >= 0 && page < num_pages ? page : -1;
             return out;
         }
@@ -72,6 +76,33 @@ __device__ __forceinline__ Unit find_unit(int u, const int* __restrict__ q_start
 }
 
 template <typename T, int V> struct Vec;
+template <> struct Vec<__nv_bfloat16, 8> {
+    static __device__ __forceinline__ void load(float (&f)[8], const __nv_bfloat16* p) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[8]) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned*>(&v);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Vec<float, 8> {
+    static __device__ __forceinline__ void load(float (&f)[8], const float* p) {
+        *reinterpret_cast<float4*>(f) = reinterpret_cast<const float4*>(p)[0];
+        *reinterpret_cast<float4*>(f + 4) = reinterpret_cast<const float4*>(p)[1];
+    }
+    static __device__ __forceinline__ void store(float* p, const float (&f)[8]) {
+        reinterpret_cast<float4*>(p)[0] = *reinterpret_cast<const float4*>(f);
+        reinterpret_cast<float4*>(p)[1] = *reinterpret_cast<const float4*>(f + 4);
+    }
+};
 template <> struct Vec<__nv_bfloat16, 4> {
     static __device__ __forceinline__ void load(float (&f)[4], const __nv_bfloat16* p) {
         const uint2 u = *reinterpret_cast<const uint2*>(p);
@@ -84,22 +115,38 @@ template <> struct Vec<float, 4> {
 };
 template <typename T> struct Vec<T, 1> {
     static __device__ __forceinline__ void load(float (&f)[1], const T* p) { f[0] = Elem<T>::load(p); }
+    static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { Elem<T>::store(p, f[0]); }
 };
 
 template <int V> __device__ __forceinline__ void store_codes(signed char* p, const int (&c)[V]) {
-    if (V == 4) {
-        *reinterpret_cast<unsigned*>(p) = (unsigned)(c[0] & 0xff) | ((unsigned)(c[V > 1 ? 1 : 0] & 0xff) << 8) |
-                                          ((unsigned)(c[V > 2 ? 2 : 0] & 0xff) << 16) | ((unsigned)(c[V > 3 ? 3 : 0] & 0xff) << 24);
+    if constexpr (V == 4) {
+        *reinterpret_cast<unsigned*>(p) = (unsigned)(c[0] & 0xff) | ((unsigned)(c[1] & 0xff) << 8) | ((unsigned)(c[2] & 0xff) << 16) | ((unsigned)(c[3] & 0xff) << 24);
     } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = (signed char)c[i];
+        p[0] = (signed char)c[0];
     }
 }
 
-// rint(x / s) within -127..127; inv = 1 / s exactly. Of a NaN: 0 (its block's scale says so).
-__device__ __forceinline__ int code_of(double x, double inv) {
-    const double y = fmin(fmax(x * inv, -127.0), 127.0);
-    return y == y ? __double2int_rn(y) : 0;
+// a * b + c * d as hi + lo, hi the nearest float.
+struct Two { float hi, lo; };
+__device__ __forceinline__ Two sum_of_products(float a, float b, float c, float d) {
+    const float p = __fmul_rn(a, b), pe = __fmaf_rn(a, b, -p), q = __fmul_rn(c, d), qe = __fmaf_rn(c, d, -q);
+    const float s = __fadd_rn(p, q), bb = __fsub_rn(s, p), se = __fadd_rn(__fsub_rn(p, __fsub_rn(s, bb)), __fsub_rn(q, bb));
+    const float e = __fadd_rn(se, __fadd_rn(pe, qe)), hi = __fadd_rn(s, e);
+    return {hi, __fsub_rn(e, __fsub_rn(hi, s))};
+}
+// The magnitude of hi + lo rounded up to a float, as an integer, in whose order a NaN's bits are above everything. (127 * 2^e is a
+// float, so the comparison with it stays what it is.)
+__device__ __forceinline__ unsigned magnitude_up(const Two& y) {
+    const unsigned bits = __float_as_uint(y.hi) & 0x7fffffffu;
+    return bits + ((y.lo != 0.f && (y.lo > 0.f) == (y.hi > 0.f) && bits < 0x7f800000u) ? 1u : 0u);
+}
+// rint((hi + lo) / s) within -127..127, inv = 1 / s, a power of two: the product with it is exact. Of a NaN: 0 (its block's scale
+// says so).
+__device__ __forceinline__ int code_of(const Two& y, float inv) {
+    const float v = fminf(fmaxf(__fmul_rn(y.hi, inv), -127.f), 127.f);          // (a NaN becomes a bound; the scale is what says so)
+    float r = rintf(v);
+    if (fabsf(v - r) == 0.5f && y.lo != 0.f) r = y.lo > 0.f ? ceilf(v) : floorf(v);
+    return (int)r;
 }
 
 constexpr int KV_WARPS = 4;
@@ -112,55 +159,57 @@ struct AppendArgs {
     int units, kv_blocks;       // the first kv_blocks CTAs append, a warp for each (unit, kv head, keys or values); the others rotate queries
 };
 
-// V: elements of a chunk (4, or 1 where widths or addresses do not allow it).
-template <typename T, int V>
-__global__ void __launch_bounds__(Q_THREADS)
+// WIDE: chunks of 8 elements of queries and 4 of keys and values; 1 where widths or addresses do not allow it.
+// Keys and values: a warp for each (unit, kv head, keys or values), two items a lane at a time, whose loads are all on their way
+// before the first is used. Twice: for the largest magnitude, then for the codes (the second time the rows come from L1).
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(Q_THREADS, 8)
 append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_out may be qkv)
+    constexpr int VQ = WIDE ? 8 : 1, V = WIDE ? 4 : 1, B = 2;
     const int half = a.rot >> 1, hd = a.head_dim, lane = threadIdx.x & 31;
-    // This kernel lets the one behind it in only after its own wait: whatever starts early behind it then knows that everything
-    // before it in the stream is complete (the attention reads the pages of earlier steps on that ground).
-    pdl_wait();
-    pdl_launch_dependents();
     if ((int)blockIdx.x >= a.kv_blocks) {
-        // ---- queries: an item is a chunk of pairs (or a chunk beyond the rotated width) of one head of one token
-        const int per_head = half / V + (hd - a.rot) / V;
-        const long long items = (long long)a.m * a.heads * per_head;
-        const long long i = (long long)(blockIdx.x - a.kv_blocks) * Q_THREADS + threadIdx.x;
-        if (i >= items) return;
-        const int c = (int)(i % per_head);
-        const long long th = i / per_head;
-        const int head = (int)(th % a.heads), tok = (int)(th / a.heads);
-        const T* p = qkv + (size_t)tok * a.q_stride + (size_t)head * hd;
-        T* o = q_out + (size_t)tok * a.out_stride + (size_t)head * hd;
-        float x1[V], x2[V];
-        if (c < half / V) {
-            const int d = c * V, pos = a.positions[tok];
-            Vec<T, V>::load(x1, p + d);
-            Vec<T, V>::load(x2, p + d + half);
-            const bool known = pos >= 0 && pos < a.table_rows;
-            float cs[V], sn[V];
+        // ---- queries: a CTA a token; an item is a chunk of pairs (or a chunk beyond the rotated width) of a head
+        const int tok = blockIdx.x - a.kv_blocks, pos = a.positions[tok];       // (positions and tables are the step's inputs)
+        const int pairs = half / VQ, tails = (hd - a.rot) / VQ;
+        const bool known = pos >= 0 && pos < a.table_rows;
+        const T* row = qkv + (size_t)tok * a.q_stride;
+        T* to = q_out + (size_t)tok * a.out_stride;
+        bool waited = false;
+        for (int i = threadIdx.x; i < a.heads * pairs; i += Q_THREADS) {
+            const int head = i / pairs, d = (i - head * pairs) * VQ;
+            float x1[VQ], x2[VQ], cs[VQ], sn[VQ], y1[VQ], y2[VQ];
             const size_t at = (size_t)(known ? pos : 0) * half + d;
-            Vec<float, V>::load(cs, a.cos_t + at);
-            Vec<float, V>::load(sn, a.sin_t + at);
+            Vec<float, VQ>::load(cs, a.cos_t + at);
+            Vec<float, VQ>::load(sn, a.sin_t + at);
+            if (!waited) { pdl_wait(); pdl_launch_dependents(); waited = true; }
+            Vec<T, VQ>::load(x1, row + (size_t)head * hd + d);
+            Vec<T, VQ>::load(x2, row + (size_t)head * hd + d + half);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                Elem<T>::store(o + d + j, known ? x1[j] * cs[j] - x2[j] * sn[j] : NAN);
-                Elem<T>::store(o + d + half + j, known ? x2[j] * cs[j] + x1[j] * sn[j] : NAN);
+            for (int j = 0; j < VQ; ++j) {
+                y1[j] = known ? x1[j] * cs[j] - x2[j] * sn[j] : NAN;
+                y2[j] = known ? x2[j] * cs[j] + x1[j] * sn[j] : NAN;
             }
-        } else {
-            const int d = a.rot + (c - half / V) * V;
-            Vec<T, V>::load(x1, p + d);
-#pragma unroll
-            for (int j = 0; j < V; ++j) Elem<T>::store(o + d + j, x1[j]);
+            Vec<T, VQ>::store(to + (size_t)head * hd + d, y1);
+            Vec<T, VQ>::store(to + (size_t)head * hd + d + half, y2);
+        }
+        if (!waited) pdl_wait();
+        for (int i = threadIdx.x; i < a.heads * tails; i += Q_THREADS) {
+            const int head = i / tails, d = a.rot + (i - head * tails) * VQ;
+            float x[VQ];
+            Vec<T, VQ>::load(x, row + (size_t)head * hd + d);
+            Vec<T, VQ>::store(to + (size_t)head * hd + d, x);
         }
         return;
     }
-    // ---- keys and values
-    const int job = blockIdx.x * KV_WARPS + (threadIdx.x >> 5);
-    const int per_unit = 2 * a.kv_heads;
-    if (job >= a.units * per_unit) return;
+    const int job = blockIdx.x * KV_WARPS + (threadIdx.x >> 5), per_unit = 2 * a.kv_heads;
     const int u = job / per_unit, kvh = (job - u * per_unit) >> 1, values = job & 1;
-    const Unit unit = find_unit(u, a.q_start, a.ctx_lens, a.n_req, a.block_table, a.bt_stride, a.bt_width, a.page_size, a.num_pages, lane);
+    Unit unit{0, 0, 0, 0, -1};
+    if (job < a.units * per_unit)           // (lengths and tables, too)
+        unit = find_unit(u, a.q_start, a.ctx_lens, a.n_req, a.block_table, a.bt_stride, a.bt_width, a.page_size, a.num_pages, lane);
+    // (The attention behind is let in only now: its CTAs, placed while the kernel before this one still holds its SMs, would share few of
+    // them. 8 tokens of 4,096 keys, 28 heads of 128, both calls: 17 us, and 21 let in at once.)
+    pdl_wait();
+    pdl_launch_dependents();
     if (unit.page < 0) return;
     const size_t block = (size_t)unit.page * a.kv_heads + kvh;
     signed char* codes = (values ? a.v_pages : a.k_pages) + block * a.page_size * hd;
@@ -170,47 +219,43 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
     const int rot = values ? 0 : a.rot, pairs = (rot >> 1) / V, per_token = pairs + (hd - rot) / V;
     const int items = unit.count * per_token;
 
-    // the two chunks of an item (the second only of a rotated pair), in 64 bits
-    auto item = [&](int i, int& tok, int& d, bool& pair, double (&y1)[V], double (&y2)[V]) {
-        tok = i / per_token;
-        const int c = i - tok * per_token;
-        pair = c < pairs;
-        d = pair ? c * V : rot + (c - pairs) * V;
-        const T* p = rows + (size_t)tok * a.q_stride;
-        float x1[V], x2[V];
-        Vec<T, V>::load(x1, p + d);
-        if (pair) {
-            Vec<T, V>::load(x2, p + d + half);
-            const int pos = a.positions[unit.row + tok];
-            const bool known = pos >= 0 && pos < a.table_rows;
-            float cs[V], sn[V];
-            const size_t at = (size_t)(known ? pos : 0) * half + d;
-            Vec<float, V>::load(cs, a.cos_t + at);
-            Vec<float, V>::load(sn, a.sin_t + at);
+    struct Item { float x1[V], x2[V], cs[V], sn[V]; int row, d; bool pair; };       // the second chunk only of a rotated pair
+    auto load = [&](Item& it, int i) {
+        it.row = i / per_token;
+        const int c = i - it.row * per_token;
+        it.pair = c < pairs;
+        it.d = it.pair ? c * V : rot + (c - pairs) * V;
+        const T* p = rows + (size_t)it.row * a.q_stride;
+        Vec<T, V>::load(it.x1, p + it.d);
+        if (it.pair) {
+            Vec<T, V>::load(it.x2, p + it.d + half);
+            const int pos = unit.pos + it.row;
+            const size_t at = (size_t)min(pos, a.table_rows - 1) * half + it.d;
+            Vec<float, V>::load(it.cs, a.cos_t + at);
+            Vec<float, V>::load(it.sn, a.sin_t + at);
+            if (pos >= a.table_rows) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const double c64 = known ? (double)cs[j] : (double)NAN, s64 = sn[j];
-                y1[j] = (double)x1[j] * c64 - (double)x2[j] * s64;
-                y2[j] = (double)x2[j] * c64 + (double)x1[j] * s64;
+                for (int j = 0; j < V; ++j) it.cs[j] = NAN;
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) y1[j] = y2[j] = (double)x1[j];
         }
     };
-    // the largest magnitude, rounded up to 32 bits (127 * 2^e is one of those numbers, so the comparison with it stays what it
-    // is); as an integer, in whose order a NaN's bits are above everything
+    auto first_of = [&](const Item& it, int j) { return it.pair ? sum_of_products(it.x1[j], it.cs[j], -it.x2[j], it.sn[j]) : Two{it.x1[j], 0.f}; };
+    auto second_of = [&](const Item& it, int j) { return sum_of_products(it.x2[j], it.cs[j], it.x1[j], it.sn[j]); };
+
+    Item it[B];
     unsigned top = 0;
-    for (int i = lane; i < items; i += 32) {
-        int tok, d;
-        bool pair;
-        double y1[V], y2[V];
-        item(i, tok, d, pair, y1, y2);
+    for (int i0 = lane; i0 < items; i0 += 32 * B) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            top = max(top, __float_as_uint(__double2float_ru(fabs(y1[j]))) & 0x7fffffffu);
-            top = max(top, __float_as_uint(__double2float_ru(fabs(y2[j]))) & 0x7fffffffu);
-        }
+        for (int b = 0; b < B; ++b) if (i0 + 32 * b < items) load(it[b], i0 + 32 * b);
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (i0 + 32 * b < items) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    top = max(top, magnitude_up(first_of(it[b], j)));
+                    if (it[b].pair) top = max(top, magnitude_up(second_of(it[b], j)));
+                }
+            }
     }
     top = __reduce_max_sync(0xffffffffu, top);
     float scale = block_scale(__uint_as_float(top));
@@ -222,21 +267,26 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
             for (int i = lane; i < unit.slot * hd; i += 32) codes[i] = (signed char)__float2int_rn((float)codes[i] * by);
         }
     }
-    const double inv = 1.0 / (double)scale;
-    for (int i = lane; i < items; i += 32) {
-        int tok, d, c[V];
-        bool pair;
-        double y1[V], y2[V];
-        item(i, tok, d, pair, y1, y2);
-        signed char* dst = codes + (size_t)(unit.slot + tok) * hd + d;
+    const float inv = 1.0f / scale;
+    for (int i0 = lane; i0 < items; i0 += 32 * B) {
+        if (items > 32 * B) {           // (else the items are still at hand)
 #pragma unroll
-        for (int j = 0; j < V; ++j) c[j] = code_of(y1[j], inv);
-        store_codes<V>(dst, c);
-        if (pair) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) c[j] = code_of(y2[j], inv);
-            store_codes<V>(dst + half, c);
+            for (int b = 0; b < B; ++b) if (i0 + 32 * b < items) load(it[b], i0 + 32 * b);
         }
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (i0 + 32 * b < items) {
+                signed char* dst = codes + (size_t)(unit.slot + it[b].row) * hd + it[b].d;
+                int c[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) c[j] = code_of(first_of(it[b], j), inv);
+                store_codes<V>(dst, c);
+                if (it[b].pair) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) c[j] = code_of(second_of(it[b], j), inv);
+                    store_codes<V>(dst + half, c);
+                }
+            }
     }
     if (lane == 0) *scale_at = scale;
 }
@@ -271,8 +321,8 @@ template <> __device__ __forceinline__ void store16<__nv_bfloat16>(__nv_bfloat16
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 unpack_int8_kernel(const signed char* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, long long items, int per_block) {
-    pdl_wait();
     pdl_launch_dependents();
+    pdl_wait();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= items) return;
     const float s = __ldg(scales + i / per_block);
@@ -329,13 +379,10 @@ gather_int8_kernel(const signed char* __restrict__ k_pages, const signed char* _
     }
 }
 
-template <typename T, int V>
+template <typename T, bool WIDE>
 int launch_append(const void* qkv, void* q_out, const AppendArgs& a, cudaStream_t stream) {
-    const int per_head = (a.rot >> 1) / V + (a.head_dim - a.rot) / V;
-    const long long q_blocks = ((long long)a.m * a.heads * per_head + Q_THREADS - 1) / Q_THREADS;
-    NIB_REQUIRE(q_blocks + a.kv_blocks < (1LL << 31) - 1, "rope_store_int8: too many elements for one launch");
-    NIB_CUDA(launch_pdl(append_int8_kernel<T, V>, dim3((unsigned)(q_blocks + a.kv_blocks)), dim3(Q_THREADS), (size_t)0, stream,
-                        (const T*)qkv, (T*)q_out, a));
+    NIB_REQUIRE((long long)a.m + a.kv_blocks < (1LL << 31) - 1, "rope_store_int8: too many tokens for one launch");
+    NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE>, dim3((unsigned)(a.m + a.kv_blocks)), dim3(Q_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
     return 0;
 }
 
@@ -366,11 +413,11 @@ NIB_API int nib_rope_store_int8(const void* args, cudaStream_t stream) {
     const long long jobs = (long long)c.units * 2 * c.kv_heads;
     NIB_REQUIRE(jobs < (1LL << 31) - KV_WARPS, "rope_store_int8: too many pages for one launch");
     a.kv_blocks = (int)((jobs + KV_WARPS - 1) / KV_WARPS);
-    const int esize = c.dtype == NIB_F32 ? 4 : 2;
-    const bool wide = (c.rot / 2) % 4 == 0 && c.head_dim % 4 == 0 && c.q_stride % 4 == 0 && ((uintptr_t)c.qkv) % (4 * esize) == 0 &&
-                      (((uintptr_t)c.cos_t | (uintptr_t)c.sin_t) & 15) == 0 && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 3) == 0;
-    if (c.dtype == NIB_F32) return wide ? launch_append<float, 4>(c.qkv, c.q_out, a, stream) : launch_append<float, 1>(c.qkv, c.q_out, a, stream);
-    return wide ? launch_append<__nv_bfloat16, 4>(c.qkv, c.q_out, a, stream) : launch_append<__nv_bfloat16, 1>(c.qkv, c.q_out, a, stream);
+    const bool wide = (c.rot / 2) % 8 == 0 && c.head_dim % 8 == 0 && c.q_stride % 8 == 0 && c.out_stride % 8 == 0 &&
+                      (((uintptr_t)c.qkv | (uintptr_t)c.q_out | (uintptr_t)c.cos_t | (uintptr_t)c.sin_t) & 15) == 0 &&
+                      (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 7) == 0;
+    if (c.dtype == NIB_F32) return wide ? launch_append<float, true>(c.qkv, c.q_out, a, stream) : launch_append<float, false>(c.qkv, c.q_out, a, stream);
+    return wide ? launch_append<__nv_bfloat16, true>(c.qkv, c.q_out, a, stream) : launch_append<__nv_bfloat16, false>(c.qkv, c.q_out, a, stream);
 }
 
 // out = codes * scale for ``blocks`` blocks of ``per_block`` codes each.

@@ -837,9 +837,12 @@ class Kernels:
         self._check(self._lib.nib_unpack_int8(_ptr(pages), _ptr(scales), _ptr(out), c_longlong(scales.numel()), pages.shape[2] * pages.shape[3],
                                               _DT[out.dtype], self._stream()), "unpack (8-bit cache)")
 
-    def attention_int8(self, qkv, out, heads, kv_heads, head_dim, scale, window, ctx, block_table, page_size, k_pages, v_pages, k_scales, v_scales):
+    def attention_int8(self, qkv, out, heads, kv_heads, head_dim, scale, window, ctx, block_table, page_size, k_pages, v_pages, k_scales, v_scales,
+                       earlier_complete=False):
         """``attention`` over the 8-bit cache that ``rope_store_int8`` fills: the rotated queries are the first columns of the rows of
-        ``qkv``, the step's own keys and values are in the pages already."""
+        ``qkv``, the step's own keys and values are in the pages already. ``earlier_complete``: the caller promises that
+        the pages before the one that a token's own key lies in are no running kernel's results (the engine's steps begin with a copy, which
+        waits for the step before); single tokens' earlier pages are then sent for while the kernel before this one is still running."""
         n_req = self._cache_int8("attention_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales)
         m, dtype = qkv.shape[0], _DT[qkv.dtype]
         if heads <= 0 or heads % kv_heads or qkv.shape[1] < heads * head_dim or out.shape != (m, heads * head_dim) or window < 0:
@@ -864,7 +867,7 @@ class Kernels:
             args = _ATTEND_INT8.pack(
                 qkv.data_ptr(), out.data_ptr(), ctx.ctx_lens.data_ptr(), block_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                 k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, qkv.stride(0), block_table.stride(0), block_table.shape[1], page_size,
-                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 0, scale, 0)
+                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 1 if earlier_complete else 0, scale, 0)
             self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
         if n_dec == n_req:
             return

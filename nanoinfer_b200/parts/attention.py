@@ -104,7 +104,7 @@ class GroupedQueryAttention(Mixer):
             self.ops.rope_store(qkv, self.heads, self.kv_heads, self.head_dim, ctx.positions, ctx.req_index, self._rotary, None, cache.page_size,
                                 None, None, False)
         self.ops.attention_int8(qkv, attn, self.heads, self.kv_heads, self.head_dim, self.scale, self.window, ctx, cache.block_table,
-                                cache.page_size, cache.k_pages, cache.v_pages, k_scales, v_scales)
+                                cache.page_size, cache.k_pages, cache.v_pages, k_scales, v_scales, earlier_complete=True)
         self.ops.linear(attn, self.w_o, None, residual32, "add")
 
 

@@ -332,9 +332,12 @@ def test_append_and_attention_run_together_as_a_model_calls_them(ops):
                     table[i, lp] = order.pop()
         b.pools, b.pool_scales, b.table, b.rotary = pools, scales, table, rotary
         q = b.append(ops)
+        out = torch.empty(q.shape, dtype=q.dtype, device="cuda")
+        ops.rope_store_int8(b.qkv, q, heads, kv, d, b.ctx, rotary, table, page, *pools, *scales)        # (again: the same codes)
+        ops.attention_int8(q, out, heads, kv, d, d ** -0.5, 0, b.ctx, table, page, *pools, *scales, earlier_complete=True)
         b.rows[:, :heads] = q.reshape(-1, heads, d).cpu()
         b.qkv = q
-        check_attention(ops, b)
+        assert torch.equal(out, check_attention(ops, b))
         lengths = [a + n for a, n in zip(lengths, lens)]
 
 
