@@ -149,6 +149,14 @@ __device__ __forceinline__ int code_of(const Two& y, float inv) {
     return (int)r;
 }
 
+// rint(code * by) of four codes.
+__device__ __forceinline__ unsigned smaller(unsigned w, float by) {
+    unsigned r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= (unsigned)(__float2int_rn((float)(signed char)(w >> (8 * i)) * by) & 0xff) << (8 * i);
+    return r;
+}
+
 constexpr int KV_WARPS = 4;
 constexpr int Q_THREADS = KV_WARPS * 32;
 
@@ -159,46 +167,65 @@ struct AppendArgs {
     int units, kv_blocks;       // the first kv_blocks CTAs append, a warp for each (unit, kv head, keys or values); the others rotate queries
 };
 
-// WIDE: chunks of 8 elements of queries and 4 of keys and values; 1 where widths or addresses do not allow it.
-// Keys and values: a warp for each (unit, kv head, keys or values), two items a lane at a time, whose loads are all on their way
-// before the first is used. Twice: for the largest magnitude, then for the codes (the second time the rows come from L1).
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(Q_THREADS, 8)
-append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_out may be qkv)
-    constexpr int VQ = WIDE ? 8 : 1, V = WIDE ? 4 : 1, B = 2;
-    const int half = a.rot >> 1, hd = a.head_dim, lane = threadIdx.x & 31;
-    if ((int)blockIdx.x >= a.kv_blocks) {
-        // ---- queries: a CTA a token; an item is a chunk of pairs (or a chunk beyond the rotated width) of a head
-        const int tok = blockIdx.x - a.kv_blocks, pos = a.positions[tok];       // (positions and tables are the step's inputs)
-        const int pairs = half / VQ, tails = (hd - a.rot) / VQ;
+// ---- queries: an item is a chunk of VQ pairs, or a chunk beyond the rotated width, of one head of one token.
+template <typename T, int VQ>
+__device__ __forceinline__ void rotate_queries(const T* qkv, T* q_out, const AppendArgs& a, long long i, bool& waited) {
+    const int half = a.rot >> 1, hd = a.head_dim, pairs = half / VQ, per_head = pairs + (hd - a.rot) / VQ, per_token = a.heads * per_head;
+    const int tok = (int)(i / per_token), rest = (int)(i - (long long)tok * per_token), head = rest / per_head, c = rest - head * per_head;
+    const T* p = qkv + (size_t)tok * a.q_stride + (size_t)head * hd;
+    T* o = q_out + (size_t)tok * a.out_stride + (size_t)head * hd;
+    float x1[VQ], x2[VQ], cs[VQ], sn[VQ], y1[VQ], y2[VQ];
+    if (c < pairs) {
+        const int d = c * VQ, pos = a.positions[tok];         // (positions and tables are the step's inputs)
         const bool known = pos >= 0 && pos < a.table_rows;
-        const T* row = qkv + (size_t)tok * a.q_stride;
-        T* to = q_out + (size_t)tok * a.out_stride;
-        bool waited = false;
-        for (int i = threadIdx.x; i < a.heads * pairs; i += Q_THREADS) {
-            const int head = i / pairs, d = (i - head * pairs) * VQ;
-            float x1[VQ], x2[VQ], cs[VQ], sn[VQ], y1[VQ], y2[VQ];
-            const size_t at = (size_t)(known ? pos : 0) * half + d;
-            Vec<float, VQ>::load(cs, a.cos_t + at);
-            Vec<float, VQ>::load(sn, a.sin_t + at);
-            if (!waited) { pdl_wait(); pdl_launch_dependents(); waited = true; }
-            Vec<T, VQ>::load(x1, row + (size_t)head * hd + d);
-            Vec<T, VQ>::load(x2, row + (size_t)head * hd + d + half);
+        const size_t at = (size_t)(known ? pos : 0) * half + d;
+        Vec<float, VQ>::load(cs, a.cos_t + at);
+        Vec<float, VQ>::load(sn, a.sin_t + at);
+        if (!waited) { pdl_wait(); pdl_launch_dependents(); waited = true; }
+        Vec<T, VQ>::load(x1, p + d);
+        Vec<T, VQ>::load(x2, p + d + half);
 #pragma unroll
-            for (int j = 0; j < VQ; ++j) {
-                y1[j] = known ? x1[j] * cs[j] - x2[j] * sn[j] : NAN;
-                y2[j] = known ? x2[j] * cs[j] + x1[j] * sn[j] : NAN;
-            }
-            Vec<T, VQ>::store(to + (size_t)head * hd + d, y1);
-            Vec<T, VQ>::store(to + (size_t)head * hd + d + half, y2);
+        for (int j = 0; j < VQ; ++j) {
+            y1[j] = known ? x1[j] * cs[j] - x2[j] * sn[j] : NAN;
+            y2[j] = known ? x2[j] * cs[j] + x1[j] * sn[j] : NAN;
         }
-        if (!waited) pdl_wait();
-        for (int i = threadIdx.x; i < a.heads * tails; i += Q_THREADS) {
-            const int head = i / tails, d = a.rot + (i - head * tails) * VQ;
-            float x[VQ];
-            Vec<T, VQ>::load(x, row + (size_t)head * hd + d);
-            Vec<T, VQ>::store(to + (size_t)head * hd + d, x);
-        }
+        Vec<T, VQ>::store(o + d, y1);
+        Vec<T, VQ>::store(o + d + half, y2);
+    } else {
+        const int d = a.rot + (c - pairs) * VQ;
+        if (!waited) { pdl_wait(); pdl_launch_dependents(); waited = true; }
+        Vec<T, VQ>::load(x1, p + d);
+        Vec<T, VQ>::store(o + d, x1);
+    }
+}
+
+constexpr int ROTATE_THREADS = 256;
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(ROTATE_THREADS)
+rotate_queries_kernel(const T* qkv, T* q_out, const AppendArgs a, long long items) {
+    const long long i = (long long)blockIdx.x * ROTATE_THREADS + threadIdx.x;
+    bool waited = false;
+    if (i < items) rotate_queries<T, WIDE ? 8 : 1>(qkv, q_out, a, i, waited);
+    if (!waited) { pdl_wait(); pdl_launch_dependents(); }
+}
+
+// ---- keys and values: a warp for each (unit, kv head, keys or values), two items a lane at a time, whose loads are all on their way
+// before the first is used. Twice: for the largest magnitude, then for the codes (the second time the rows come from L1).
+// WIDE: chunks of 8 elements of queries and 4 of keys and values; 1 where widths or addresses do not allow it.
+// QUERIES: CTAs from kv_blocks on rotate a token's queries each (one launch for few tokens). Without, the kernel that rotates them
+// runs before and beside this one: it lets this one in when what both read is complete, and this one waits for it at its end.
+template <typename T, bool WIDE, bool QUERIES>
+__global__ void __launch_bounds__(Q_THREADS)
+append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_out may be qkv)
+    constexpr int V = WIDE ? 4 : 1, B = 2;
+    const int half = a.rot >> 1, hd = a.head_dim, lane = threadIdx.x & 31;
+    if (QUERIES && (int)blockIdx.x >= a.kv_blocks) {
+        constexpr int VQ = WIDE ? 8 : 1;
+        const int per_token = a.heads * ((half + hd - a.rot) / VQ);
+        bool waited = false;
+        for (int i = threadIdx.x; i < per_token; i += Q_THREADS)
+            rotate_queries<T, VQ>(qkv, q_out, a, (long long)(blockIdx.x - a.kv_blocks) * per_token + i, waited);
+        if (!waited) { pdl_wait(); pdl_launch_dependents(); }
         return;
     }
     const int job = blockIdx.x * KV_WARPS + (threadIdx.x >> 5), per_unit = 2 * a.kv_heads;
@@ -208,8 +235,9 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
         unit = find_unit(u, a.q_start, a.ctx_lens, a.n_req, a.block_table, a.bt_stride, a.bt_width, a.page_size, a.num_pages, lane);
     // (The attention behind is let in only now: its CTAs, placed while the kernel before this one still holds its SMs, would share few of
     // them. 8 tokens of 4,096 keys, 28 heads of 128, both calls: 17 us, and 21 let in at once.)
-    pdl_wait();
+    if (QUERIES) pdl_wait();
     pdl_launch_dependents();
+    struct AtEnd { __device__ ~AtEnd() { if (!QUERIES) pdl_wait(); } } at_end;
     if (unit.page < 0) return;
     const size_t block = (size_t)unit.page * a.kv_heads + kvh;
     signed char* codes = (values ? a.v_pages : a.k_pages) + block * a.page_size * hd;
@@ -264,7 +292,19 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
         scale = undefined ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale);
         if (scale > old) {          // (not where it is undefined)
             const float by = old / scale;       // a power of two, or 0 where the block had no scale yet
-            for (int i = lane; i < unit.slot * hd; i += 32) codes[i] = (signed char)__float2int_rn((float)codes[i] * by);
+            const int bytes = unit.slot * hd, wide = ((uintptr_t)codes & 15) == 0 ? bytes >> 4 : 0;
+            // 16 codes at a time, four loads under way (a byte at a time the one block of a step's whose scale grew was what the
+            // kernel's time went by: 13 us for 64 tokens of 4 heads of 128)
+            for (int i0 = lane; i0 < wide; i0 += 32 * 4) {
+                uint4 w[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) if (i0 + 32 * b < wide) w[b] = reinterpret_cast<const uint4*>(codes)[i0 + 32 * b];
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (i0 + 32 * b < wide)
+                        reinterpret_cast<uint4*>(codes)[i0 + 32 * b] = make_uint4(smaller(w[b].x, by), smaller(w[b].y, by), smaller(w[b].z, by), smaller(w[b].w, by));
+            }
+            for (int i = wide * 16 + lane; i < bytes; i += 32) codes[i] = (signed char)__float2int_rn((float)codes[i] * by);
         }
     }
     const float inv = 1.0f / scale;
@@ -382,7 +422,15 @@ gather_int8_kernel(const signed char* __restrict__ k_pages, const signed char* _
 template <typename T, bool WIDE>
 int launch_append(const void* qkv, void* q_out, const AppendArgs& a, cudaStream_t stream) {
     NIB_REQUIRE((long long)a.m + a.kv_blocks < (1LL << 31) - 1, "rope_store_int8: too many tokens for one launch");
-    NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE>, dim3((unsigned)(a.m + a.kv_blocks)), dim3(Q_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
+    if (a.m <= 64) {
+        NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE, true>, dim3((unsigned)(a.m + a.kv_blocks)), dim3(Q_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
+        return 0;
+    }
+    const int vq = WIDE ? 8 : 1;
+    const long long items = (long long)a.m * a.heads * (((a.rot >> 1) + a.head_dim - a.rot) / vq), grid = (items + ROTATE_THREADS - 1) / ROTATE_THREADS;
+    NIB_REQUIRE(grid < (1LL << 31) - 1, "rope_store_int8: too many elements for one launch");
+    NIB_CUDA(launch_pdl(rotate_queries_kernel<T, WIDE>, dim3((unsigned)grid), dim3(ROTATE_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a, items));
+    NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE, false>, dim3((unsigned)a.kv_blocks), dim3(Q_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
     return 0;
 }
 

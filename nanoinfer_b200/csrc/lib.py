@@ -821,6 +821,7 @@ class Kernels:
             qkv.data_ptr(), q_out.data_ptr(), ctx.positions.data_ptr(), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), cos, sin, block_table.data_ptr(),
             k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), qkv.stride(0), q_out.stride(0), n_req, units, rows, rot,
             block_table.stride(0), block_table.shape[1], page_size, k_pages.shape[0], m, heads, kv_heads, head_dim, _DT[qkv.dtype], 0)
+        self.launches += 1 if m > 64 else 0         # (queries, and keys and values, each a kernel)
         self._check(self._lib.nib_rope_store_int8(args, self._stream()), "rope_store (8-bit cache)")
 
     def unpack_int8(self, pages, scales, out):
@@ -899,6 +900,8 @@ class Kernels:
         ctas = _cluster_splits(max(1, min(8, chunks, room // 2 // units)))
         if chunks <= ctas * (1 if kind == 0 else 16):
             return ctas, 0
+        if kind and units >= 128:       # (rows enough that the SMs even out different lengths by themselves)
+            return 4, 0
         return 1, min(room, units * min(chunks, 64))        # (a row's parts are one kernel's sum)
 
     def attention_tc_error(self) -> int:
