@@ -119,8 +119,13 @@ template <typename T> struct Vec<T, 1> {
 };
 
 template <int V> __device__ __forceinline__ void store_codes(signed char* p, const int (&c)[V]) {
-    if constexpr (V == 4) {
-        *reinterpret_cast<unsigned*>(p) = (unsigned)(c[0] & 0xff) | ((unsigned)(c[1] & 0xff) << 8) | ((unsigned)(c[2] & 0xff) << 16) | ((unsigned)(c[3] & 0xff) << 24);
+    if constexpr (V > 1) {
+        unsigned w[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            w[i] = (unsigned)(c[4 * i] & 0xff) | ((unsigned)(c[4 * i + 1] & 0xff) << 8) | ((unsigned)(c[4 * i + 2] & 0xff) << 16) | ((unsigned)(c[4 * i + 3] & 0xff) << 24);
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<unsigned*>(p) = w[0];
     } else {
         p[0] = (signed char)c[0];
     }
@@ -157,14 +162,34 @@ __device__ __forceinline__ unsigned smaller(unsigned w, float by) {
     return r;
 }
 
-constexpr int KV_WARPS = 4;
-constexpr int Q_THREADS = KV_WARPS * 32;
+constexpr int KV_THREADS = 128;
+
+// The scale of a block whose new elements' largest magnitude is ``top``, and the codes that it held before made smaller where that
+// scale is larger than theirs. All threads take part.
+__device__ __forceinline__ float scale_of(unsigned top, float old, int slots, signed char* codes, int hd, int tid) {
+    float scale = block_scale(__uint_as_float(top));
+    if (slots == 0) return scale;
+    const bool undefined = scale != scale || old != old;
+    scale = undefined ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale);
+    if (scale > old) {          // (not where it is undefined)
+        const float by = old / scale;       // a power of two, or 0 where the block had no scale yet
+        const int bytes = slots * hd, wide = ((uintptr_t)codes & 15) == 0 ? bytes >> 4 : 0;
+        // 16 codes at a time (a byte at a time the one block of a step's whose scale grew was what the kernel's time went by: 13 us
+        // for 64 tokens of 4 heads of 128)
+        for (int i = tid; i < wide; i += KV_THREADS) {
+            const uint4 w = reinterpret_cast<const uint4*>(codes)[i];
+            reinterpret_cast<uint4*>(codes)[i] = make_uint4(smaller(w.x, by), smaller(w.y, by), smaller(w.z, by), smaller(w.w, by));
+        }
+        for (int i = wide * 16 + tid; i < bytes; i += KV_THREADS) codes[i] = (signed char)__float2int_rn((float)codes[i] * by);
+    }
+    return scale;
+}
 
 struct AppendArgs {
     const int* positions; const int* q_start; const int* ctx_lens; const float* cos_t; const float* sin_t;
     const int* block_table; signed char* k_pages; signed char* v_pages; float* k_scales; float* v_scales;
     int table_rows, rot, bt_stride, bt_width, page_size, num_pages, m, n_req, heads, kv_heads, head_dim, q_stride, out_stride;
-    int units, kv_blocks;       // the first kv_blocks CTAs append, a warp for each (unit, kv head, keys or values); the others rotate queries
+    int units, kv_blocks;       // the first kv_blocks CTAs append, one for each (unit, kv head); the others rotate queries
 };
 
 // ---- queries: an item is a chunk of VQ pairs, or a chunk beyond the rotated width, of one head of one token.
@@ -209,30 +234,33 @@ rotate_queries_kernel(const T* qkv, T* q_out, const AppendArgs a, long long item
     if (!waited) { pdl_wait(); pdl_launch_dependents(); }
 }
 
-// ---- keys and values: a warp for each (unit, kv head, keys or values), two items a lane at a time, whose loads are all on their way
-// before the first is used. Twice: for the largest magnitude, then for the codes (the second time the rows come from L1).
-// WIDE: chunks of 8 elements of queries and 4 of keys and values; 1 where widths or addresses do not allow it.
+// ---- keys and values: a CTA for each (unit, kv head), two items of keys and two of values a thread at a time, whose loads are all on
+// their way before the first is used; a page of 16 tokens of 128 elements is one such turn, and its items stay in registers from the
+// search for the largest magnitude to their codes. (A warp for each of keys and values took 29 us for 4,096 tokens of 4 heads of 128,
+// waiting for one load after another.)
+// WIDE: chunks of 8 elements of queries and values and 4 of keys; 1 where widths or addresses do not allow it.
 // QUERIES: CTAs from kv_blocks on rotate a token's queries each (one launch for few tokens). Without, the kernel that rotates them
 // runs before and beside this one: it lets this one in when what both read is complete, and this one waits for it at its end.
+template <typename T, int V> struct KeyItem { float x1[V], x2[V], cs[V], sn[V]; int row, d; bool pair; };       // the second chunk only of a rotated pair
+template <typename T, int V> struct ValueItem { float x[V]; int row, d; };
+
 template <typename T, bool WIDE, bool QUERIES>
-__global__ void __launch_bounds__(Q_THREADS)
+__global__ void __launch_bounds__(KV_THREADS)
 append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_out may be qkv)
-    constexpr int V = WIDE ? 4 : 1, B = 2;
-    const int half = a.rot >> 1, hd = a.head_dim, lane = threadIdx.x & 31;
+    constexpr int V = WIDE ? 4 : 1, VV = WIDE ? 8 : 1, B = 2, TURN = KV_THREADS * B;
+    __shared__ unsigned s_top[2][KV_THREADS / 32];
+    const int half = a.rot >> 1, hd = a.head_dim, tid = threadIdx.x, lane = tid & 31;
     if (QUERIES && (int)blockIdx.x >= a.kv_blocks) {
         constexpr int VQ = WIDE ? 8 : 1;
         const int per_token = a.heads * ((half + hd - a.rot) / VQ);
         bool waited = false;
-        for (int i = threadIdx.x; i < per_token; i += Q_THREADS)
+        for (int i = tid; i < per_token; i += KV_THREADS)
             rotate_queries<T, VQ>(qkv, q_out, a, (long long)(blockIdx.x - a.kv_blocks) * per_token + i, waited);
         if (!waited) { pdl_wait(); pdl_launch_dependents(); }
         return;
     }
-    const int job = blockIdx.x * KV_WARPS + (threadIdx.x >> 5), per_unit = 2 * a.kv_heads;
-    const int u = job / per_unit, kvh = (job - u * per_unit) >> 1, values = job & 1;
-    Unit unit{0, 0, 0, 0, -1};
-    if (job < a.units * per_unit)           // (lengths and tables, too)
-        unit = find_unit(u, a.q_start, a.ctx_lens, a.n_req, a.block_table, a.bt_stride, a.bt_width, a.page_size, a.num_pages, lane);
+    const int u = blockIdx.x / a.kv_heads, kvh = blockIdx.x - u * a.kv_heads;
+    const Unit unit = find_unit(u, a.q_start, a.ctx_lens, a.n_req, a.block_table, a.bt_stride, a.bt_width, a.page_size, a.num_pages, lane);     // (lengths and tables, too)
     // (The attention behind is let in only now: its CTAs, placed while the kernel before this one still holds its SMs, would share few of
     // them. 8 tokens of 4,096 keys, 28 heads of 128, both calls: 17 us, and 21 let in at once.)
     if (QUERIES) pdl_wait();
@@ -240,20 +268,21 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
     struct AtEnd { __device__ ~AtEnd() { if (!QUERIES) pdl_wait(); } } at_end;
     if (unit.page < 0) return;
     const size_t block = (size_t)unit.page * a.kv_heads + kvh;
-    signed char* codes = (values ? a.v_pages : a.k_pages) + block * a.page_size * hd;
-    float* scale_at = (values ? a.v_scales : a.k_scales) + block;
-    const T* rows = qkv + (size_t)unit.row * a.q_stride + (size_t)(a.heads + (values ? a.kv_heads : 0) + kvh) * hd;
-    const float old = unit.slot > 0 ? *scale_at : 0.f;
-    const int rot = values ? 0 : a.rot, pairs = (rot >> 1) / V, per_token = pairs + (hd - rot) / V;
-    const int items = unit.count * per_token;
+    signed char* k_codes = a.k_pages + block * a.page_size * hd;
+    signed char* v_codes = a.v_pages + block * a.page_size * hd;
+    const T* k_rows = qkv + (size_t)unit.row * a.q_stride + (size_t)(a.heads + kvh) * hd;
+    const T* v_rows = k_rows + (size_t)a.kv_heads * hd;
+    const float k_old = unit.slot > 0 ? a.k_scales[block] : 0.f, v_old = unit.slot > 0 ? a.v_scales[block] : 0.f;
+    const int pairs = half / V, k_per_token = pairs + (hd - a.rot) / V, v_per_token = hd / VV;
+    const int k_items = unit.count * k_per_token, v_items = unit.count * v_per_token;
+    const int k_first = tid, v_first = (tid + KV_THREADS / 2) % KV_THREADS;       // (few items: keys and values are different warps')
 
-    struct Item { float x1[V], x2[V], cs[V], sn[V]; int row, d; bool pair; };       // the second chunk only of a rotated pair
-    auto load = [&](Item& it, int i) {
-        it.row = i / per_token;
-        const int c = i - it.row * per_token;
+    auto load_key = [&](KeyItem<T, V>& it, int i) {
+        it.row = i / k_per_token;
+        const int c = i - it.row * k_per_token;
         it.pair = c < pairs;
-        it.d = it.pair ? c * V : rot + (c - pairs) * V;
-        const T* p = rows + (size_t)it.row * a.q_stride;
+        it.d = it.pair ? c * V : a.rot + (c - pairs) * V;
+        const T* p = k_rows + (size_t)it.row * a.q_stride;
         Vec<T, V>::load(it.x1, p + it.d);
         if (it.pair) {
             Vec<T, V>::load(it.x2, p + it.d + half);
@@ -267,68 +296,82 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
             }
         }
     };
-    auto first_of = [&](const Item& it, int j) { return it.pair ? sum_of_products(it.x1[j], it.cs[j], -it.x2[j], it.sn[j]) : Two{it.x1[j], 0.f}; };
-    auto second_of = [&](const Item& it, int j) { return sum_of_products(it.x2[j], it.cs[j], it.x1[j], it.sn[j]); };
+    auto load_value = [&](ValueItem<T, VV>& it, int i) {
+        it.row = i / v_per_token;
+        it.d = (i - it.row * v_per_token) * VV;
+        Vec<T, VV>::load(it.x, v_rows + (size_t)it.row * a.q_stride + it.d);
+    };
+    auto first_of = [&](const KeyItem<T, V>& it, int j) { return it.pair ? sum_of_products(it.x1[j], it.cs[j], -it.x2[j], it.sn[j]) : Two{it.x1[j], 0.f}; };
+    auto second_of = [&](const KeyItem<T, V>& it, int j) { return sum_of_products(it.x2[j], it.cs[j], it.x1[j], it.sn[j]); };
 
-    Item it[B];
-    unsigned top = 0;
-    for (int i0 = lane; i0 < items; i0 += 32 * B) {
+    KeyItem<T, V> key[B];
+    ValueItem<T, VV> value[B];
+    unsigned k_top = 0, v_top = 0;
+    const int turns = max((k_items + TURN - 1) / TURN, (v_items + TURN - 1) / TURN);
+    for (int turn = 0; turn < turns; ++turn) {
 #pragma unroll
-        for (int b = 0; b < B; ++b) if (i0 + 32 * b < items) load(it[b], i0 + 32 * b);
+        for (int b = 0; b < B; ++b) {
+            const int at = turn * TURN + b * KV_THREADS;
+            if (at + k_first < k_items) load_key(key[b], at + k_first);
+            if (at + v_first < v_items) load_value(value[b], at + v_first);
+        }
 #pragma unroll
-        for (int b = 0; b < B; ++b)
-            if (i0 + 32 * b < items) {
+        for (int b = 0; b < B; ++b) {
+            const int at = turn * TURN + b * KV_THREADS;
+            if (at + k_first < k_items) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    top = max(top, magnitude_up(first_of(it[b], j)));
-                    if (it[b].pair) top = max(top, magnitude_up(second_of(it[b], j)));
+                    k_top = max(k_top, magnitude_up(first_of(key[b], j)));
+                    if (key[b].pair) k_top = max(k_top, magnitude_up(second_of(key[b], j)));
                 }
             }
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    float scale = block_scale(__uint_as_float(top));
-    if (unit.slot > 0) {
-        const bool undefined = scale != scale || old != old;
-        scale = undefined ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale);
-        if (scale > old) {          // (not where it is undefined)
-            const float by = old / scale;       // a power of two, or 0 where the block had no scale yet
-            const int bytes = unit.slot * hd, wide = ((uintptr_t)codes & 15) == 0 ? bytes >> 4 : 0;
-            // 16 codes at a time, four loads under way (a byte at a time the one block of a step's whose scale grew was what the
-            // kernel's time went by: 13 us for 64 tokens of 4 heads of 128)
-            for (int i0 = lane; i0 < wide; i0 += 32 * 4) {
-                uint4 w[4];
+            if (at + v_first < v_items) {
 #pragma unroll
-                for (int b = 0; b < 4; ++b) if (i0 + 32 * b < wide) w[b] = reinterpret_cast<const uint4*>(codes)[i0 + 32 * b];
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    if (i0 + 32 * b < wide)
-                        reinterpret_cast<uint4*>(codes)[i0 + 32 * b] = make_uint4(smaller(w[b].x, by), smaller(w[b].y, by), smaller(w[b].z, by), smaller(w[b].w, by));
+                for (int j = 0; j < VV; ++j) v_top = max(v_top, __float_as_uint(value[b].x[j]) & 0x7fffffffu);
             }
-            for (int i = wide * 16 + lane; i < bytes; i += 32) codes[i] = (signed char)__float2int_rn((float)codes[i] * by);
         }
     }
-    const float inv = 1.0f / scale;
-    for (int i0 = lane; i0 < items; i0 += 32 * B) {
-        if (items > 32 * B) {           // (else the items are still at hand)
+    k_top = __reduce_max_sync(0xffffffffu, k_top);
+    v_top = __reduce_max_sync(0xffffffffu, v_top);
+    if (lane == 0) { s_top[0][tid >> 5] = k_top; s_top[1][tid >> 5] = v_top; }
+    __syncthreads();
 #pragma unroll
-            for (int b = 0; b < B; ++b) if (i0 + 32 * b < items) load(it[b], i0 + 32 * b);
+    for (int w = 0; w < KV_THREADS / 32; ++w) { k_top = max(k_top, s_top[0][w]); v_top = max(v_top, s_top[1][w]); }
+    const float k_scale = scale_of(k_top, k_old, unit.slot, k_codes, hd, tid), v_scale = scale_of(v_top, v_old, unit.slot, v_codes, hd, tid);
+    const float k_inv = 1.0f / k_scale, v_inv = 1.0f / v_scale;
+    for (int turn = 0; turn < turns; ++turn) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int at = turn * TURN + b * KV_THREADS;
+            if (turns > 1) {            // (else the items are still at hand)
+                if (at + k_first < k_items) load_key(key[b], at + k_first);
+                if (at + v_first < v_items) load_value(value[b], at + v_first);
+            }
         }
 #pragma unroll
-        for (int b = 0; b < B; ++b)
-            if (i0 + 32 * b < items) {
-                signed char* dst = codes + (size_t)(unit.slot + it[b].row) * hd + it[b].d;
+        for (int b = 0; b < B; ++b) {
+            const int at = turn * TURN + b * KV_THREADS;
+            if (at + k_first < k_items) {
+                signed char* dst = k_codes + (size_t)(unit.slot + key[b].row) * hd + key[b].d;
                 int c[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) c[j] = code_of(first_of(it[b], j), inv);
+                for (int j = 0; j < V; ++j) c[j] = code_of(first_of(key[b], j), k_inv);
                 store_codes<V>(dst, c);
-                if (it[b].pair) {
+                if (key[b].pair) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) c[j] = code_of(second_of(it[b], j), inv);
+                    for (int j = 0; j < V; ++j) c[j] = code_of(second_of(key[b], j), k_inv);
                     store_codes<V>(dst + half, c);
                 }
             }
+            if (at + v_first < v_items) {
+                int c[VV];
+#pragma unroll
+                for (int j = 0; j < VV; ++j) c[j] = code_of(Two{value[b].x[j], 0.f}, v_inv);
+                store_codes<VV>(v_codes + (size_t)(unit.slot + value[b].row) * hd + value[b].d, c);
+            }
+        }
     }
-    if (lane == 0) *scale_at = scale;
+    if (tid == 0) { a.k_scales[block] = k_scale; a.v_scales[block] = v_scale; }
 }
 
 // ------------------------------------------------------------------------------------------ reading pages back
@@ -423,14 +466,14 @@ template <typename T, bool WIDE>
 int launch_append(const void* qkv, void* q_out, const AppendArgs& a, cudaStream_t stream) {
     NIB_REQUIRE((long long)a.m + a.kv_blocks < (1LL << 31) - 1, "rope_store_int8: too many tokens for one launch");
     if (a.m <= 64) {
-        NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE, true>, dim3((unsigned)(a.m + a.kv_blocks)), dim3(Q_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
+        NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE, true>, dim3((unsigned)(a.m + a.kv_blocks)), dim3(KV_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
         return 0;
     }
     const int vq = WIDE ? 8 : 1;
     const long long items = (long long)a.m * a.heads * (((a.rot >> 1) + a.head_dim - a.rot) / vq), grid = (items + ROTATE_THREADS - 1) / ROTATE_THREADS;
     NIB_REQUIRE(grid < (1LL << 31) - 1, "rope_store_int8: too many elements for one launch");
     NIB_CUDA(launch_pdl(rotate_queries_kernel<T, WIDE>, dim3((unsigned)grid), dim3(ROTATE_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a, items));
-    NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE, false>, dim3((unsigned)a.kv_blocks), dim3(Q_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
+    NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE, false>, dim3((unsigned)a.kv_blocks), dim3(KV_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
     return 0;
 }
 
@@ -458,9 +501,9 @@ NIB_API int nib_rope_store_int8(const void* args, cudaStream_t stream) {
     AppendArgs a{c.positions, c.q_start, c.ctx_lens, c.cos_t, c.sin_t, c.block_table, (signed char*)c.k_pages, (signed char*)c.v_pages, c.k_scales,
                  c.v_scales, c.table_rows, c.rot, c.bt_stride, c.bt_width, c.page_size, c.num_pages, c.m, c.n_req, c.heads, c.kv_heads, c.head_dim,
                  c.q_stride, c.out_stride, c.units, 0};
-    const long long jobs = (long long)c.units * 2 * c.kv_heads;
-    NIB_REQUIRE(jobs < (1LL << 31) - KV_WARPS, "rope_store_int8: too many pages for one launch");
-    a.kv_blocks = (int)((jobs + KV_WARPS - 1) / KV_WARPS);
+    const long long jobs = (long long)c.units * c.kv_heads;
+    NIB_REQUIRE(jobs < (1LL << 31) - 1, "rope_store_int8: too many pages for one launch");
+    a.kv_blocks = (int)jobs;
     const bool wide = (c.rot / 2) % 8 == 0 && c.head_dim % 8 == 0 && c.q_stride % 8 == 0 && c.out_stride % 8 == 0 &&
                       (((uintptr_t)c.qkv | (uintptr_t)c.q_out | (uintptr_t)c.cos_t | (uintptr_t)c.sin_t) & 15) == 0 &&
                       (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 7) == 0;
