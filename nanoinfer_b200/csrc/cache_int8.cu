@@ -266,7 +266,7 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
     if (QUERIES) pdl_wait();
     pdl_launch_dependents();
     struct AtEnd { __device__ ~AtEnd() { if (!QUERIES) pdl_wait(); } } at_end;
-    if (unit.page < 0) return;
+    if (unit.page < 0 || unit.row < 0 || unit.row + unit.count > a.m) return;       // (never a row that the call did not bring)
     const size_t block = (size_t)unit.page * a.kv_heads + kvh;
     signed char* k_codes = a.k_pages + block * a.page_size * hd;
     signed char* v_codes = a.v_pages + block * a.page_size * hd;

@@ -777,7 +777,7 @@ class Kernels:
             if t.get_device() != device or t.dtype != dtype or not t.is_contiguous():
                 _here(t, dtype, f"{what} {name}")
         pages = k_pages.shape[0]
-        if pages == 0 or k_pages.shape != (pages, kv_heads, page_size, head_dim) or v_pages.shape != k_pages.shape:
+        if k_pages.numel() == 0 or k_pages.shape != (pages, kv_heads, page_size, head_dim) or v_pages.shape != k_pages.shape:
             raise KernelError(f"{what}: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} do not fit kv_heads/page_size/head_dim")
         if k_scales.numel() != pages * kv_heads or v_scales.numel() != pages * kv_heads:
             raise KernelError(f"{what}: scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}: one for each page and kv head")
@@ -875,6 +875,9 @@ class Kernels:
         # The other requests' pages are read back once, in the order of their positions, and the prompt kernels run on them: a portion
         # reads its keys once for each of its row tiles, and what the tensor cores multiply is 16 bits wide either way.
         n_rest, width = n_req - n_dec, -(-block_table.shape[1] * page_size // 64)
+        if not qkv.is_contiguous() or qkv.data_ptr() % 16:          # (the prompt kernels copy aligned, dense rows)
+            qkv = qkv[:, :heads * head_dim].clone(memory_format=torch.contiguous_format)
+        rows = out if out.data_ptr() % 16 == 0 else torch.empty_like(out)
         keys = torch.empty((n_rest * width, kv_heads, 64, head_dim), dtype=qkv.dtype, device=qkv.device)
         values = torch.empty_like(keys)
         table = torch.empty((n_req, width), dtype=torch.int32, device=qkv.device)
@@ -885,7 +888,9 @@ class Kernels:
             c_int(page_size), c_int(k_pages.shape[0]), c_int(kv_heads), c_int(head_dim), c_int(width), c_int(window), c_int(dtype), self._stream()),
             "gather (8-bit cache)")
         self._lib.nib_pdl_skip_next()       # the attention reads its table and earlier pages before its wait: here they are the kernel's before it
-        self.attention(qkv, out, heads, kv_heads, head_dim, scale, window, ctx, table, 64, keys, values, first=n_dec)
+        self.attention(qkv, rows, heads, kv_heads, head_dim, scale, window, ctx, table, 64, keys, values, first=n_dec)
+        if rows is not out:
+            out[n_dec:].copy_(rows[n_dec:])
 
     def _decode_int8_split(self, n_tokens: int, kv_heads: int, max_ctx: int, window: int, kind: int, head_dim: int):
         """How the keys of decoding tokens over the 8-bit cache are cut: (CTAs of a cluster that share a row's keys, 0), or (1, the CTAs that

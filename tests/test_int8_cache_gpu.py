@@ -341,6 +341,112 @@ def test_append_and_attention_run_together_as_a_model_calls_them(ops):
         lengths = [a + n for a, n in zip(lengths, lens)]
 
 
+def test_rows_and_results_off_16_bytes(ops):
+    """Strided rows, and memory that begins in the middle of what a kernel likes to read at a time: the same values."""
+    for heads, kv, d, page in ((14, 2, 64, 16), (4, 2, 128, 8)):
+        b = Batch(heads, kv, d, 0, page, [1, 1, 30], [40, 9, 20], torch.bfloat16, seed=60)
+        want = attention_rows(ops, b)
+        m = b.qkv.shape[0]
+        for lead, width in ((1, b.qkv.shape[1] + 1), (2, b.qkv.shape[1] + 6), (8, b.qkv.shape[1] + 8)):
+            wide = torch.zeros(m, width + lead, dtype=torch.bfloat16, device="cuda")
+            wide[:, lead:lead + b.qkv.shape[1]] = b.qkv
+            room = torch.zeros(m * heads * d + 8, dtype=torch.bfloat16, device="cuda")
+            out = room[lead:lead + m * heads * d].view(m, heads * d)
+            ops.attention_int8(wide[:, lead:lead + b.qkv.shape[1]], out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, page, *b.pools, *b.pool_scales)
+            # another kernel takes some of them: its weights are not rounded to 16 bits
+            assert (out.double() - want.double()).abs().max() <= 2.0 ** -6 * want.double().abs().max()
+            assert (room[:lead] == 0).all() and (room[lead + m * heads * d:] == 0).all()
+        pools = [torch.zeros(p.numel() + 16, dtype=torch.int8, device="cuda")[8:8 + p.numel()].view(p.shape).copy_(p) for p in b.pools]
+        out = torch.empty_like(want)
+        ops.attention_int8(b.qkv, out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, page, *pools, *b.pool_scales)
+        assert (out.double() - want.double()).abs().max() <= 2.0 ** -6 * want.double().abs().max()
+
+
+def test_pools_of_more_than_2_to_the_31_codes(ops):
+    heads, kv, d, page, pages = 8, 8, 128, 64, 36000          # 2.4e9 codes
+    b = Batch(heads, kv, d, d, page, [1, 70], [130, 60], torch.bfloat16, seed=61)
+    small = b.pools[0].shape[0]
+    pools = [torch.zeros(pages, kv, page, d, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(pages, kv, dtype=torch.float32, device="cuda") for _ in range(2)]
+    for j in range(2):
+        pools[j][-small:] = b.pools[j]
+        scales[j][-small:] = b.pool_scales[j]
+    table = torch.where(b.table >= 0, b.table + pages - small, b.table)
+    q, q2 = (torch.empty(71, heads * d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ops.rope_store_int8(b.qkv, q, heads, kv, d, b.ctx, b.rotary, table, page, *pools, *scales)
+    b.append(ops, q_out=q2)
+    for j in range(2):
+        assert torch.equal(pools[j][-small:], b.pools[j]) and torch.equal(scales[j][-small:], b.pool_scales[j]) and (pools[j][:-small] == 0).all()
+    b.qkv = q2
+    want, out = attention_rows(ops, b), torch.empty_like(q)
+    ops.attention_int8(q, out, heads, kv, d, d ** -0.5, 0, b.ctx, table, page, *pools, *scales)
+    assert torch.equal(q, q2) and torch.equal(out, want)
+
+
+def test_two_streams_at_once_and_a_replayed_graph(ops):
+    """Calls on two streams share nothing; a captured pair of calls follows its inputs' contents."""
+    batches = [Batch(14, 2, 64, 64, 16, [1] * n, [300 + 700 * i for i in range(n)], torch.bfloat16, seed=70 + n) for n in (3, 5)]
+    want = []
+    for b in batches:
+        q = b.append(ops)
+        want.append(attention_of(ops, b, q))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i, (b, st) in enumerate(zip(batches, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(attention_of(ops, b, b.append(ops)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+    b = batches[1]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        out = attention_of(ops, b, b.append(ops))
+        graph.capture_end()
+    torch.cuda.current_stream().wait_stream(side)
+    b.qkv.copy_(b.qkv.flip(0))
+    b.ctx.ctx_lens.sub_(1)
+    b.ctx.positions.sub_(1)
+    graph.replay()
+    replayed = out.clone()
+    assert torch.equal(replayed, attention_of(ops, b, b.append(ops))) and not torch.equal(replayed, want[1])
+
+
+def attention_of(ops, b, q):
+    out = torch.empty_like(q)
+    ops.attention_int8(q, out, b.heads, b.kv, b.d, b.d ** -0.5, 0, b.ctx, b.table, b.page, *b.pools, *b.pool_scales)
+    return out
+
+
+def test_every_way_of_cutting_the_keys_gives_the_row(ops):
+    """Clusters of one to eight CTAs, and shares: against 64 bits."""
+    for heads, kv, d, dtype in ((14, 2, 64, torch.bfloat16), (20, 2, 128, torch.bfloat16), (4, 2, 32, torch.bfloat16), (6, 3, 64, torch.float32)):
+        b = Batch(heads, kv, d, 0, 16, [1, 1, 1, 1], [700, 3, 1500, 64], dtype, seed=80)
+        b.ctx.ctx_lens[3] = 0           # a padding row
+        for splits in (1, 2, 4, 8, 9, 40, 200):
+            check_attention_rows(ops.with_options(fixed_decode_splits=splits), b, skip=3)
+
+
+def check_attention_rows(ops, b, skip):
+    out = torch.full((b.qkv.shape[0], b.heads * b.d), float("nan"), dtype=b.dtype, device="cuda")
+    ops.attention_int8(b.qkv, out, b.heads, b.kv, b.d, b.d ** -0.5, 0, b.ctx, b.table, b.page, *b.pools, *b.pool_scales)
+    keys, vals = (ref.values(c.cpu(), s.cpu()) for c, s in zip(b.pools, b.pool_scales))
+    rounding = (2.0 ** -8 if b.dtype == torch.bfloat16 else 0.0) + 2.0 ** -14
+    for i, p in enumerate(b.before):
+        if i == skip:
+            assert (out[i] == 0).all()
+            continue
+        want, size, small = ref.attend(b.rows[i, :b.heads], keys, vals, b.pool_scales[1].cpu(), b.table.cpu().tolist()[i], b.page, p, b.d ** -0.5, 0, b.kv)
+        assert ((out[i].cpu().double().reshape(b.heads, b.d) - want).abs() <= HALF_STEP[b.dtype] * want.abs() + rounding * size + 2.0 ** -25 * small).all(), i
+
+
+def test_contexts_of_one_token_and_many_requests(ops):
+    check_attention(ops, Batch(4, 2, 64, 0, 16, [1] * 130, [(37 * i) % 90 for i in range(130)], torch.bfloat16, seed=81))
+    check_attention(ops, Batch(4, 2, 128, 0, 16, [1] * 70, [(i % 3) * 17 for i in range(70)], torch.bfloat16, seed=82))
+
+
 def test_refusals(ops):
     from nanoinfer_b200.csrc.lib import KernelError
     b = Batch(4, 2, 64, 64, 16, [1, 3], [5, 25], torch.bfloat16, seed=50)      # (a table of two columns: one of one column is dense turned over, too)
