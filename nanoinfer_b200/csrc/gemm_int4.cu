@@ -470,11 +470,12 @@ template <int R, bool DUAL, bool G32, bool F16>
 int by_tokens(const Args& a, int blocks, cudaStream_t stream) {
     if (a.tokens <= 8) return launch<1, R, DUAL, G32, F16>(a, blocks, stream);
     if (a.tokens <= 16) return launch<2, R, DUAL, G32, F16>(a, blocks, stream);
-    if constexpr (R <= 2) {
+    if constexpr (R <= 2 && !F16) {
         if (a.tokens <= 32) return launch<4, R, DUAL, G32, F16>(a, blocks, stream);
         return launch<8, R, DUAL, G32, F16>(a, blocks, stream);
     }
-    return 1;       // (four row tiles are up to 16 tokens' choice)
+    nib_set_error("gemm_int4: four row tiles a warp and prepared activations are for up to 16 tokens");
+    return 1;
 }
 
 bool fits(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0; }
@@ -484,17 +485,14 @@ bool fits(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || gr
 // The arguments of a product, one block of memory.
 struct NibGemmInt4 {
     const void* x; const void* w; const void* scales; const float* bias; void* out;
-    void* scratch;                                      // nib_gemm_int4_scratch bytes, 16-byte aligned
+    void* scratch;              // nib_gemm_int4_scratch bytes, 16-byte aligned; without, the codes meet the activations as they are
     int tokens, n, k, group, ldx, ldo, epi, sms;        // sms: SMs of the device
     float alpha, limit, shift;                          // the constants of EPI_GLU
     int pad;
 };
 
-// Whether a product's activations are prepared as 16-bit floats, and the scratch bytes that takes (0: not).
-static long long f16_scratch(int tokens, int n, int k, bool dual) {
-    return (long long)(dual ? 2 : 1) * n * k / 2 >= (48LL << 20) && tokens <= 16 ? (long long)tokens * k * 2 + (long long)ceil_div(k, 32) * 64 * 4 + 256 : 0;
-}
-NIB_API long long nib_gemm_int4_scratch(int tokens, int n, int k, int dual) { return tokens > 64 ? 0 : f16_scratch(tokens, n, k, dual != 0); }
+// Bytes of scratch with which a product prepares its activations as 16-bit floats.
+NIB_API long long nib_gemm_int4_scratch(int tokens, int k) { return (long long)tokens * k * 2 + (long long)ceil_div(k, 32) * 64 * 4 + 256; }
 
 // out[tokens, n] from the packed weights of n rows (of 2 n rows, gate then up, for the gated epilogues). -1, and nothing done, where
 // another product has to take these operands: more than 64 tokens, rows that do not begin on 16 bytes, a gated product whose halves
@@ -507,10 +505,11 @@ NIB_API int nib_gemm_int4(const void* args, cudaStream_t stream) {
     NIB_REQUIRE(tokens >= 0 && sms > 0 && fits(n, k, group), "gemm_int4: %d tokens, %d x %d weights in groups of %d are not supported", tokens, n, k, group);
     NIB_REQUIRE(epi == EPI_STORE || epi == EPI_ADD || epi == EPI_F32 || dual, "gemm_int4: unknown epilogue %d", epi);
     NIB_REQUIRE((((uintptr_t)c.w) & 15) == 0 && (((uintptr_t)c.scales) & 3) == 0, "gemm_int4: weights must be 16-byte aligned");
+    NIB_REQUIRE(((uintptr_t)c.scratch & 15) == 0, "gemm_int4: scratch must be 16-byte aligned");
     if (tokens > 64 || c.ldx % 8 != 0 || ((uintptr_t)c.x & 15) != 0 || (dual && n % 16 != 0)) return -1;
     if (tokens == 0) return 0;
     const int out_tiles = ceil_div(n, 16);
-    const bool g32 = group == 32, f16 = c.scratch != nullptr && f16_scratch(tokens, n, k, dual) > 0;
+    const bool g32 = group == 32, f16 = c.scratch != nullptr;
     Args a{(const __nv_bfloat16*)c.x, (const uint4*)c.w, (const unsigned*)c.scales, c.bias, c.out, nullptr, nullptr, tokens, n, k, c.ldx, c.ldo, epi,
            dual ? 2 * out_tiles : out_tiles, ceil_div(k, 64), group == 32 ? 5 : group == 64 ? 6 : 7, k / group, 1, 1, NibGlu{c.alpha, c.limit, c.shift}};
     if (f16) {

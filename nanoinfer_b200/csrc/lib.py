@@ -161,6 +161,7 @@ class Kernels:
             getattr(self._lib, name).restype = c_int
         self.sample_rows_most = int(self._lib.nib_sample_rows_most())      # rows whose parameters a launch takes by value
         self._lib.nib_gemm_int4_scratch.restype = c_longlong
+        self._lib.nib_unpack_int8.argtypes = [c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p]
         self._lib.nib_grouped_state_scratch.restype = self._lib.nib_decay_state_scratch.restype = c_longlong
 
     # ---- plumbing ---------------------------------------------------------------------------
@@ -536,8 +537,8 @@ class Kernels:
         if isinstance(a, LazyNorm):
             a = self._resolve(a, a.shape[0] <= 16)
         device = torch.cuda.current_device()
-        for name, t in (("a", a), ("out", out), ("w", w.packed)):
-            if t.get_device() != device:
+        if not device == a.get_device() == out.get_device() == w.packed.get_device():
+            for name, t in (("a", a), ("out", out), ("w", w.packed)):
                 _here(t, None, f"{what} {name}", contiguous=False)
         epi = _EPI[mode]
         dual = epi in _DUAL
@@ -559,7 +560,10 @@ class Kernels:
             if not self.weights_ahead:
                 self._lib.nib_pdl_skip_next()
             alpha, limit, shift = (0.0, 0.0, 0.0) if glu is None else glu
-            scratch = self._lib.nib_gemm_int4_scratch(m, n, k, 1 if dual else 0)
+            # Activations prepared as 16-bit floats: 11 instructions of every tile's 65 for a kernel of two microseconds before, which pays
+            # where a product takes twenty (7B widths, us with / without: gate/up at 8 tokens 18.8 / 23.1, at 16 24.4 / 26.4, at 32 45.8 /
+            # 42.5; down at 8 23.0 / 20.7).
+            scratch = self._lib.nib_gemm_int4_scratch(m, k) if m <= 16 and w.packed.numel() >= 48 << 20 else 0
             room = torch.empty(scratch, dtype=torch.uint8, device=a.device) if scratch else None
             args = _GEMM_INT4.pack(a.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), 0 if bias32 is None else bias32.data_ptr(), out.data_ptr(),
                                    0 if room is None else room.data_ptr(), m, n, k, w.group, a.stride(0), out.stride(0), epi, self.sm_count, alpha, limit, shift, 0)
@@ -770,11 +774,17 @@ class Kernels:
     def _cache_int8(what, qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales) -> int:
         """Refuses pools, scales, a block table or a step that the kernels of the 8-bit cache cannot take, or tensors of another device
         than the current one; returns the number of the step's requests."""
-        device = torch.cuda.current_device()
-        for name, t, dtype in (("k_pages", k_pages, torch.int8), ("v_pages", v_pages, torch.int8), ("k_scales", k_scales, torch.float32),
-                               ("v_scales", v_scales, torch.float32), ("positions", ctx.positions, torch.int32), ("req_index", ctx.req_index, torch.int32),
-                               ("q_start", ctx.q_start, torch.int32), ("ctx_lens", ctx.ctx_lens, torch.int32)):
-            if t.get_device() != device or t.dtype != dtype or not t.is_contiguous():
+        device, i8, i32, f32 = torch.cuda.current_device(), torch.int8, torch.int32, torch.float32
+        positions, req_index, q_start, ctx_lens = ctx.positions, ctx.req_index, ctx.q_start, ctx.ctx_lens
+        # (one condition for all: a decode step of few tokens waits for the host, and this is called for every layer of it)
+        if not (k_pages.dtype is i8 and v_pages.dtype is i8 and k_scales.dtype is f32 and v_scales.dtype is f32 and positions.dtype is i32
+                and req_index.dtype is i32 and q_start.dtype is i32 and ctx_lens.dtype is i32
+                and device == k_pages.get_device() == v_pages.get_device() == k_scales.get_device() == v_scales.get_device() == positions.get_device()
+                == req_index.get_device() == q_start.get_device() == ctx_lens.get_device()
+                and k_pages.is_contiguous() and v_pages.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()
+                and positions.is_contiguous() and req_index.is_contiguous() and q_start.is_contiguous() and ctx_lens.is_contiguous()):
+            for name, t, dtype in (("k_pages", k_pages, i8), ("v_pages", v_pages, i8), ("k_scales", k_scales, f32), ("v_scales", v_scales, f32),
+                                   ("positions", positions, i32), ("req_index", req_index, i32), ("q_start", q_start, i32), ("ctx_lens", ctx_lens, i32)):
                 _here(t, dtype, f"{what} {name}")
         pages = k_pages.shape[0]
         if k_pages.numel() == 0 or k_pages.shape != (pages, kv_heads, page_size, head_dim) or v_pages.shape != k_pages.shape:
@@ -788,8 +798,8 @@ class Kernels:
         if block_table.dim() != 2 or block_table.stride(1) != 1:
             raise KernelError(f"{what}: block_table rows must be dense")
         m, n_req = qkv.shape[0], len(ctx.host.q_lens)
-        if sum(ctx.host.q_lens) != m or ctx.positions.numel() < m or ctx.req_index.numel() < m or ctx.q_start.numel() != n_req + 1 \
-                or ctx.ctx_lens.numel() != n_req or block_table.shape[0] < n_req:
+        if sum(ctx.host.q_lens) != m or positions.numel() < m or req_index.numel() < m or q_start.numel() != n_req + 1 \
+                or ctx_lens.numel() != n_req or block_table.shape[0] < n_req:
             raise KernelError(f"{what}: the step's lengths do not fit {m} rows and {block_table.shape[0]} rows of the block table")
         return n_req
 
@@ -816,7 +826,8 @@ class Kernels:
                     or not cos_t.is_contiguous() or not sin_t.is_contiguous() or cos_t.dim() != 2 or cos_t.shape[1] != rot // 2 or sin_t.shape != cos_t.shape:
                 raise KernelError("rope_store_int8: the tables are dense float32 [positions, rot/2] on the device of the rows")
             cos, sin, rows = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0]
-        units = sum((n + page_size - 2) // page_size + 1 for n in ctx.host.q_lens)
+        # (a request has no more units than tokens)
+        units = m if m == n_req else sum((n + page_size - 2) // page_size + 1 for n in ctx.host.q_lens)
         args = _APPEND_INT8.pack(
             qkv.data_ptr(), q_out.data_ptr(), ctx.positions.data_ptr(), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), cos, sin, block_table.data_ptr(),
             k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), qkv.stride(0), q_out.stride(0), n_req, units, rows, rot,
@@ -828,14 +839,14 @@ class Kernels:
         """out = what the codes of a pool stand for: ``pages`` int8 [pages, kv_heads, page_size, head_dim], ``scales`` a float for each
         page and kv head, ``out`` of the pool's shape in bfloat16 or float32 (both hold the values exactly)."""
         device = torch.cuda.current_device()
-        for name, t, dtype in (("pages", pages, torch.int8), ("scales", scales, torch.float32), ("out", out, out.dtype)):
-            if t.get_device() != device or t.dtype != dtype or not t.is_contiguous():
-                _here(t, dtype, f"unpack_int8 {name}")
+        if not (pages.dtype is torch.int8 and scales.dtype is torch.float32 and device == pages.get_device() == scales.get_device() == out.get_device()
+                and pages.is_contiguous() and scales.is_contiguous() and out.is_contiguous()):
+            _here(pages, torch.int8, "unpack_int8 pages"); _here(scales, torch.float32, "unpack_int8 scales"); _here(out, None, "unpack_int8 out")
         if pages.dim() != 4 or scales.numel() != pages.shape[0] * pages.shape[1] or out.shape != pages.shape or out.dtype not in _DT:
             raise KernelError(f"unpack_int8: pages {tuple(pages.shape)}, scales {tuple(scales.shape)} and {out.dtype} {tuple(out.shape)} do not fit")
         if pages.numel() == 0:
             return
-        self._check(self._lib.nib_unpack_int8(_ptr(pages), _ptr(scales), _ptr(out), c_longlong(scales.numel()), pages.shape[2] * pages.shape[3],
+        self._check(self._lib.nib_unpack_int8(pages.data_ptr(), scales.data_ptr(), out.data_ptr(), scales.numel(), pages.shape[2] * pages.shape[3],
                                               _DT[out.dtype], self._stream()), "unpack (8-bit cache)")
 
     def attention_int8(self, qkv, out, heads, kv_heads, head_dim, scale, window, ctx, block_table, page_size, k_pages, v_pages, k_scales, v_scales,
@@ -854,6 +865,8 @@ class Kernels:
             return
         n_dec, q_lens = 0, ctx.host.q_lens
         kind = self._lib.nib_attention_int8_decode_kind(heads, kv_heads, head_dim, page_size, dtype)
+        if kind >= 0 and m == n_req and max(q_lens) == 1:
+            n_dec = n_req
         while kind >= 0 and n_dec < n_req and q_lens[n_dec] == 1:
             n_dec += 1
         if n_dec:

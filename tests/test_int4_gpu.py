@@ -70,26 +70,51 @@ def test_products_of_many_rows(ops):
 
 
 def test_products_of_few_tokens_with_many_weights(ops):
-    """From 4 MB of codes on the activations are prepared as 16-bit floats."""
     for n, k, group in ((2080, 4128, 32), (2050, 4096, 64), (2064, 4352, 128)):
         for i, m in enumerate((1, 3, 8, 9, 16, 24, 40, 64)):
             check(ops, n, k, group, m, ("f32", "store", "add")[i % 3], bias=i % 2 == 0, seed=m)
 
 
-def test_many_weights_with_activations_of_very_different_sizes(ops):
-    """A token's own size does not matter (its largest element takes a power of two to 2^13), nor do elements far below the largest:
-    what 16 bits lose of them is 2^-38 of the largest."""
-    n, k = 2080, 4096
-    w, w64 = matrix(n, k, 64, 3)
+def large(n, k, group, seed):
+    """As ``matrix``, made and kept on the device."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 16, (n, k), generator=g, device="cuda").to(torch.uint8)
+    scales = (torch.exp(torch.randn(n, k // group, generator=g, device="cuda")) * k ** -0.5 / 4).to(torch.bfloat16)
+    return Int4Matrix.from_codes(codes, scales, group), (codes.double() - 8) * scales.double().repeat_interleave(group, dim=1)
+
+
+@pytest.mark.parametrize("n,k,group", [(25610, 4128, 32), (24600, 4096, 64), (24600, 4096, 128)])
+def test_products_whose_activations_are_prepared(ops, n, k, group):
+    """From 48 MB of codes on, up to 16 tokens. A token's own size does not matter (its largest element takes a power of two to 2^13),
+    nor do elements far below the largest: what 16 bits lose of them is 2^-38 of the largest."""
+    w, w64 = large(n, k, group, 3)
+    assert w.packed.numel() >= 48 << 20
     g = torch.Generator().manual_seed(4)
-    x = torch.randn(9, k, generator=g) * torch.exp2(torch.randint(-20, 21, (9, k), generator=g).float())
-    x *= torch.exp2(torch.tensor([0.0, -100.0, 80.0, -30.0, 15.0, 60.0, -60.0, 3.0, 0.0]))[:, None]
-    x[8] = 0.0
-    x = x.to(torch.bfloat16)
-    out = torch.empty(9, n, dtype=torch.float32, device="cuda")
-    ops.linear(x.cuda(), w, None, out, "f32")
-    bound = bounds(x, w64, False) + x.double().abs().amax(dim=1, keepdim=True) * 2.0 ** -38 * w64.abs().sum(dim=1)[None]
-    assert ((out.cpu().double() - x.double() @ w64.T).abs() <= bound).all()
+    for m in (1, 8, 9, 16):
+        x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-20, 21, (m, k), generator=g).float())
+        x *= torch.exp2(torch.randint(-100, 81, (m, 1), generator=g).float())
+        x[m // 2] = torch.randn(k, generator=g) if m > 1 else x[0]
+        x = x.to(torch.bfloat16).cuda()
+        if m == 9:
+            x[8] = 0.0
+        out = torch.empty(m, n, dtype=torch.float32, device="cuda")
+        ops.linear(x, w, None, out, "f32")
+        bound = bounds(x, w64, False) + x.double().abs().amax(dim=1, keepdim=True) * 2.0 ** -38 * w64.abs().sum(dim=1)[None]
+        assert ((out.double() - x.double() @ w64.T).abs() <= bound).all(), m
+        half = torch.empty(m, n // 2, dtype=torch.bfloat16, device="cuda")
+        if n // 2 % 16 == 0:
+            y = x[m // 2:m // 2 + 1].contiguous()
+            ops.linear_swiglu(y, w, half[:1])
+            v = y.double() @ w64.T
+            want, e = torch.nn.functional.silu(v[:, :n // 2]) * v[:, n // 2:], bounds(y, w64, False)
+            slope = 1.2 * (v[:, :n // 2].abs() + v[:, n // 2:].abs() + 2)
+            assert ((half[:1].double() - want).abs() <= slope * (e[:, :n // 2] + e[:, n // 2:] + 2.0 ** -19) + 2.0 ** -8 * want.abs()).all()
+    x = torch.randn(3, k, generator=g).to(torch.bfloat16).cuda()
+    clean, out = (torch.empty(3, n, dtype=torch.float32, device="cuda") for _ in range(2))
+    ops.linear(x, w, None, clean, "f32")
+    x[1, 7] = float("inf")
+    ops.linear(x, w, None, out, "f32")
+    assert not torch.isfinite(out[1]).any() and torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2])
 
 
 @pytest.mark.parametrize("narrow", [False, True])
