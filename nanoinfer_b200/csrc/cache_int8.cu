@@ -241,7 +241,8 @@ rotate_queries_kernel(const T* qkv, T* q_out, const AppendArgs a, long long item
 // WIDE: chunks of 8 elements of queries and values and 4 of keys; 1 where widths or addresses do not allow it.
 // QUERIES: CTAs from kv_blocks on rotate a token's queries each (one launch for few tokens). Without, the kernel that rotates them
 // runs before and beside this one: it lets this one in when what both read is complete, and this one waits for it at its end.
-template <typename T, int V> struct KeyItem { float x1[V], x2[V], cs[V], sn[V]; int row, d; bool pair; };       // the second chunk only of a rotated pair
+template <typename T, int V> struct KeyRaw { float x1[V], x2[V], cs[V], sn[V]; int row, d; bool pair; };       // the second chunk only of a rotated pair
+template <int V> struct KeyItem { Two y1[V], y2[V]; int row, d; bool pair; };
 template <typename T, int V> struct ValueItem { float x[V]; int row, d; };
 
 template <typename T, bool WIDE, bool QUERIES>
@@ -277,7 +278,7 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
     const int k_items = unit.count * k_per_token, v_items = unit.count * v_per_token;
     const int k_first = tid, v_first = (tid + KV_THREADS / 2) % KV_THREADS;       // (few items: keys and values are different warps')
 
-    auto load_key = [&](KeyItem<T, V>& it, int i) {
+    auto load_key = [&](KeyRaw<T, V>& it, int i) {
         it.row = i / k_per_token;
         const int c = i - it.row * k_per_token;
         it.pair = c < pairs;
@@ -301,29 +302,43 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
         it.d = (i - it.row * v_per_token) * VV;
         Vec<T, VV>::load(it.x, v_rows + (size_t)it.row * a.q_stride + it.d);
     };
-    auto first_of = [&](const KeyItem<T, V>& it, int j) { return it.pair ? sum_of_products(it.x1[j], it.cs[j], -it.x2[j], it.sn[j]) : Two{it.x1[j], 0.f}; };
-    auto second_of = [&](const KeyItem<T, V>& it, int j) { return sum_of_products(it.x2[j], it.cs[j], it.x1[j], it.sn[j]); };
-
-    KeyItem<T, V> key[B];
+    auto turned = [&](KeyItem<V>& it, const KeyRaw<T, V>& raw) {
+        it.row = raw.row; it.d = raw.d; it.pair = raw.pair;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            it.y1[j] = Two{raw.x1[j], 0.f};
+            it.y2[j] = Two{0.f, 0.f};
+            if (raw.pair) {
+                it.y1[j] = sum_of_products(raw.x1[j], raw.cs[j], -raw.x2[j], raw.sn[j]);
+                it.y2[j] = sum_of_products(raw.x2[j], raw.cs[j], raw.x1[j], raw.sn[j]);
+            }
+        }
+    };
+    // a turn's keys and values, loads first
+    KeyItem<V> key[B];
     ValueItem<T, VV> value[B];
     unsigned k_top = 0, v_top = 0;
     const int turns = max((k_items + TURN - 1) / TURN, (v_items + TURN - 1) / TURN);
-    for (int turn = 0; turn < turns; ++turn) {
+    auto take = [&](int turn) {
+        KeyRaw<T, V> raw[B];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int at = turn * TURN + b * KV_THREADS;
-            if (at + k_first < k_items) load_key(key[b], at + k_first);
+            if (at + k_first < k_items) load_key(raw[b], at + k_first);
             if (at + v_first < v_items) load_value(value[b], at + v_first);
         }
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (turn * TURN + b * KV_THREADS + k_first < k_items) turned(key[b], raw[b]);
+    };
+    for (int turn = 0; turn < turns; ++turn) {
+        take(turn);
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int at = turn * TURN + b * KV_THREADS;
             if (at + k_first < k_items) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    k_top = max(k_top, magnitude_up(first_of(key[b], j)));
-                    if (key[b].pair) k_top = max(k_top, magnitude_up(second_of(key[b], j)));
-                }
+                for (int j = 0; j < V; ++j) k_top = max(k_top, max(magnitude_up(key[b].y1[j]), magnitude_up(key[b].y2[j])));
             }
             if (at + v_first < v_items) {
 #pragma unroll
@@ -340,14 +355,7 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
     const float k_scale = scale_of(k_top, k_old, unit.slot, k_codes, hd, tid), v_scale = scale_of(v_top, v_old, unit.slot, v_codes, hd, tid);
     const float k_inv = 1.0f / k_scale, v_inv = 1.0f / v_scale;
     for (int turn = 0; turn < turns; ++turn) {
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const int at = turn * TURN + b * KV_THREADS;
-            if (turns > 1) {            // (else the items are still at hand)
-                if (at + k_first < k_items) load_key(key[b], at + k_first);
-                if (at + v_first < v_items) load_value(value[b], at + v_first);
-            }
-        }
+        if (turns > 1) take(turn);          // (else the items are still at hand)
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int at = turn * TURN + b * KV_THREADS;
@@ -355,11 +363,11 @@ append_int8_kernel(const T* qkv, T* q_out, const AppendArgs a) {        // (q_ou
                 signed char* dst = k_codes + (size_t)(unit.slot + key[b].row) * hd + key[b].d;
                 int c[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) c[j] = code_of(first_of(key[b], j), k_inv);
+                for (int j = 0; j < V; ++j) c[j] = code_of(key[b].y1[j], k_inv);
                 store_codes<V>(dst, c);
                 if (key[b].pair) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) c[j] = code_of(second_of(key[b], j), k_inv);
+                    for (int j = 0; j < V; ++j) c[j] = code_of(key[b].y2[j], k_inv);
                     store_codes<V>(dst + half, c);
                 }
             }
