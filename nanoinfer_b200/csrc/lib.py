@@ -771,9 +771,10 @@ class Kernels:
 
     # ---- the 8-bit cache of keys and values (cache_int8.cu, attention_int8.cu) ----------------------------------------------
     @staticmethod
-    def _cache_int8(what, qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales) -> int:
+    def _cache_int8(what, qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales):
         """Refuses pools, scales, a block table or a step that the kernels of the 8-bit cache cannot take, or tensors of another device
-        than the current one; returns the number of the step's requests."""
+        than the current one; returns what has been looked up: the step's requests, the rows, their width and stride, the pages of the
+        pool, the width and stride of the table."""
         device, i8, i32, f32 = torch.cuda.current_device(), torch.int8, torch.int32, torch.float32
         positions, req_index, q_start, ctx_lens = ctx.positions, ctx.req_index, ctx.q_start, ctx.ctx_lens
         # (one condition for all: a decode step of few tokens waits for the host, and this is called for every layer of it)
@@ -786,22 +787,24 @@ class Kernels:
             for name, t, dtype in (("k_pages", k_pages, i8), ("v_pages", v_pages, i8), ("k_scales", k_scales, f32), ("v_scales", v_scales, f32),
                                    ("positions", positions, i32), ("req_index", req_index, i32), ("q_start", q_start, i32), ("ctx_lens", ctx_lens, i32)):
                 _here(t, dtype, f"{what} {name}")
-        pages = k_pages.shape[0]
-        if k_pages.numel() == 0 or k_pages.shape != (pages, kv_heads, page_size, head_dim) or v_pages.shape != k_pages.shape:
+        shape = k_pages.shape
+        pages = shape[0]
+        if k_pages.numel() == 0 or shape != (pages, kv_heads, page_size, head_dim) or v_pages.shape != shape:
             raise KernelError(f"{what}: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} do not fit kv_heads/page_size/head_dim")
         if k_scales.numel() != pages * kv_heads or v_scales.numel() != pages * kv_heads:
             raise KernelError(f"{what}: scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}: one for each page and kv head")
         if qkv.get_device() != device or block_table.get_device() != device or block_table.dtype != torch.int32:
             _here(qkv, None, f"{what} qkv"); _here(block_table, torch.int32, f"{what} block_table", contiguous=False)
-        if qkv.dtype not in _DT or qkv.dim() != 2 or qkv.stride(1) != 1:
+        rows, table, row_stride, table_stride = qkv.shape, block_table.shape, qkv.stride(), block_table.stride()
+        if qkv.dtype not in _DT or len(rows) != 2 or row_stride[1] != 1:
             raise KernelError(f"{what}: dense rows of bfloat16 or float32, not {qkv.dtype} {tuple(qkv.shape)}")
-        if block_table.dim() != 2 or block_table.stride(1) != 1:
+        if len(table) != 2 or table_stride[1] != 1:
             raise KernelError(f"{what}: block_table rows must be dense")
-        m, n_req = qkv.shape[0], len(ctx.host.q_lens)
+        m, n_req = rows[0], len(ctx.host.q_lens)
         if sum(ctx.host.q_lens) != m or positions.numel() < m or req_index.numel() < m or q_start.numel() != n_req + 1 \
-                or ctx_lens.numel() != n_req or block_table.shape[0] < n_req:
-            raise KernelError(f"{what}: the step's lengths do not fit {m} rows and {block_table.shape[0]} rows of the block table")
-        return n_req
+                or ctx_lens.numel() != n_req or table[0] < n_req:
+            raise KernelError(f"{what}: the step's lengths do not fit {m} rows and {table[0]} rows of the block table")
+        return n_req, m, rows[1], row_stride[0], pages, table[1], table_stride[0]
 
     def rope_store_int8(self, qkv, q_out, heads, kv_heads, head_dim, ctx, rotary, block_table, page_size, k_pages, v_pages, k_scales, v_scales):
         """Rotates the queries of the rows [q heads | k heads | v heads] of ``qkv`` by their positions into ``q_out`` [m, heads *
@@ -813,25 +816,28 @@ class Kernels:
         the rounding to a larger scale, if a new token needs one; a page that the step begins anew forgets its old scale. A
         token whose key or value is not finite, or whose position the tables of ``rotary`` do not hold, makes its block's scale NaN.
         No two requests may append to the same page."""
-        n_req = self._cache_int8("rope_store_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales)
-        m, device = qkv.shape[0], qkv.get_device()
-        if qkv.shape[1] != (heads + 2 * kv_heads) * head_dim or q_out.shape != (m, heads * head_dim):
+        n_req, m, width, q_stride, pages, bt_width, bt_stride = self._cache_int8("rope_store_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table,
+                                                                                 k_pages, v_pages, k_scales, v_scales)
+        device = qkv.get_device()
+        if width != (heads + 2 * kv_heads) * head_dim or q_out.shape != (m, heads * head_dim):
             raise KernelError("rope_store_int8: widths do not fit the head counts")
-        if q_out.get_device() != device or q_out.dtype != qkv.dtype or q_out.stride(1) != 1:
+        out_stride = q_out.stride()
+        if q_out.get_device() != device or q_out.dtype != qkv.dtype or out_stride[1] != 1:
             raise KernelError(f"rope_store_int8: q_out is {q_out.dtype} on {q_out.device}, {qkv.dtype} in dense rows on {qkv.device} is wanted")
         cos = sin = rot = rows = 0
         if rotary is not None:
             cos_t, sin_t, rot = rotary
+            tables = cos_t.shape
             if cos_t.get_device() != device or sin_t.get_device() != device or cos_t.dtype != torch.float32 or sin_t.dtype != torch.float32 \
-                    or not cos_t.is_contiguous() or not sin_t.is_contiguous() or cos_t.dim() != 2 or cos_t.shape[1] != rot // 2 or sin_t.shape != cos_t.shape:
+                    or not cos_t.is_contiguous() or not sin_t.is_contiguous() or len(tables) != 2 or tables[1] != rot // 2 or sin_t.shape != tables:
                 raise KernelError("rope_store_int8: the tables are dense float32 [positions, rot/2] on the device of the rows")
-            cos, sin, rows = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0]
+            cos, sin, rows = cos_t.data_ptr(), sin_t.data_ptr(), tables[0]
         # (a request has no more units than tokens)
         units = m if m == n_req else sum((n + page_size - 2) // page_size + 1 for n in ctx.host.q_lens)
         args = _APPEND_INT8.pack(
             qkv.data_ptr(), q_out.data_ptr(), ctx.positions.data_ptr(), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), cos, sin, block_table.data_ptr(),
-            k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), qkv.stride(0), q_out.stride(0), n_req, units, rows, rot,
-            block_table.stride(0), block_table.shape[1], page_size, k_pages.shape[0], m, heads, kv_heads, head_dim, _DT[qkv.dtype], 0)
+            k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), q_stride, out_stride[0], n_req, units, rows, rot,
+            bt_stride, bt_width, page_size, pages, m, heads, kv_heads, head_dim, _DT[qkv.dtype], 0)
         self.launches += 1 if m > 64 else 0         # (queries, and keys and values, each a kernel)
         self._check(self._lib.nib_rope_store_int8(args, self._stream()), "rope_store (8-bit cache)")
 
@@ -842,11 +848,12 @@ class Kernels:
         if not (pages.dtype is torch.int8 and scales.dtype is torch.float32 and device == pages.get_device() == scales.get_device() == out.get_device()
                 and pages.is_contiguous() and scales.is_contiguous() and out.is_contiguous()):
             _here(pages, torch.int8, "unpack_int8 pages"); _here(scales, torch.float32, "unpack_int8 scales"); _here(out, None, "unpack_int8 out")
-        if pages.dim() != 4 or scales.numel() != pages.shape[0] * pages.shape[1] or out.shape != pages.shape or out.dtype not in _DT:
+        shape, blocks = pages.shape, scales.numel()
+        if len(shape) != 4 or blocks != shape[0] * shape[1] or out.shape != shape or out.dtype not in _DT:
             raise KernelError(f"unpack_int8: pages {tuple(pages.shape)}, scales {tuple(scales.shape)} and {out.dtype} {tuple(out.shape)} do not fit")
         if pages.numel() == 0:
             return
-        self._check(self._lib.nib_unpack_int8(pages.data_ptr(), scales.data_ptr(), out.data_ptr(), scales.numel(), pages.shape[2] * pages.shape[3],
+        self._check(self._lib.nib_unpack_int8(pages.data_ptr(), scales.data_ptr(), out.data_ptr(), blocks, shape[2] * shape[3],
                                               _DT[out.dtype], self._stream()), "unpack (8-bit cache)")
 
     def attention_int8(self, qkv, out, heads, kv_heads, head_dim, scale, window, ctx, block_table, page_size, k_pages, v_pages, k_scales, v_scales,
@@ -855,9 +862,10 @@ class Kernels:
         ``qkv``, the step's own keys and values are in the pages already. ``earlier_complete``: the caller promises that
         the pages before the one that a token's own key lies in are no running kernel's results (the engine's steps begin with a copy, which
         waits for the step before); single tokens' earlier pages are then sent for while the kernel before this one is still running."""
-        n_req = self._cache_int8("attention_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table, k_pages, v_pages, k_scales, v_scales)
-        m, dtype = qkv.shape[0], _DT[qkv.dtype]
-        if heads <= 0 or heads % kv_heads or qkv.shape[1] < heads * head_dim or out.shape != (m, heads * head_dim) or window < 0:
+        n_req, m, width, q_stride, pages, bt_width, bt_stride = self._cache_int8("attention_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table,
+                                                                                 k_pages, v_pages, k_scales, v_scales)
+        dtype = _DT[qkv.dtype]
+        if heads <= 0 or heads % kv_heads or width < heads * head_dim or out.shape != (m, heads * head_dim) or window < 0:
             raise KernelError("attention_int8: widths do not fit the head counts")
         if out.get_device() != qkv.get_device() or out.dtype != qkv.dtype or not out.is_contiguous():
             _here(out, qkv.dtype, "attention_int8 out")
@@ -880,8 +888,7 @@ class Kernels:
                 self.launches += 1
             args = _ATTEND_INT8.pack(
                 qkv.data_ptr(), out.data_ptr(), ctx.ctx_lens.data_ptr(), block_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, qkv.stride(0), block_table.stride(0), block_table.shape[1], page_size,
-                k_pages.shape[0], n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 1 if earlier_complete else 0, scale, 0)
+                k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, q_stride, bt_stride, bt_width, page_size, pages, n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 1 if earlier_complete else 0, scale, 0)
             self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
         if n_dec == n_req:
             return
@@ -907,7 +914,16 @@ class Kernels:
 
     def _decode_int8_split(self, n_tokens: int, kv_heads: int, max_ctx: int, window: int, kind: int, head_dim: int):
         """How the keys of decoding tokens over the 8-bit cache are cut: (CTAs of a cluster that share a row's keys, 0), or (1, the CTAs that
-        all rows' keys are dealt to)."""
+        all rows' keys are dealt to, with a second kernel for the rows that lie in several shares).
+
+        Measured on B200, us in a chain of such calls, by CTAs a row / dealt out. A row's CTAs while they are two an SM at most and
+        have 16 chunks each or less: one token of 777 keys, heads of 64, eight 3.4, four 3.8 / 4.6; 8 of 4,096 6.6 / 7.8; 64 of 1,000,
+        heads of 128, two 11.3, four 12.3 / 14.4; 64 of 2,000 18.0, 18.7 / 24.0; 64 of 1,000 with 4 kv heads, one 17.2, two 18.8 / 29.0. With
+        rows enough for every SM the SMs even out different lengths by themselves: 64 of 4,000 with 4 kv heads, four 61.9 / 66.0; 64
+        of 200 to 4,000, heads of 64, 16.0 / 15.1, of 128 28.1 / 23.4 (with keys from memory 16.1 / 20.7 and 25.3 / 28.2). Few long rows are
+        dealt out, to at most 64 CTAs a row: one token of 32,000 keys, two kv heads, 128 CTAs 9.1, 500 10.9, eight CTAs a row 27; 8 of
+        32,768 65.9 (eight 69.7, and what the longest row takes where lengths differ). The general kernel takes longer for a chunk and is
+        dealt out from two chunks a CTA on: 4 of 150 to 300 keys in 32 bits 10.0 / 8.3."""
         keys = max(1, min(max_ctx, window) if window > 0 else max_ctx)
         units = max(1, n_tokens * kv_heads)
         chunk = 32 if kind == 0 else 128 if head_dim == 64 else 64          # keys that a CTA takes at a time
