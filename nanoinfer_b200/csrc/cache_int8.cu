@@ -17,7 +17,8 @@
 // products: an element is formed as the sum of a float and what its rounding left (the products' errors by a fused multiply-add, the
 // sum's by the two-sum), some 48 bits, of which the second part decides ties. (In 64 bits it was twice as slow: conversions.)
 //
-// What bounds it: a decode step's launch and three dependent loads; for a prompt's portion the bytes, queries above all.
+// What bounds it: a decode step's launch and three dependent loads (2.7 us a call in a chain, one token of 14 + 2 x 2 heads of 64); for a
+// prompt's portion loads that wait for loads, and the queries' bytes (3,789 tokens of 28 + 2 x 4 heads of 128: 19.8 us, 66 MB).
 #include "common.cuh"
 
 namespace {
