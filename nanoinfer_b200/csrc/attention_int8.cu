@@ -863,9 +863,8 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     if (kind == 1 && ((uintptr_t)q & 3) == 0 && c.q_stride % 2 == 0 && ((uintptr_t)out & 7) == 0 && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0) {
 #define CALL(KERNEL, T, CH, THREADS, SMEM, MOST)                                                                                \
     do {                                                                                                                        \
-        static const cudaError_t set = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MOST));  \
-        NIB_CUDA(set);                                                                                                          \
-        rc = launch_rows<T, CH>(KERNEL, a, THREADS, SMEM, q, out, stream);                                                      \
+        NIB_CUDA((allow_smem_once<KERNEL>((int)(MOST))));                                                                       \
+        rc = launch_rows<T, CH>((KERNEL), a, THREADS, SMEM, q, out, stream);                                                      \
     } while (0)
 #define MMA(HD, NH, WHOLE)                                                                                                      \
     CALL((attention_int8_mma_kernel<HD, NH, WHOLE>), __nv_bfloat16, (Mma<HD, NH>::CHUNK), WARPS * 32, (Mma<HD, NH>::BYTES), (Mma<HD, NH>::BYTES))

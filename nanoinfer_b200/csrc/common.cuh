@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -94,6 +95,19 @@ __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepc
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
 bool nib_pdl_enabled();
+
+// The most dynamic shared memory that launches of ``KERNEL`` take, set once for each device (the attribute is a kernel's on a device).
+template <auto KERNEL>
+static inline cudaError_t allow_smem_once(int bytes) {
+    static std::atomic<unsigned long long> configured{0};       // a bit a device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (e != cudaSuccess || (configured.load(std::memory_order_relaxed) & bit)) return e;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) configured.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,

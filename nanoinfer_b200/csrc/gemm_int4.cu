@@ -439,8 +439,7 @@ unpack_int4_kernel(const uint4* __restrict__ w, const unsigned* __restrict__ sca
 template <int NT, int R, bool DUAL, bool G32, bool F16>
 int launch(const Args& a, int blocks, cudaStream_t stream) {
     constexpr int bytes = Ring<NT, R, G32, F16>::BYTES;
-    static const cudaError_t set = cudaFuncSetAttribute(gemm_int4_kernel<NT, R, DUAL, G32, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    NIB_CUDA(set);
+    NIB_CUDA((allow_smem_once<gemm_int4_kernel<NT, R, DUAL, G32, F16>>(bytes)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(WARPS * 32);

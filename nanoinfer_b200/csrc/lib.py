@@ -890,7 +890,7 @@ class Kernels:
                 qkv.data_ptr(), out.data_ptr(), ctx.ctx_lens.data_ptr(), block_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                 k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, q_stride, bt_stride, bt_width, page_size, pages, n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 1 if earlier_complete else 0, scale, 0)
             self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
-        if n_dec == n_req:
+        if n_dec == m:          # (all rows: a request may bring none)
             return
         # The other requests' pages are read back once, in the order of their positions, and the prompt kernels run on them: a portion
         # reads its keys once for each of its row tiles, and what the tensor cores multiply is 16 bits wide either way.

@@ -227,3 +227,20 @@ def test_refusals(ops):
     for bad in ((x, w, out), (x, w, half.float()), (x, w, half, None, "relu"), (x, w, half, (1.0, 2.0, 3.0), "gelu_tanh")):
         with pytest.raises(KernelError):
             ops.linear_swiglu(*bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [5, 70, 300])
+def test_rows_of_wider_tensors_in_every_mode(ops, m, dtype):
+    """Rows of activations and results that begin on and off 16 bytes, at strides that are and are not a multiple of them."""
+    w, w64 = matrix(96, 128, 64, 21, narrow=True)
+    for width, lead in ((160, 8), (161, 3), (160, 1)):
+        x = rows(m, width, dtype, 22).cuda()[:, lead:lead + 128]
+        want = x.cpu().double() @ w64.T
+        bound = bounds(x.cpu(), w64, False) + 2.0 ** -23 * (want.abs() + 1)
+        for mode in ("store", "f32", "add"):
+            out = torch.full((m, 101), 0.5, dtype=dtype if mode == "store" else torch.float32, device="cuda")
+            ops.linear(x, w, None, out[:, 3:99], mode)
+            extra = 2.0 ** -8 * want.abs() if mode == "store" and dtype == torch.bfloat16 else 0.0
+            assert ((out[:, 3:99].cpu().double() - want - (0.5 if mode == "add" else 0.0)).abs() <= bound + extra).all(), (width, lead, mode)
+            assert (out[:, :3] == 0.5).all() and (out[:, 99:] == 0.5).all()

@@ -482,3 +482,27 @@ def test_refusals(ops):
         ops.unpack_int8(b.pools[0], b.pool_scales[0], torch.empty(b.pools[0].shape, dtype=torch.float16, device="cuda"))
     with pytest.raises(KernelError):
         ops.unpack_int8(b.pools[0], b.pool_scales[0], torch.empty(2, 2, dtype=torch.float32, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("q_lens,before", [([0, 2], [7, 15]), ([2, 0], [31, 5]), ([1, 0], [40, 9]), ([0, 1, 0, 1, 3], [3, 16, 0, 33, 14]),
+                                           ([0, 70, 0, 5], [1, 11, 130, 60])])
+def test_requests_that_bring_no_token(ops, q_lens, before, dtype):
+    """Their pages stay as they are, and the other requests' rows are theirs."""
+    b = Batch(4, 2, 64, 64, 16, q_lens, before, dtype, seed=90)
+    codes, scales = [c.clone() for c in b.codes], [s.clone() for s in b.scales]
+    tables, at, turned = b.table.cpu().tolist(), 0, []
+    for i, (n, p) in enumerate(zip(q_lens, before)):
+        rows = b.rows[at:at + n]
+        at += n
+        for t in range(n):
+            turned.append(ref.rotate(rows[t, :b.heads + b.kv], p + t, b.rotary))
+        if n:
+            ref.append(codes[0], scales[0], torch.stack(turned[-n:])[:, b.heads:], p, tables[i], b.page)
+            ref.append(codes[1], scales[1], rows[:, b.heads + b.kv:].double(), p, tables[i], b.page)
+    q = b.append(ops)
+    assert torch.isfinite(q).all()
+    for got, want in zip(b.pools + b.pool_scales, codes + scales):
+        assert torch.equal(got.cpu().double(), want)
+    b.qkv, b.rows = q, q.reshape(-1, b.heads, b.d).cpu()
+    check_attention(ops, b)
