@@ -560,7 +560,7 @@ class Kernels:
             if not self.weights_ahead:
                 self._lib.nib_pdl_skip_next()
             alpha, limit, shift = (0.0, 0.0, 0.0) if glu is None else glu
-            # Activations prepared as 16-bit floats: 11 instructions of every tile's 65 for a kernel of two microseconds before, which pays
+            # Activations prepared as 16-bit floats: 11 instructions of every tile's 65 for a kernel before (3.5 us by itself at 8 tokens of 3,584), which pays
             # where a product takes twenty (7B widths, us with / without: gate/up at 8 tokens 18.8 / 23.1, at 16 24.4 / 26.4, at 32 45.8 /
             # 42.5; down at 8 23.0 / 20.7).
             scratch = self._lib.nib_gemm_int4_scratch(m, k) if m <= 16 and w.packed.numel() >= 48 << 20 else 0
