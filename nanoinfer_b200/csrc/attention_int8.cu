@@ -14,6 +14,9 @@
 // head) among the CTAs of a cluster, which merge their partial (max, sum, output) through distributed shared memory and store the row.
 // Many, or long ones: the chunks of all rows, in order, in equal shares to as many CTAs as find room at a time, whatever the lengths
 // are; a row that lies within one CTA's share is stored, the others' parts are merged in order by a second kernel.
+//
+// A kernel of a chain is on its SM before the kernel ahead of it has ended, so what that one writes (queries, codes, scales, parts) is read
+// behind the wait and by loads that know of other writers (no __ldg, no const __restrict__); lengths and tables are the step's inputs.
 #include "attention_common.cuh"
 #include "pipeline.cuh"
 #include <cuda_fp16.h>
@@ -327,7 +330,7 @@ __device__ __forceinline__ void store_row4(__nv_bfloat16* out, const float4& acc
 // WHOLE: pages of a multiple of 16 tokens, so that 16 keys lie in one.
 template <int HD, int NH, bool WHOLE>
 __global__ void __launch_bounds__(WARPS * 32, NH == 1 ? 4 : 2)
-attention_int8_mma_kernel(const __nv_bfloat16* __restrict__ q_rows, __nv_bfloat16* __restrict__ out, const Args a) {
+attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict__ out, const Args a) {
     using C = Mma<HD, NH>;
     constexpr int KU = C::KU, STEP = C::STEP, MS = C::MS, ROWS = C::ROWS, H = WHOLE ? 1 : 2, IDS = KU * H, ID_KEYS = 16 / H;
     constexpr int V_AT = STEP * HD, S_AT = 2 * STEP * HD;
@@ -677,7 +680,7 @@ constexpr int GT = 32, GEN_THREADS = 128;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(GEN_THREADS)
-attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, const Args a) {
+attention_int8_any_kernel(const T* q_rows, T* __restrict__ out, const Args a) {
     extern __shared__ __align__(16) float smem[];
     const int hd = a.head_dim, n_rep = a.n_rep, tid = threadIdx.x;
     const int ks_stride = VEC ? hd + 4 : hd | 1;        // (a warp's threads read 32 rows at the same column)
@@ -710,8 +713,8 @@ attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, con
             const int page = key >= lo && key <= p ? page_at(a, bt, key, slot) : -1;
             const size_t block = (size_t)max(page, 0) * a.kv_heads + kvh;
             from[tid] = page >= 0 ? (long long)((block * a.page_size + slot) * hd) : -1;
-            ks[tid] = page >= 0 ? __ldg(a.k_scales + block) : 0.f;
-            vs[tid] = page >= 0 ? __ldg(a.v_scales + block) : 0.f;
+            ks[tid] = page >= 0 ? __ldcg(a.k_scales + block) : 0.f;
+            vs[tid] = page >= 0 ? __ldcg(a.v_scales + block) : 0.f;
         }
         __syncthreads();
         if (VEC) {
@@ -720,7 +723,7 @@ attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, con
                 const int row = i / chunks, d = (i - row * chunks) * 16;
                 const long long at = from[row];
                 uint4 k = make_uint4(0, 0, 0, 0), v = k;
-                if (at >= 0) { k = __ldg(reinterpret_cast<const uint4*>(a.k_pages + at + d)); v = __ldg(reinterpret_cast<const uint4*>(a.v_pages + at + d)); }
+                if (at >= 0) { k = __ldcg(reinterpret_cast<const uint4*>(a.k_pages + at + d)); v = __ldcg(reinterpret_cast<const uint4*>(a.v_pages + at + d)); }
                 const unsigned kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
                 const float s = ks[row];
 #pragma unroll
@@ -736,8 +739,8 @@ attention_int8_any_kernel(const T* __restrict__ q_rows, T* __restrict__ out, con
             for (int i = tid; i < GT * hd; i += GEN_THREADS) {
                 const int row = i / hd, d = i - row * hd;
                 const long long at = from[row];
-                kt[row * ks_stride + d] = at >= 0 ? (float)__ldg(a.k_pages + at + d) * ks[row] : 0.f;
-                vt[i] = at >= 0 ? (float)__ldg(a.v_pages + at + d) : 0.f;
+                kt[row * ks_stride + d] = at >= 0 ? (float)a.k_pages[at + d] * ks[row] : 0.f;
+                vt[i] = at >= 0 ? (float)a.v_pages[at + d] : 0.f;
             }
         }
         __syncthreads();

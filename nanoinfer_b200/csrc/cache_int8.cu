@@ -412,14 +412,14 @@ template <> __device__ __forceinline__ void store16<__nv_bfloat16>(__nv_bfloat16
 // out = codes * scale, block by block. Wide: the block's bytes are a multiple of 16.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
-unpack_int8_kernel(const signed char* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out, long long items, int per_block) {
+unpack_int8_kernel(const signed char* codes, const float* scales, T* __restrict__ out, long long items, int per_block) {      // (pools are kernels' results)
     pdl_launch_dependents();
     pdl_wait();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= items) return;
-    const float s = __ldg(scales + i / per_block);
+    const float s = __ldcg(scales + i / per_block);
     if (WIDE) {
-        store16<T>(out + i * 16, reinterpret_cast<const uint4*>(codes)[i], s);
+        store16<T>(out + i * 16, __ldcg(reinterpret_cast<const uint4*>(codes) + i), s);
     } else {
         Elem<T>::store(out + i, (float)codes[i] * s);
     }
@@ -434,10 +434,10 @@ constexpr int GATHER = 64;
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(128)
-gather_int8_kernel(const signed char* __restrict__ k_pages, const signed char* __restrict__ v_pages, const float* __restrict__ k_scales,
-                   const float* __restrict__ v_scales, T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table_out,
-                   const int* __restrict__ q_start, const int* __restrict__ ctx_lens, const int* __restrict__ block_table, int bt_stride,
-                   int bt_width, int page_size, int num_pages, int kv_heads, int head_dim, int width, int window) {
+gather_int8_kernel(const signed char* k_pages, const signed char* v_pages, const float* k_scales, const float* v_scales,
+                   T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table_out, const int* __restrict__ q_start, const int* __restrict__ ctx_lens,
+                   const int* __restrict__ block_table, int bt_stride, int bt_width, int page_size, int num_pages, int kv_heads, int head_dim,
+                   int width, int window) {
     pdl_wait();
     pdl_launch_dependents();
     const int i = blockIdx.x, kvh = blockIdx.y, r = blockIdx.z;
@@ -457,11 +457,11 @@ gather_int8_kernel(const signed char* __restrict__ k_pages, const signed char* _
         if (page >= num_pages) page = -1;
         const size_t block = (size_t)max(page, 0) * kv_heads + kvh;
         const size_t from = (block * page_size + (pos - lp * page_size)) * head_dim + d, dst = to + (size_t)row * head_dim + d;
-        float ks = page >= 0 ? __ldg(k_scales + block) : 0.f, vs = page >= 0 ? __ldg(v_scales + block) : 0.f;
+        float ks = page >= 0 ? __ldcg(k_scales + block) : 0.f, vs = page >= 0 ? __ldcg(v_scales + block) : 0.f;
         if (ks != ks || vs != vs) { ks = NAN; vs = 0.f; }
         if (WIDE) {
             uint4 k = make_uint4(0, 0, 0, 0), v = k;         // slots that nobody sees are finite
-            if (page >= 0) { k = *reinterpret_cast<const uint4*>(k_pages + from); v = *reinterpret_cast<const uint4*>(v_pages + from); }
+            if (page >= 0) { k = __ldcg(reinterpret_cast<const uint4*>(k_pages + from)); v = __ldcg(reinterpret_cast<const uint4*>(v_pages + from)); }
             store16<T>(k_out + dst, k, ks);
             store16<T>(v_out + dst, v, vs);
         } else {

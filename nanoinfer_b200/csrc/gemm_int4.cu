@@ -90,7 +90,7 @@ struct Args {
 // The activations of F16: a CTA a token. x16 [tokens][k] = x * 2^e, sums as Args has them, factors = 2^24 / 2^e. step: 64 or 32.
 constexpr int PREP_THREADS = 512;
 __global__ void __launch_bounds__(PREP_THREADS)
-prepare_f16_kernel(const __nv_bfloat16* __restrict__ x, int ldx, __half* __restrict__ x16, float* __restrict__ sums, float* __restrict__ factors, int k, int step) {
+prepare_f16_kernel(const __nv_bfloat16* x, int ldx, __half* __restrict__ x16, float* __restrict__ sums, float* __restrict__ factors, int k, int step) {
     __shared__ unsigned s_top[PREP_THREADS / 32];
     const int token = blockIdx.x, lane = threadIdx.x & 31;
     const uint4* row = reinterpret_cast<const uint4*>(x + (size_t)token * ldx);
@@ -291,7 +291,7 @@ gemm_int4_kernel(const Args a) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int tok = n * 8 + 2 * t + j;
-                const float f = tok < a.tokens ? __ldg(a.factors + tok) : 0.f;
+                const float f = tok < a.tokens ? __ldcg(a.factors + tok) : 0.f;        // (the kernel before this one writes them)
 #pragma unroll
                 for (int r = 0; r < R; ++r) { v[r][j] *= f; v[r][2 + j] *= f * 0.0625f; }
             }
