@@ -506,3 +506,34 @@ def test_requests_that_bring_no_token(ops, q_lens, before, dtype):
         assert torch.equal(got.cpu().double(), want)
     b.qkv, b.rows = q, q.reshape(-1, b.heads, b.d).cpu()
     check_attention(ops, b)
+
+
+@pytest.mark.parametrize("q_lens,before", [([300], [50]), ([1, 1, 90], [700, 33, 0]), ([1, 1], [515, 90])])
+def test_rows_that_the_kernel_before_makes(ops, q_lens, before):
+    """Product, append and attention launched one behind the other, many times over the same buffers with other inputs each time: what each
+    leaves is what it leaves when every kernel before it has ended."""
+    heads, kv, d, hidden = 14, 2, 64, 896
+    b = Batch(heads, kv, d, d, 16, q_lens, before, torch.bfloat16, seed=100)
+    m = sum(q_lens)
+    g = torch.Generator().manual_seed(101)
+    w = (torch.randn((heads + 2 * kv) * d, hidden, generator=g) * hidden ** -0.5).to(torch.bfloat16).cuda()
+    inputs = [(torch.randn(m, hidden, generator=g) * 2.0 ** i).to(torch.bfloat16).cuda() for i in range(4)]
+    start = [t.clone() for t in b.pools + b.pool_scales]
+    q, out = (torch.empty(m, heads * d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+
+    def run(x, wait):
+        for step in (lambda: ops.linear(x, w, None, b.qkv, "store"), lambda: b.append(ops, q_out=q),
+                     lambda: ops.attention_int8(q, out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, 16, *b.pools, *b.pool_scales)):
+            step()
+            if wait:
+                torch.cuda.synchronize()
+        return out.clone(), [t.clone() for t in b.pools + b.pool_scales]
+
+    def runs(wait):
+        for t, s in zip(b.pools + b.pool_scales, start):
+            t.copy_(s)
+        torch.cuda.synchronize()
+        return [run(inputs[i % 4], wait) for i in range(20)]
+
+    for (row, pools), (want, want_pools) in zip(runs(False), runs(True)):
+        assert torch.equal(row, want) and all(torch.equal(x, y) for x, y in zip(pools, want_pools))

@@ -44,3 +44,12 @@ def test_results_of_other_kernels_are_read_coherently():
                 assert source in allowed, (name, kernel, source)
     assert {"attention_int8_mma_kernel", "attention_int8_any_kernel", "merge_int8_kernel", "append_int8_kernel", "unpack_int8_kernel", "gather_int8_kernel",
             "prepare_f16_kernel", "gemm_int4_kernel", "unpack_int4_kernel"} <= seen
+
+
+def test_every_kernel_waits_before_it_reads_rows_and_pools_and_before_it_writes():
+    """What a kernel behind the wait of the one before it sees is not what the kernels before both have written unless it waits itself."""
+    (append,) = [body for name, _, body in kernels(code("cache_int8.cu")) if name == "append_int8_kernel"]
+    before, _, behind = append.partition("\n    pdl_wait();\n")         # (the CTAs of keys and values: a statement of its own, under no condition)
+    assert behind, "no unconditional wait"
+    for touched in ("k_codes", "v_codes", "k_rows", "v_rows", "k_scales", "v_scales"):
+        assert touched not in before and touched in behind, touched
