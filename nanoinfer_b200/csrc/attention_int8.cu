@@ -20,6 +20,7 @@
 #include "attention_common.cuh"
 #include "pipeline.cuh"
 #include <cuda_fp16.h>
+#include <type_traits>
 
 using namespace nibp;
 
@@ -352,7 +353,7 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
     };
     const long long page_bytes = (long long)a.kv_heads * a.page_size * HD;
     // A page that the request does not hold is read as the pool's first with scales of 0: nothing leaves the pool.
-    auto send = [&](int chunk, int stage) {
+    auto send = [&](int chunk, int stage, auto with_scales, auto with_codes) {
         const unsigned dst = ring + stage * C::STAGE;
         const int from = (chunk - piece.begin) & 31;
         const signed char* k_lane = a.k_pages + (size_t)piece.kvh * a.page_size * HD + g * HD + t * 16;
@@ -362,12 +363,13 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
             const int key = chunk * C::CHUNK + warp * STEP + i * ID_KEYS;
             const int page = __shfl_sync(0xffffffffu, ids[i], from);
             const bool held = page >= 0;
-            const int slot = !held ? 0 : a.shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
-            const long long at = max(page, 0) * page_bytes + slot * HD;
-            if (lane < 2) {
+            if (with_scales && lane < 2) {
                 const size_t block = (size_t)max(page, 0) * a.kv_heads + piece.kvh;
                 copy_async_or_zero(dst + S_AT + i * 8 + lane * 4, (lane ? a.v_scales : a.k_scales) + block, held);
             }
+            if (!with_codes) continue;
+            const int slot = !held ? 0 : a.shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
+            const long long at = max(page, 0) * page_bytes + slot * HD;
 #pragma unroll
             for (int h = 0; h < 2 / H; ++h) {
                 const int part = i * (2 / H) + h;               // 8 keys
@@ -379,15 +381,18 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
             }
         }
     };
+    const auto yes = std::true_type{};
+    const auto no = std::false_type{};
     bool more = piece.first(a, lane);
     if (more) look_up(piece.begin);         // lengths and tables are the step's inputs; queries, keys, values and scales are kernels' results
-    // Where the caller says so, pages before the one that the token's own key goes to are sent for before the wait.
+    // Where the caller says so, the codes of pages before the one that the token's own key goes to are sent for before the wait. Not their
+    // scales: one of another page, which the kernel before this one may be writing, can lie in the same 32 bytes, and a copy of 4 bytes
+    // leaves those in the SM's first cache. (Codes of 8 bytes go through it too: pools that begin on 128 bytes have pages of whole lines.)
     int sent = 0;
     if (a.early && more) {
         const int own_page = piece.p >= 0 ? piece.p - piece.p % a.page_size : 0;
         while (sent < STAGES - 1 && piece.begin + sent < piece.end && (piece.begin + sent + 1) * C::CHUNK <= own_page) {
-            send(piece.begin + sent, sent);
-            asm volatile("cp.async.commit_group;\n" ::: "memory");
+            send(piece.begin + sent, sent, no, yes);
             ++sent;
         }
     }
@@ -408,8 +413,9 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
                 for (int j = 0; j < 2; ++j)
                     raw[kk][nh][j] = head < a.n_rep ? *reinterpret_cast<const unsigned*>(qp + (kk >> 2) * 64 + (kk & 3) * 4 + 2 * j) : 0u;
         }
-        for (int i = sent; i < STAGES - 1; ++i) {
-            if (piece.begin + i < piece.end) send(piece.begin + i, i);
+        for (int i = 0; i < STAGES - 1; ++i) {
+            if (i < sent) send(piece.begin + i, i, yes, no);
+            else if (piece.begin + i < piece.end) send(piece.begin + i, i, yes, yes);
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
         sent = 0;
@@ -463,7 +469,7 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
 #pragma unroll 1
         for (int chunk = piece.begin; chunk < piece.end; ++chunk) {
             if (((chunk + STAGES - 1 - piece.begin) & 31) == 0) look_up(chunk + STAGES - 1);
-            if (chunk + STAGES - 1 < piece.end) send(chunk + STAGES - 1, ahead);
+            if (chunk + STAGES - 1 < piece.end) send(chunk + STAGES - 1, ahead, yes, yes);
             asm volatile("cp.async.commit_group;\ncp.async.wait_group %0;\n" ::"n"(STAGES - 1) : "memory");
             __syncwarp();                           // (the scales are two lanes' copies)
             const unsigned src = ring + stage * C::STAGE;
@@ -860,7 +866,8 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     int shift = -1;
     if ((page_size & (page_size - 1)) == 0) for (shift = 0; (1 << shift) < page_size;) ++shift;
     const Args a{c.ctx_lens, c.block_table, (const signed char*)c.k_pages, (const signed char*)c.v_pages, c.k_scales, c.v_scales, c.part_o, c.part_ml,
-                 c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, n_tokens, heads, kv_heads, heads / kv_heads, head_dim, c.window, c.ctas, c.shares, c.early, c.scale};
+                 c.q_stride, c.bt_stride, c.bt_width, page_size, shift, c.num_pages, n_tokens, heads, kv_heads, heads / kv_heads, head_dim, c.window, c.ctas, c.shares,
+                 c.early && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 127) == 0, c.scale};
     int rc;
     // (rows and pools that lie off the pieces that a thread reads and writes at a time go to the general kernel)
     if (kind == 1 && ((uintptr_t)q & 3) == 0 && c.q_stride % 2 == 0 && ((uintptr_t)out & 7) == 0 && (((uintptr_t)c.k_pages | (uintptr_t)c.v_pages) & 15) == 0) {

@@ -537,3 +537,71 @@ def test_rows_that_the_kernel_before_makes(ops, q_lens, before):
 
     for (row, pools), (want, want_pools) in zip(runs(False), runs(True)):
         assert torch.equal(row, want) and all(torch.equal(x, y) for x, y in zip(pools, want_pools))
+
+
+@pytest.mark.parametrize("heads,kv,d,page", [(14, 2, 64, 16), (14, 2, 64, 8), (16, 4, 64, 64), (28, 4, 128, 16), (12, 2, 128, 8), (24, 2, 128, 32)])
+def test_pages_that_are_sent_for_ahead_of_the_wait(ops, heads, kv, d, page):
+    """Decoding as an engine does it: a copy of the step's lengths, the product that makes the rows, append, attention with the promise that
+    earlier pages are complete. The requests' pages follow one another, so that scales of earlier pages lie beside the one that
+    the append writes, and every token is larger than the one before: its page's scale grows. The rows are those without the
+    promise, bit for bit, launched and replayed, and those of 64 bits."""
+    before, steps, hidden = [130, 255, 64, 1041, 5000, 3], 6, 256
+    n = len(before)
+    total = [p + steps for p in before]
+    pages = sum(-(-t // page) for t in total) + 1
+    b = Batch(heads, kv, d, d, page, [1] * n, total, torch.bfloat16, seed=110, pages=sum(-(-(t + 1) // page) for t in total) + 2)
+    table, at = torch.full_like(b.table, -1), 0
+    for i, t in enumerate(total):
+        held = -(-t // page)
+        table[i, :held] = torch.arange(at, at + held, dtype=torch.int32, device="cuda")
+        at += held
+    assert at < pages
+    b.table = table
+    g = torch.Generator().manual_seed(111)
+    w = (torch.randn((heads + 2 * kv) * d, hidden, generator=g) * hidden ** -0.5).to(torch.bfloat16).cuda()
+    x = [(torch.randn(n, hidden, generator=g) * 1.5 ** t).to(torch.bfloat16).cuda() for t in range(steps)]
+    lens = [torch.tensor([p + t + 1 for p in before], dtype=torch.int32, device="cuda") for t in range(steps)]
+    start = [t.clone() for t in b.pools + b.pool_scales]
+    feed = torch.empty_like(x[0])
+    rows, q, out = b.qkv, *(torch.empty(n, heads * d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+
+    def step(ops, early):
+        ops.linear(feed, w, None, rows, "store")
+        b.append(ops, q_out=q)
+        ops.attention_int8(q, out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, page, *b.pools, *b.pool_scales, earlier_complete=early)
+
+    def decode(one_step):
+        for t, s in zip(b.pools + b.pool_scales, start):
+            t.copy_(s)
+        got = []
+        for t in range(steps):
+            feed.copy_(x[t])
+            b.ctx.positions.copy_(lens[t] - 1)
+            b.ctx.ctx_lens.copy_(lens[t])
+            one_step()
+            got.append(out.clone())
+        return got
+
+    for splits in (0, 1, 4, 8, 40):
+        k = ops.with_options(fixed_decode_splits=splits)
+        want = decode(lambda: step(k, False))
+        grown = [(t != s).sum().item() for t, s in zip(b.pool_scales, start[2:])]
+        assert min(grown) > 0
+        for i in range(3):
+            assert all(torch.equal(a, c) for a, c in zip(decode(lambda: step(k, True)), want)), (splits, i)
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.capture_begin()
+            step(k, True)
+            graph.capture_end()
+        torch.cuda.current_stream().wait_stream(side)
+        for i in range(3):
+            assert all(torch.equal(a, c) for a, c in zip(decode(graph.replay), want)), (splits, i)
+    # the last step's rows
+    keys, vals = (ref.values(c.cpu(), s.cpu()) for c, s in zip(b.pools, b.pool_scales))
+    tables, q64 = b.table.cpu().tolist(), q.cpu().reshape(n, heads, d)
+    for i, p in enumerate(total):
+        want, size, small = ref.attend(q64[i], keys, vals, b.pool_scales[1].cpu(), tables[i], page, p - 1, d ** -0.5, 0, kv)
+        bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size + 2.0 ** -25 * small
+        assert ((out[i].cpu().double().reshape(heads, d) - want).abs() <= bound).all(), i

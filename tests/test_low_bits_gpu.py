@@ -164,3 +164,35 @@ def test_both_together_through_generation_and_the_scheduler(model_dirs):
     model.engine.cache.check()
     breakdown = model.weight_breakdown()
     assert breakdown["int4"][0] == 8 and model.engine.storage.bytes_per_token() == 2 * (2 * 2 * 64 + 1)
+
+
+@pytest.mark.parametrize("weights", [None, 64])
+def test_decoding_behind_prompts_of_hundreds_of_tokens(model_dirs, tmp_path, weights):
+    """Contexts of several chunks of the decode kernel, whose earlier pages are sent for while the append still runs: logits of replayed and
+    of eager steps against the plain model with the same codes, with weights of 16 bits and of 4. Replayed and eager are equal where both cut
+    the keys alike: by themselves they choose 8 CTAs a row for the 1,024 keys that a graph is captured for and 4 for 534, whose sums of
+    32 bits are of other terms. So the number is fixed."""
+    from nanoinfer_b200.config import KernelOptions
+    from nanoinfer_b200.engine import StepEntry
+    d, page = model_dirs["C"]
+    kw = {}
+    if weights:
+        dequantized(d, str(tmp_path / "q"), weights)
+        kw = dict(weight_format="int4", weight_group=weights)
+    model = plain.PlainModel(str(tmp_path / "q") if weights else d)
+    prompts = [tokens(n, model.cfg["vocab"], n) for n in (301, 140, 522)]
+    more, steps = tokens(36, model.cfg["vocab"], 10), 12
+    want = [plain_rows(model, p + more[r::3], [len(p)] + [1] * steps, page)[len(p) - 1:] for r, p in enumerate(prompts)]
+    runs = []
+    for graphs in (True, False):
+        eng = engine(d, page, "bfloat16", num_pages=300, cache_dtype="int8", cuda_graphs=graphs, kernel_options=KernelOptions(fixed_decode_splits=4), **kw)
+        rcs = [eng.open(i) for i in range(3)]
+        rows = [eng.step([StepEntry(rc, p, [len(p) - 1]) for rc, p in zip(rcs, prompts)]).clone()]
+        for t in range(steps):
+            rows.append(eng.step([StepEntry(rc, [more[3 * t + r]], [0]) for r, rc in enumerate(rcs)]).clone())
+        runs.append(torch.stack(rows))
+        assert eng.graph_launches > 0 if graphs else eng.graph_launches == 0
+        eng.check_device()
+    assert torch.equal(runs[0], runs[1])
+    for r in range(3):
+        assert_close(runs[0][:, r], want[r], torch.bfloat16, f"request {r}")

@@ -53,3 +53,11 @@ def test_every_kernel_waits_before_it_reads_rows_and_pools_and_before_it_writes(
     assert behind, "no unconditional wait"
     for touched in ("k_codes", "v_codes", "k_rows", "v_rows", "k_scales", "v_scales"):
         assert touched not in before and touched in behind, touched
+
+
+def test_no_scale_is_sent_for_ahead_of_the_wait():
+    """Scales of several pages share 32 bytes: one that is fetched early would bring in the one that the append before is writing."""
+    (body,) = [body for name, _, body in kernels(code("attention_int8.cu")) if name == "attention_int8_mma_kernel"]
+    early = body[body.index("a.early"):body.index("pdl_wait();")]
+    assert re.findall(r"\bsend\(([^;]*)\);", early) == ["piece.begin + sent, sent, no, yes"]
+    assert re.search(r"auto send = \[&\]\(int chunk, int stage, auto with_scales, auto with_codes\)", body)
