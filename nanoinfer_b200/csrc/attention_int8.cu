@@ -353,7 +353,13 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
     };
     const long long page_bytes = (long long)a.kv_heads * a.page_size * HD;
     // A page that the request does not hold is read as the pool's first with scales of 0: nothing leaves the pool.
-    auto send = [&](int chunk, int stage, auto with_scales, auto with_codes) {
+    auto send_scales = [&](int stage, int i, int page) {
+        if (lane < 2) {
+            const size_t block = (size_t)max(page, 0) * a.kv_heads + piece.kvh;
+            copy_async_or_zero(ring + stage * C::STAGE + S_AT + i * 8 + lane * 4, (lane ? a.v_scales : a.k_scales) + block, page >= 0);
+        }
+    };
+    auto send = [&](int chunk, int stage, auto with_scales) {
         const unsigned dst = ring + stage * C::STAGE;
         const int from = (chunk - piece.begin) & 31;
         const signed char* k_lane = a.k_pages + (size_t)piece.kvh * a.page_size * HD + g * HD + t * 16;
@@ -363,13 +369,9 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
             const int key = chunk * C::CHUNK + warp * STEP + i * ID_KEYS;
             const int page = __shfl_sync(0xffffffffu, ids[i], from);
             const bool held = page >= 0;
-            if (with_scales && lane < 2) {
-                const size_t block = (size_t)max(page, 0) * a.kv_heads + piece.kvh;
-                copy_async_or_zero(dst + S_AT + i * 8 + lane * 4, (lane ? a.v_scales : a.k_scales) + block, held);
-            }
-            if (!with_codes) continue;
             const int slot = !held ? 0 : a.shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
             const long long at = max(page, 0) * page_bytes + slot * HD;
+            if (with_scales) send_scales(stage, i, page);
 #pragma unroll
             for (int h = 0; h < 2 / H; ++h) {
                 const int part = i * (2 / H) + h;               // 8 keys
@@ -381,8 +383,6 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
             }
         }
     };
-    const auto yes = std::true_type{};
-    const auto no = std::false_type{};
     bool more = piece.first(a, lane);
     if (more) look_up(piece.begin);         // lengths and tables are the step's inputs; queries, keys, values and scales are kernels' results
     // Where the caller says so, the codes of pages before the one that the token's own key goes to are sent for before the wait. Not their
@@ -392,7 +392,7 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
     if (a.early && more) {
         const int own_page = piece.p >= 0 ? piece.p - piece.p % a.page_size : 0;
         while (sent < STAGES - 1 && piece.begin + sent < piece.end && (piece.begin + sent + 1) * C::CHUNK <= own_page) {
-            send(piece.begin + sent, sent, no, yes);
+            send(piece.begin + sent, sent, std::false_type{});
             ++sent;
         }
     }
@@ -413,9 +413,14 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
                 for (int j = 0; j < 2; ++j)
                     raw[kk][nh][j] = head < a.n_rep ? *reinterpret_cast<const unsigned*>(qp + (kk >> 2) * 64 + (kk & 3) * 4 + 2 * j) : 0u;
         }
-        for (int i = 0; i < STAGES - 1; ++i) {
-            if (i < sent) send(piece.begin + i, i, yes, no);
-            else if (piece.begin + i < piece.end) send(piece.begin + i, i, yes, yes);
+#pragma unroll 1
+        for (int i = 0; i < sent; ++i) {
+#pragma unroll
+            for (int j = 0; j < IDS; ++j) send_scales(i, j, __shfl_sync(0xffffffffu, ids[j], i));
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
+        for (int i = sent; i < STAGES - 1; ++i) {
+            if (piece.begin + i < piece.end) send(piece.begin + i, i, std::true_type{});
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         }
         sent = 0;
@@ -469,7 +474,7 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
 #pragma unroll 1
         for (int chunk = piece.begin; chunk < piece.end; ++chunk) {
             if (((chunk + STAGES - 1 - piece.begin) & 31) == 0) look_up(chunk + STAGES - 1);
-            if (chunk + STAGES - 1 < piece.end) send(chunk + STAGES - 1, ahead, yes, yes);
+            if (chunk + STAGES - 1 < piece.end) send(chunk + STAGES - 1, ahead, std::true_type{});
             asm volatile("cp.async.commit_group;\ncp.async.wait_group %0;\n" ::"n"(STAGES - 1) : "memory");
             __syncwarp();                           // (the scales are two lanes' copies)
             const unsigned src = ring + stage * C::STAGE;

@@ -59,5 +59,6 @@ def test_no_scale_is_sent_for_ahead_of_the_wait():
     """Scales of several pages share 32 bytes: one that is fetched early would bring in the one that the append before is writing."""
     (body,) = [body for name, _, body in kernels(code("attention_int8.cu")) if name == "attention_int8_mma_kernel"]
     early = body[body.index("a.early"):body.index("pdl_wait();")]
-    assert re.findall(r"\bsend\(([^;]*)\);", early) == ["piece.begin + sent, sent, no, yes"]
-    assert re.search(r"auto send = \[&\]\(int chunk, int stage, auto with_scales, auto with_codes\)", body)
+    calls = re.findall(r"\bsend\w*\([^;]*;", early)
+    assert calls and all(c.startswith("send(") and c.endswith("std::false_type{});") for c in calls)        # (the codes alone)
+    assert re.search(r"auto send = \[&\]\(int chunk, int stage, auto with_scales\)", body)
