@@ -4,10 +4,13 @@
 //
 // The key scale multiplies a score. The value scale would multiply a row of V before a tensor core sums it; it goes into the
 // softmax instead: with t_j = s_j log2(e) + log2(sv_j) and a running reference M of max t,
-//     w_j = 2^(s_j log2(e) - M + 20),  p_j = w_j sv_j 2^-20  (about 1 at most),  l = sum_j w_j,  o = 2^20 sum_j p_j cv_j / l,
+//     w_j = 2^(s_j log2(e) - M + 20),  p_j = w_j sv_j 2^-11  (about 2^9 at most),  l = sum_j w_j,  o = 2^11 sum_j p_j cv_j / l,
 // so the tensor core multiplies p_j, in 16 bits, with whole numbers that 16 bits hold exactly, and a row is right to its own
 // size however much the scales of its blocks differ. l and o are summed in 32 bits; with scales of 2^-80 .. 2^121 the terms of l that
-// count lie between 2^-125 and 2^106 (the 20 is what centres them).
+// count lie between 2^-125 and 2^106 (the 20 is what centres them). The tensor core's p_j is rounded to 11 bits, as the 16-bit caches' weights
+// are to 8; the reference may lag by 2^6, and 2^15 is what a 16-bit float holds: the 2^9 is the room that is left, so that a weight 2^-23
+// of the reference still has its 11 bits and one down to 2^-34 counts (with p_j of 1 at most it was 2^-25, and tens of thousands of
+// keys below that were in l and not in o).
 //
 // Two kernels. The one on the tensor cores takes heads of 64 and 128, at most 16 query heads a kv head and pages of a multiple of
 // 8 tokens; the general one takes any shape and 32-bit rows. The keys are dealt out in one of two ways. Few rows: those of a (token, kv
@@ -27,7 +30,7 @@ using namespace nibp;
 namespace {
 
 constexpr int WARPS = 4;
-constexpr float LIFT = 20.f, UNLIFT = 0x1p-20f, RELIFT = 0x1p20f;
+constexpr float LIFT = 20.f, UNLIFT = 0x1p-11f, RELIFT = 0x1p11f;
 
 struct Args {
     const int* ctx_lens; const int* block_table; const signed char* k_pages; const signed char* v_pages;
@@ -527,7 +530,7 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
                         s[ku][nh][e] = v;
                         top[e & 1] = fmaxf(top[e & 1], v + lv[id]);
                     }
-                // the reference moves only where a key is 2^6 above it: p stays far inside 16 bits meanwhile
+                // the reference moves only where a key is 2^6 above it: p is at most 2^15 meanwhile, within 16 bits
                 if (__any_sync(0xffffffffu, top[0] > m_ref[nh][0] + 6.f || top[1] > m_ref[nh][1] + 6.f)) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {

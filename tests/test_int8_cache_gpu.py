@@ -605,3 +605,39 @@ def test_pages_that_are_sent_for_ahead_of_the_wait(ops, heads, kv, d, page):
         want, size, small = ref.attend(q64[i], keys, vals, b.pool_scales[1].cpu(), tables[i], page, p - 1, d ** -0.5, 0, kv)
         bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size + 2.0 ** -25 * small
         assert ((out[i].cpu().double().reshape(heads, d) - want).abs() <= bound).all(), i
+
+
+@pytest.mark.parametrize("heads,kv,d", [(14, 2, 64), (6, 2, 128), (24, 2, 128)])
+@pytest.mark.parametrize("below", [(42, 75), (70, 78)])
+def test_one_sharp_key_before_tens_of_thousands_that_weigh_little(ops, heads, kv, d, below):
+    """Keys 15 to 27, and 25 to 28, octaves below the largest, whose values are all of a sign and are all that some dims of the row consist of. Their weights
+    are 16-bit numbers as the largest one's is, and the denominator holds them in 32 bits: what is lost of one is half a step of it (2^-11) or
+    2^-34 of the reference (2^-25, half of the smallest 16-bit number, which stands 2^9 above the row's reference); the row's rounding
+    to bfloat16 and 32-bit sums come on top."""
+    before = [40000, 9000, 700]
+    b = Batch(heads, kv, d, 0, 16, [1] * 3, before, torch.bfloat16, seed=120)
+    g = torch.Generator().manual_seed(121)
+    codes = [torch.zeros_like(c) for c in b.codes]
+    codes[0][..., 0] = torch.randint(100 - below[1], 101 - below[0], codes[0][..., 0].shape, generator=g).double()       # a quarter each
+    codes[1][:] = torch.randint(60, 128, codes[1].shape, generator=g).double()
+    for i, p in enumerate(before):
+        at = 5 + 37 * i
+        page, slot = int(b.table[i, at // 16]), at % 16
+        codes[0][page, :, slot, 0] = 100
+        codes[1][page, :, slot, ::2] = 0
+    for t, c in zip(b.pools, codes):
+        t.copy_(c)
+    b.pool_scales[0].fill_(0.25)
+    b.pool_scales[1].fill_(2.0 ** -3)
+    b.rows[:, :heads] = 0
+    b.rows[:, :heads, 0] = 1
+    b.qkv.copy_(b.rows.reshape(3, -1))
+    keys, vals = (ref.values(c, s.cpu()) for c, s in zip(codes, b.pool_scales))
+    tables = b.table.cpu().tolist()
+    want = [ref.attend(b.rows[i, :heads], keys, vals, b.pool_scales[1].cpu(), tables[i], 16, p, 1.0, 0, kv) for i, p in enumerate(before)]
+    for splits in (0, 1, 8, 40):
+        out = torch.empty(3, heads * d, dtype=torch.bfloat16, device="cuda")
+        ops.with_options(fixed_decode_splits=splits).attention_int8(b.qkv, out, heads, kv, d, 1.0, 0, b.ctx, b.table, 16, *b.pools, *b.pool_scales)
+        for i, (row, size, small) in enumerate(want):
+            err = (out[i].cpu().double().reshape(heads, d) - row).abs()
+            assert (err <= 2.0 ** -8 * row.abs() + (2.0 ** -11 + 2.0 ** -14) * size + 2.0 ** -34 * small).all(), (splits, i)
