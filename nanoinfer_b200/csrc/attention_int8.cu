@@ -555,7 +555,7 @@ attention_int8_mma_kernel(const __nv_bfloat16* q_rows, __nv_bfloat16* __restrict
                             const float w = exp2_ftz(s[ku][nh][2 * h + q] - m_use);
                             l_part[nh][q] += w;
                             float pv = w * vs[WHOLE ? ku : ku * 2 + h];
-                            if (edge && w == 0.f) pv = 0.f;             // (a hidden key's block may be undefined)
+                            if (edge && s[ku][nh][2 * h + q] == -INFINITY) pv = 0.f;        // (a hidden key's block may be undefined; a seen one's counts, however little it weighs)
                             s[ku][nh][2 * h + q] = pv;
                         }
                 }
@@ -786,7 +786,7 @@ attention_int8_any_kernel(const T* q_rows, T* __restrict__ out, const Args a) {
                 cta_ml[2 * h] = m_new;
                 cta_ml[2 * h + 1] = cta_ml[2 * h + 1] * f * f + sum;
             }
-            w[i] = e == 0.f ? 0.f : e * (vs[row] * UNLIFT);
+            w[i] = e * (vs[row] * UNLIFT);          // (of a hidden key both are 0)
         }
         __syncthreads();
         for (int i = tid; i < n_rep * hd; i += GEN_THREADS) {

@@ -641,3 +641,25 @@ def test_one_sharp_key_before_tens_of_thousands_that_weigh_little(ops, heads, kv
         for i, (row, size, small) in enumerate(want):
             err = (out[i].cpu().double().reshape(heads, d) - row).abs()
             assert (err <= 2.0 ** -8 * row.abs() + (2.0 ** -11 + 2.0 ** -14) * size + 2.0 ** -34 * small).all(), (splits, i)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,page", [(4, 2, 64, 16), (4, 2, 128, 8), (4, 2, 32, 16)])
+def test_an_undefined_block_is_undefined_however_little_it_weighs(ops, heads, kv, d, page, dtype):
+    """0 times an undefined value is undefined, in the middle of the keys and among the last ones alike; behind the last key, and before a
+    window, it is nobody's."""
+    for n, at in ((300, 1), (300, 290 // page), (41, 40 // page), (41, 0)):
+        b = Batch(heads, kv, d, 0, page, [1, 1], [n - 1, n - 1], dtype, seed=130)
+        b.rows[:, :heads] = 0
+        b.rows[:, :heads, 0] = 1
+        b.qkv.copy_(b.rows.reshape(2, -1))
+        for t in b.pools[0]:
+            t[..., 0] = 100
+        b.pool_scales[0].fill_(4.0)
+        bad = int(b.table[0, at])
+        b.pools[0][bad, :, :, 0] = -100             # 800 below the others: 2^-1154 of their weight
+        b.pool_scales[1][bad, 1] = float("nan")
+        out = torch.empty(2, heads * d, dtype=dtype, device="cuda")
+        ops.attention_int8(b.qkv, out, heads, kv, d, 1.0, 0, b.ctx, b.table, page, *b.pools, *b.pool_scales)
+        rows = out.reshape(2, kv, heads // kv, d)
+        assert torch.isnan(rows[0, 1]).all() and torch.isfinite(rows[0, 0]).all() and torch.isfinite(rows[1]).all(), (n, at)
