@@ -663,3 +663,22 @@ def test_an_undefined_block_is_undefined_however_little_it_weighs(ops, heads, kv
         ops.attention_int8(b.qkv, out, heads, kv, d, 1.0, 0, b.ctx, b.table, page, *b.pools, *b.pool_scales)
         rows = out.reshape(2, kv, heads // kv, d)
         assert torch.isnan(rows[0, 1]).all() and torch.isfinite(rows[0, 0]).all() and torch.isfinite(rows[1]).all(), (n, at)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv,d,page", [(4, 2, 64, 16), (12, 2, 128, 16), (4, 2, 32, 8)])
+def test_undefined_blocks_in_portions_are_their_tokens_alone(ops, heads, kv, d, page, dtype):
+    """A portion's tokens that see an undefined block are undefined; those before it, those whose window has left it, the other kv head's and
+    the other request's are what they are without it."""
+    for j in range(2):
+        for window in (0, 50):
+            b = Batch(heads, kv, d, 0, page, [150, 20], [40, 9], dtype, seed=140)
+            want = attention_rows(ops, b, window).reshape(-1, kv, heads // kv, d)
+            first = 4 * page                    # position of the block's first token
+            b.pool_scales[j][int(b.table[0, 4]), 1] = float("nan")
+            got = attention_rows(ops, b, window).reshape(-1, kv, heads // kv, d)
+            sees = torch.zeros(170, dtype=torch.bool)
+            for t in range(150):
+                lo = max(0, 40 + t - window + 1) if window else 0
+                sees[t] = 40 + t >= first and lo < first + page
+            assert torch.isnan(got[sees, 1]).all() and torch.equal(got[~sees], want[~sees]) and torch.equal(got[:, 0], want[:, 0]), (j, window)
