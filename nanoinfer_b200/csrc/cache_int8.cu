@@ -425,30 +425,61 @@ unpack_int8_kernel(const signed char* codes, const float* scales, T* __restrict_
     }
 }
 
-// A step's requests as pages of GATHER tokens in the order of their positions: page r * width + i of the result holds
-// positions i * GATHER .. of request r; the table says so (-1 where a request has no such page). Positions before ``lo`` of a
-// window are not read by any of the request's tokens and stay unwritten where a whole result page lies before it. A block with
-// an undefined scale becomes undefined keys and values of zero: a score is left out by choosing, not by multiplying with nothing,
-// so that a token that does not see the block is not made undefined by it.
+// A step's requests as pages of GATHER tokens in the order of their positions, those that the requests' tokens read and no others: request r
+// has pages first_r .. first_r + n_r - 1 of its positions, which lie one behind the other in the result and behind those of the requests before
+// it, and the table says where (-1 where a request reads no such page). A CTA finds its request by the lengths, so that the result is as long
+// as the step needs, whatever the table's width. A block with an undefined scale becomes undefined keys and values of zero: a score is left out
+// by choosing, not by multiplying with nothing, so that a token that does not see the block is not made undefined by it.
 constexpr int GATHER = 64;
+
+__device__ __forceinline__ int gathered_pages(int n, int ctx, int window, int& first) {
+    first = 0;
+    if (n <= 0 || ctx <= 0) return 0;
+    if (window > 0 && ctx - n >= window) first = (ctx - n - window + 1) / GATHER;
+    return (ctx - 1) / GATHER - first + 1;
+}
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(128)
 gather_int8_kernel(const signed char* k_pages, const signed char* v_pages, const float* k_scales, const float* v_scales,
                    T* __restrict__ k_out, T* __restrict__ v_out, int* __restrict__ table_out, const int* __restrict__ q_start, const int* __restrict__ ctx_lens,
                    const int* __restrict__ block_table, int bt_stride, int bt_width, int page_size, int num_pages, int kv_heads, int head_dim,
-                   int width, int window) {
+                   int n_req, int pages, int width, int window) {
     pdl_wait();
     pdl_launch_dependents();
-    const int i = blockIdx.x, kvh = blockIdx.y, r = blockIdx.z;
-    const int ctx = ctx_lens[r], first = ctx - (q_start[r + 1] - q_start[r]);
-    const int lo = window > 0 ? max(0, first - window + 1) : 0;
-    const bool used = i * GATHER < ctx && (i + 1) * GATHER > lo;
-    if (kvh == 0 && threadIdx.x == 0) table_out[(size_t)r * width + i] = used ? r * width + i : -1;
-    if (!used) return;
+    const int at = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 31;
+    const bool row = kvh == 0 && at < n_req;            // the CTA writes row ``at`` of the table, too
+    int r = -1, i = 0, ctx = 0, lo = 0;                 // page ``at`` is page i of request r's positions
+    for (int r0 = 0, base = 0; r0 < n_req && (r < 0 || (row && r0 <= at)); r0 += 32) {
+        int n = 0, c = 0, first = 0;
+        if (r0 + lane < n_req) { n = q_start[r0 + lane + 1] - q_start[r0 + lane]; c = ctx_lens[r0 + lane]; }
+        const int mine = gathered_pages(n, c, window, first);
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (row && at >= r0 && at < r0 + 32) {
+            const int begin = base + __shfl_sync(0xffffffffu, sum - mine, at - r0), f = __shfl_sync(0xffffffffu, first, at - r0), count = __shfl_sync(0xffffffffu, mine, at - r0);
+            for (int e = threadIdx.x; e < width; e += 128)
+                table_out[(size_t)at * width + e] = e >= f && e < f + count && begin + e - f < pages ? begin + e - f : -1;
+        }
+        const unsigned found = __ballot_sync(0xffffffffu, at < base + sum);
+        if (r < 0 && found) {
+            const int src = __ffs(found) - 1;
+            const int q_len = __shfl_sync(0xffffffffu, n, src);
+            r = r0 + src;
+            i = at - base - __shfl_sync(0xffffffffu, sum - mine, src) + __shfl_sync(0xffffffffu, first, src);
+            ctx = __shfl_sync(0xffffffffu, c, src);
+            lo = window > 0 && ctx - q_len >= window ? ctx - q_len - window + 1 : 0;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (r < 0 || at >= pages) return;
     constexpr int E = WIDE ? 16 : 1;
     const int chunks = head_dim / E;
-    const size_t to = (((size_t)r * width + i) * kv_heads + kvh) * GATHER * head_dim;
+    const size_t to = ((size_t)at * kv_heads + kvh) * GATHER * head_dim;
     for (int j = threadIdx.x; j < GATHER * chunks; j += 128) {
         const int row = j / chunks, d = (j - row * chunks) * E;
         const int pos = i * GATHER + row, lp = pos / page_size;
@@ -536,20 +567,22 @@ NIB_API int nib_unpack_int8(const void* codes, const float* scales, void* out, l
     return 0;
 }
 
-// The pages of n_req requests as pages of 64 tokens [n_req * width, kv_heads, 64, head_dim] in the order of their positions,
-// with the block table [n_req, width] that addresses them.
+// The positions that the tokens of n_req requests read as pages of 64 tokens [pages, kv_heads, 64, head_dim] in the order of requests and
+// positions, with the block table [n_req, width] that addresses them. ``pages``: at least what the requests' lengths come to; what is more is
+// left as it is.
 NIB_API int nib_gather_int8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales, void* k_out, void* v_out,
                             int* table_out, const int* q_start, const int* ctx_lens, int n_req, const int* block_table, int bt_stride,
-                            int bt_width, int page_size, int num_pages, int kv_heads, int head_dim, int width, int window, int dtype,
+                            int bt_width, int page_size, int num_pages, int kv_heads, int head_dim, int pages, int width, int window, int dtype,
                             cudaStream_t stream) {
-    NIB_REQUIRE(n_req >= 0 && width > 0 && page_size > 0 && num_pages > 0 && kv_heads > 0 && head_dim > 0 && window >= 0, "gather_int8: bad sizes");
+    NIB_REQUIRE(n_req >= 0 && pages > 0 && width > 0 && page_size > 0 && num_pages > 0 && kv_heads > 0 && head_dim > 0 && window >= 0, "gather_int8: bad sizes");
     NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "gather_int8: unknown dtype %d", dtype);
-    NIB_REQUIRE(n_req <= 65535 && kv_heads <= 65535 && (long long)n_req * width < (1LL << 31), "gather_int8: too many requests or heads for one launch");
+    NIB_REQUIRE(kv_heads <= 65535, "gather_int8: too many heads for one launch");
     if (n_req == 0) return 0;
     const bool wide = head_dim % 16 == 0 && (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0;
-#define CALL(T, W) NIB_CUDA(launch_pdl(gather_int8_kernel<T, W>, dim3(width, kv_heads, n_req), dim3(128), (size_t)0, stream, (const signed char*)k_pages, \
+    const unsigned grid = (unsigned)(pages > n_req ? pages : n_req);        // (a request has a row of the table even if it reads no page)
+#define CALL(T, W) NIB_CUDA(launch_pdl(gather_int8_kernel<T, W>, dim3(grid, kv_heads), dim3(128), (size_t)0, stream, (const signed char*)k_pages, \
                                        (const signed char*)v_pages, k_scales, v_scales, (T*)k_out, (T*)v_out, table_out, q_start, ctx_lens, block_table, \
-                                       bt_stride, bt_width, page_size, num_pages, kv_heads, head_dim, width, window))
+                                       bt_stride, bt_width, page_size, num_pages, kv_heads, head_dim, n_req, pages, width, window))
     if (dtype == NIB_F32) { if (wide) CALL(float, true); else CALL(float, false); }
     else { if (wide) CALL(__nv_bfloat16, true); else CALL(__nv_bfloat16, false); }
 #undef CALL

@@ -861,7 +861,11 @@ class Kernels:
         """``attention`` over the 8-bit cache that ``rope_store_int8`` fills: the rotated queries are the first columns of the rows of
         ``qkv``, the step's own keys and values are in the pages already. ``earlier_complete``: the caller promises that
         the pages before the one that a token's own key lies in are no running kernel's results (the engine's steps begin with a copy, which
-        waits for the step before); single tokens' earlier pages are then sent for while the kernel before this one is still running."""
+        waits for the step before); the codes of single tokens' earlier pages are then sent for while the kernel before this one is still running.
+
+        Requests of several tokens take scratch for the positions that they see, in the type of ``qkv``, by the lengths that ``ctx.host`` has. A
+        call that is captured into a graph takes it for as many as the block table is wide, or ``ctx.host.ctx_bounds`` says that the
+        lengths may come to at a replay."""
         n_req, m, width, q_stride, pages, bt_width, bt_stride = self._cache_int8("attention_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table,
                                                                                  k_pages, v_pages, k_scales, v_scales)
         dtype = _DT[qkv.dtype]
@@ -892,20 +896,31 @@ class Kernels:
             self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
         if n_dec == m:          # (all rows: a request may bring none)
             return
-        # The other requests' pages are read back once, in the order of their positions, and the prompt kernels run on them: a portion
-        # reads its keys once for each of its row tiles, and what the tensor cores multiply is 16 bits wide either way.
-        n_rest, width = n_req - n_dec, -(-block_table.shape[1] * page_size // 64)
+        # The other requests' positions are read back once, in order, and the prompt kernels run on them: a portion reads its keys once for each
+        # of its row tiles, and what the tensor cores multiply is 16 bits wide either way. The scratch is as long as what these requests' tokens
+        # see of their own pages: of 60 prompts of 40 tokens beside a token at 128k it is 4 MB (2 kv heads of 128), by the table's width 8 GB.
+        n_rest, span = n_req - n_dec, block_table.shape[1] * page_size
+        width = -(-span // 64)
+        bounds = getattr(ctx.host, "ctx_bounds", None)
+        if bounds is None:
+            bounds = [span] * n_req if torch.cuda.is_current_stream_capturing() else ctx.host.ctx_lens
+        room = 0
+        for n, length in zip(q_lens[n_dec:], bounds[n_dec:]):
+            if n:
+                held = -(-min(length, span) // 64)
+                room += min(held, (n + window + 61) // 64 + 1) if window else held      # (n + window - 1 positions lie in no more)
+        room = max(1, room)
         if not qkv.is_contiguous() or qkv.data_ptr() % 16:          # (the prompt kernels copy aligned, dense rows)
             qkv = qkv[:, :heads * head_dim].clone(memory_format=torch.contiguous_format)
         rows = out if out.data_ptr() % 16 == 0 else torch.empty_like(out)
-        keys = torch.empty((n_rest * width, kv_heads, 64, head_dim), dtype=qkv.dtype, device=qkv.device)
+        keys = torch.empty((room, kv_heads, 64, head_dim), dtype=qkv.dtype, device=qkv.device)
         values = torch.empty_like(keys)
         table = torch.empty((n_req, width), dtype=torch.int32, device=qkv.device)
         self._check(self._lib.nib_gather_int8(
             _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), _ptr(keys), _ptr(values), c_void_p(table.data_ptr() + 4 * n_dec * width),
             c_void_p(ctx.q_start.data_ptr() + 4 * n_dec), c_void_p(ctx.ctx_lens.data_ptr() + 4 * n_dec), c_int(n_rest),
             c_void_p(block_table.data_ptr() + 4 * n_dec * block_table.stride(0)), c_int(block_table.stride(0)), c_int(block_table.shape[1]),
-            c_int(page_size), c_int(k_pages.shape[0]), c_int(kv_heads), c_int(head_dim), c_int(width), c_int(window), c_int(dtype), self._stream()),
+            c_int(page_size), c_int(k_pages.shape[0]), c_int(kv_heads), c_int(head_dim), c_int(room), c_int(width), c_int(window), c_int(dtype), self._stream()),
             "gather (8-bit cache)")
         self._lib.nib_pdl_skip_next()       # the attention reads its table and earlier pages before its wait: here they are the kernel's before it
         self.attention(qkv, rows, heads, kv_heads, head_dim, scale, window, ctx, table, 64, keys, values, first=n_dec)

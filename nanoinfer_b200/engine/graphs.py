@@ -212,7 +212,7 @@ class PortionGraphs:
     is seen, it is one launch. Everything a kernel
     reads of the step (ids, positions, lengths, wanted rows, block tables) lies in a device buffer of fixed
     address that one copy refreshes; the launch geometry depends on the shape alone (for the decoded tokens of
-    a mixed step: on the power of two that bounds their contexts, as in DecodeGraphs). A shape seen once is
+    a mixed step, and over a cache of 8 bits of the portions: on the power of two that bounds their contexts, as in DecodeGraphs). A shape seen once is
     never captured, and at most ``capacity`` shapes are kept. A request that decodes while a long prompt is
     fed in portions of the token budget repeats one shape step after step: n ones and a portion of budget - n."""
 
@@ -240,7 +240,9 @@ class PortionGraphs:
         # decoded tokens: how their keys are split over CTAs is chosen for the power of two that bounds their contexts
         decode_ctx = [e.request.length + 1 for e, n in zip(entries, q_lens) if n == 1]
         cb = max(256, _bucket(max(decode_ctx))) if decode_ctx else 0
-        return q_lens, widths, n_want, all_rows, cb
+        # over a cache of 8 bits a portion's pages are read back into scratch, whose size goes by the power of two that bounds its context
+        bounds = tuple(max(256, _bucket(e.request.length + n)) for e, n in zip(entries, q_lens) if n > 1) if eng.rt.cache_int8 else ()
+        return q_lens, widths, n_want, all_rows, cb, bounds
 
     def step(self, entries, token_arrays, borrow: bool):
         """(True, logits) if the step ran from a graph, (False, None) if the caller has to run it."""
@@ -282,6 +284,8 @@ class PortionGraphs:
         ctx, want_rows, _ = eng.build_context(entries, widths=widths, static=static, token_arrays=token_arrays)
         n_dec = sum(1 for n in key[0] if n == 1)
         ctx.host.ctx_lens[:n_dec] = [key[4]] * n_dec        # (the rows of one token come first: build_context)
+        if key[5]:
+            ctx.host.ctx_bounds = [key[4]] * n_dec + list(key[5])
         caches = eng.storage.layer_caches(ctx.block_tables)
         ops = eng.rt.ops
         torch.cuda.synchronize()

@@ -106,6 +106,7 @@ class HostBatch:
     q_lens: List[int]
     ctx_lens: List[int]            # tokens held by each request AFTER this step's tokens are appended
     slots: List[int]
+    ctx_bounds: Optional[List[int]] = None      # of a step that is captured: what ctx_lens may come to when it is replayed
 
     @property
     def num_requests(self) -> int:

@@ -682,3 +682,63 @@ def test_undefined_blocks_in_portions_are_their_tokens_alone(ops, heads, kv, d, 
                 lo = max(0, 40 + t - window + 1) if window else 0
                 sees[t] = 40 + t >= first and lo < first + page
             assert torch.isnan(got[sees, 1]).all() and torch.equal(got[~sees], want[~sees]) and torch.equal(got[:, 0], want[:, 0]), (j, window)
+
+
+@pytest.mark.parametrize("window", [0, 100])
+def test_scratch_of_portions_follows_what_they_see(ops, window):
+    """Sixty short prompts, and one portion behind 30,000 positions, beside a decoded token at 40,000: by the table's width it would be 61 times
+    40,000 positions (2.5 GB), by what the requests' tokens see it is some thousand (and the one that sees 30,070 of them without a window)."""
+    heads, kv, d, page = 12, 2, 128, 16
+    q_lens, before = [1] + [40] * 60 + [70], [40000] + [(7 * i) % 30 for i in range(60)] + [30000]
+    b = Batch(heads, kv, d, 0, page, q_lens, before, torch.bfloat16, seed=150)
+    out = torch.empty(sum(q_lens), heads * d, dtype=torch.bfloat16, device="cuda")
+
+    def call():
+        ops.attention_int8(b.qkv, out, heads, kv, d, d ** -0.5, window, b.ctx, b.table, page, *b.pools, *b.pool_scales)
+
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    call()
+    seen = sum(-(-(n + p) // 64) for n, p in zip(q_lens[1:], before[1:])) if not window else 60 * 2 + 4       # pages of 64
+    bound = seen * 64 * kv * d * 2 * 2 + 62 * 4 * -(-40001 // 64) + (8 << 20)            # keys and values, the table, queries and the token's parts
+    assert torch.cuda.max_memory_allocated() - held <= bound
+    keys, vals = (ref.values(c, s.cpu()) for c, s in zip(b.codes, b.pool_scales))
+    tables, at = b.table.cpu().tolist(), 0
+    for i, (n, p) in enumerate(zip(q_lens, before)):
+        for t in (0, n // 2, n - 1) if i % 7 in (0, 5) else ():
+            want, size, small = ref.attend(b.rows[at + t, :heads], keys, vals, b.pool_scales[1].cpu(), tables[i], page, p + t, d ** -0.5, window, kv)
+            err = (out[at + t].cpu().double().reshape(heads, d) - want).abs()
+            assert (err <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -14) * size + 2.0 ** -25 * small).all(), (i, t)
+        at += n
+
+
+@pytest.mark.parametrize("bounds", [None, [512, 256, 1024]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_portions_of_a_captured_call_may_be_longer_at_a_replay(ops, dtype, bounds):
+    """The same portions further on in their requests: a table of 1,024 positions, lengths up to it or up to what the call was told."""
+    heads, kv, d, page, q_lens = 4, 2, 64, 16, [1, 70, 33]
+    b = Batch(heads, kv, d, 0, page, q_lens, [400, 180, 980], dtype, seed=160)
+    lens = [[0, 0, 0], [100, 30, 700], [400, 180, 980], [17, 186, 5]]         # held before the step
+    b.ctx.host.ctx_lens = [n for n in q_lens]
+    b.ctx.host.ctx_bounds = bounds
+
+    def inputs(before):
+        b.ctx.ctx_lens.copy_(torch.tensor([n + p for n, p in zip(q_lens, before)], dtype=torch.int32))
+        b.ctx.positions.copy_(torch.cat([torch.arange(p, p + n) for n, p in zip(q_lens, before)]).to(torch.int32))
+
+    inputs(lens[0])
+    k = ops.with_options(fixed_decode_splits=2)
+    graph, side, out = torch.cuda.CUDAGraph(), torch.cuda.Stream(), torch.empty(104, heads * d, dtype=dtype, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        k.attention_int8(b.qkv, out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, page, *b.pools, *b.pool_scales)
+        graph.capture_end()
+    torch.cuda.current_stream().wait_stream(side)
+    for before in lens:
+        inputs(before)
+        out.fill_(float("nan"))
+        graph.replay()
+        b.ctx.host.ctx_lens, b.ctx.host.ctx_bounds = [n + p for n, p in zip(q_lens, before)], None
+        assert torch.equal(out, attention_rows(k, b)), before

@@ -196,3 +196,33 @@ def test_decoding_behind_prompts_of_hundreds_of_tokens(model_dirs, tmp_path, wei
     assert torch.equal(runs[0], runs[1])
     for r in range(3):
         assert_close(runs[0][:, r], want[r], torch.bfloat16, f"request {r}")
+
+
+def test_captured_portions_beside_decoded_tokens_follow_their_lengths(model_dirs):
+    """A prompt fed in portions of 30 beside a request that decodes at 700 and on: replayed and eager steps give the same rows, and a graph's
+    scratch is that of the power of two above the prompt's own context."""
+    from nanoinfer_b200.config import KernelOptions
+    from nanoinfer_b200.engine import StepEntry
+    d, page = model_dirs["C"]
+    model = plain.PlainModel(d)
+    long, prompt, more = tokens(700, model.cfg["vocab"], 11), tokens(450, model.cfg["vocab"], 12), tokens(15, model.cfg["vocab"], 13)
+    runs = []
+    for graphs in (True, False):
+        eng = engine(d, page, "bfloat16", num_pages=300, cache_dtype="int8", cuda_graphs=graphs, kernel_options=KernelOptions(fixed_decode_splits=4))
+        if graphs:
+            eng._portion_graphs.min_tokens, eng._portion_graphs.sightings = 16, 2
+        a, b = eng.open("a"), eng.open("b")
+        eng.step([StepEntry(a, long, [])])
+        rows = []
+        for t in range(15):
+            rows.append(eng.step([StepEntry(b, prompt[30 * t:30 * t + 30], [29]), StepEntry(a, [more[t]], [0])]).clone())
+        runs.append(torch.stack(rows))
+        if graphs:
+            captured = eng._portion_graphs.captured
+            assert sorted(key[5] for key in captured) == [(256,), (512,)] and eng.graph_launches > 0
+        eng.check_device()
+    assert torch.equal(runs[0], runs[1])
+    want = plain_rows(model, prompt, [30] * 15, page)[29::30]
+    assert_close(runs[0][:, 0], want, torch.bfloat16, "the prompt")
+    want = plain_rows(model, long + more, [700] + [1] * 15, page)[700:]
+    assert_close(runs[0][:, 1], want, torch.bfloat16, "the decoded tokens")
