@@ -12,11 +12,22 @@ GROUPS = (32, 64, 128)
 
 class Int4Matrix:
     """``shape`` (rows, columns), ``group``, and on the device ``packed`` (uint8, half a byte a weight; rows and columns are padded to
-    whole tiles) and ``scales`` (bfloat16). ``bf16_exact``: every weight is a bfloat16 number (no scale has more than 5 significant
-    bits; a code has 3)."""
+    whole tiles) and ``scales`` (bfloat16, for every row of the tiles); neither is replaced afterwards. ``bf16_exact``: every weight is a
+    bfloat16 number (no scale has more than 5 significant bits; a code has 3)."""
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, shape, group: int, bf16_exact: bool):
-        self.packed, self.scales, self.shape, self.group, self.bf16_exact = packed, scales, tuple(shape), int(group), bool(bf16_exact)
+        if group not in GROUPS:
+            raise ValueError(f"groups of {GROUPS} weights are possible, not of {group}")
+        n, k = (int(x) for x in shape)
+        if n <= 0 or k <= 0 or k % group:
+            raise ValueError(f"{n} rows of {k} weights: columns are a multiple of {group}")
+        # (the kernels read by ``shape``: what they read has to be there)
+        row_tiles, k_tiles = -(-n // 16), -(-k // 64)
+        for what, t, dtype, count in (("codes", packed, torch.uint8, row_tiles * k_tiles * 512), ("scales", scales, torch.bfloat16, row_tiles * 16 * (k // group))):
+            if t.dtype != dtype or t.numel() != count or not t.is_contiguous() or t.device != packed.device:
+                raise ValueError(f"the {what} of {n} x {k} weights in groups of {group} are {count} dense {dtype} on the codes' device; got {t.dtype} "
+                                 f"{tuple(t.shape)} on {t.device}")
+        self.packed, self.scales, self.shape, self.group, self.bf16_exact = packed, scales, (n, k), int(group), bool(bf16_exact)
 
     @property
     def device(self) -> torch.device:

@@ -66,3 +66,16 @@ def test_refusals():
                 (torch.full((4, 64), float("inf")), 32)):
         with pytest.raises(ValueError):
             Int4Matrix.quantize(*bad)
+
+
+def test_a_matrix_whose_parts_do_not_fit_its_shape_is_refused():
+    """The kernels read codes and scales by the shape: anything shorter, or of another type, would be read beyond its end."""
+    w = Int4Matrix.from_codes(torch.zeros(40, 192, dtype=torch.uint8), torch.ones(40, 3, dtype=torch.bfloat16), 64)
+    again = Int4Matrix(w.packed, w.scales, w.shape, w.group, w.bf16_exact)
+    assert again.shape == (40, 192) and torch.equal(unpacked(again), unpacked(w))
+    for bad in ((w.packed[:-512], w.scales, w.shape, 64), (w.packed, w.scales[:-1], w.shape, 64), (w.packed, w.scales, (64, 192), 64), (w.packed, w.scales, (40, 256), 64),
+                (w.packed, w.scales, w.shape, 32), (w.packed, w.scales, w.shape, 48), (w.packed, w.scales, (0, 192), 64), (w.packed, w.scales, (40, 160), 64),
+                (w.packed.to(torch.int8), w.scales, w.shape, 64), (w.packed, w.scales.float(), w.shape, 64), (w.packed.repeat(2)[::2], w.scales, w.shape, 64),
+                (w.packed, w.scales.to("meta"), w.shape, 64), (w.packed, w.scales, (40,), 64)):
+        with pytest.raises(ValueError):
+            Int4Matrix(*bad, True)
