@@ -503,7 +503,7 @@ NIB_API int nib_gemm_int4(const void* args, cudaStream_t stream) {
     const bool dual = epi_dual(epi);
     NIB_REQUIRE(tokens >= 0 && sms > 0 && fits(n, k, group), "gemm_int4: %d tokens, %d x %d weights in groups of %d are not supported", tokens, n, k, group);
     NIB_REQUIRE(epi == EPI_STORE || epi == EPI_ADD || epi == EPI_F32 || dual, "gemm_int4: unknown epilogue %d", epi);
-    NIB_REQUIRE((((uintptr_t)c.w) & 15) == 0 && (((uintptr_t)c.scales) & 3) == 0, "gemm_int4: weights must be 16-byte aligned");
+    NIB_REQUIRE((((uintptr_t)c.w) & 15) == 0 && (((uintptr_t)c.scales) & 3) == 0, "gemm_int4: weights must be 16-byte aligned, scales 4-byte");
     NIB_REQUIRE(((uintptr_t)c.scratch & 15) == 0, "gemm_int4: scratch must be 16-byte aligned");
     if (tokens > 64 || c.ldx % 8 != 0 || ((uintptr_t)c.x & 15) != 0 || (dual && n % 16 != 0)) return -1;
     if (tokens == 0) return 0;
@@ -550,7 +550,7 @@ NIB_API int nib_gemm_int4(const void* args, cudaStream_t stream) {
 NIB_API int nib_unpack_int4(const void* w, const void* scales, void* out, int n, int k, int group, int part, int dtype, cudaStream_t stream) {
     NIB_REQUIRE(fits(n, k, group), "unpack_int4: %d x %d weights in groups of %d are not supported", n, k, group);
     NIB_REQUIRE(dtype == NIB_F32 || dtype == NIB_BF16, "unpack_int4: unknown dtype %d", dtype);
-    NIB_REQUIRE((((uintptr_t)w | (uintptr_t)out) & 15) == 0, "unpack_int4: weights and result must be 16-byte aligned");
+    NIB_REQUIRE((((uintptr_t)w | (uintptr_t)out) & 15) == 0 && ((uintptr_t)scales & 3) == 0, "unpack_int4: weights and result must be 16-byte aligned, scales 4-byte");
     const int k_tiles = ceil_div(k, 64), shift = group == 32 ? 5 : group == 64 ? 6 : 7;
     const long long items = (long long)ceil_div(n, 16) * k_tiles * 32, grid = (items + 255) / 256;
     NIB_REQUIRE(grid < (1LL << 31) - 1, "unpack_int4: too many weights for one launch");

@@ -244,3 +244,15 @@ def test_rows_of_wider_tensors_in_every_mode(ops, m, dtype):
             extra = 2.0 ** -8 * want.abs() if mode == "store" and dtype == torch.bfloat16 else 0.0
             assert ((out[:, 3:99].cpu().double() - want - (0.5 if mode == "add" else 0.0)).abs() <= bound + extra).all(), (width, lead, mode)
             assert (out[:, :3] == 0.5).all() and (out[:, 99:] == 0.5).all()
+
+
+@pytest.mark.parametrize("m", [5, 70])
+def test_codes_and_scales_off_their_words_are_refused(ops, m):
+    from nanoinfer_b200.csrc.lib import KernelError
+    w, _ = matrix(64, 128, 64, 23)
+    x, out = rows(m, 128, torch.bfloat16, 24).cuda(), torch.empty(m, 64, dtype=torch.bfloat16, device="cuda")
+    for lead_codes, lead_scales in ((8, 0), (0, 1)):
+        codes = torch.empty(w.packed.numel() + 16, dtype=torch.uint8, device="cuda")[lead_codes:lead_codes + w.packed.numel()].copy_(w.packed)
+        scales = torch.empty(w.scales.numel() + 2, dtype=torch.bfloat16, device="cuda")[lead_scales:lead_scales + w.scales.numel()].copy_(w.scales.reshape(-1))
+        with pytest.raises(KernelError):
+            ops.linear(x, Int4Matrix(codes, scales, w.shape, w.group, w.bf16_exact), None, out, "store")
