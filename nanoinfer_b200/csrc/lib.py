@@ -29,6 +29,7 @@ _ADD = _EPI["add"]
 _DUAL = (3, 5, 6)       # the gated epilogues: two accumulators, gate rows and up rows
 # The arguments of calls that take them as one block of memory (NibAppendInt8, NibAttendInt8, NibGemmInt4)
 _APPEND_INT8, _ATTEND_INT8, _GEMM_INT4 = struct.Struct("=12Q16i"), struct.Struct("=10Q14ifi"), struct.Struct("=6Q8i3fi")
+_MOST = 2 ** 31 - 1     # strides go to the kernels in 32 bits
 _LAYOUT = {"interleaved": 0, "half": 1}     # which elements of a rotated vector make a pair
 
 
@@ -543,8 +544,8 @@ class Kernels:
         epi = _EPI[mode]
         dual = epi in _DUAL
         n = w.shape[0] // 2 if dual else w.shape[0]
-        if a.dim() != 2 or out.dim() != 2 or a.stride(1) != 1 or out.stride(1) != 1:
-            raise KernelError(f"{what}: rows must be dense")
+        if a.dim() != 2 or out.dim() != 2 or a.stride(1) != 1 or out.stride(1) != 1 or a.stride(0) > _MOST or out.stride(0) > _MOST:
+            raise KernelError(f"{what}: rows must be dense and at most {_MOST} elements apart")
         m, k = a.shape
         if a.dtype not in _DT or w.shape[1] != k or (dual and 2 * n != w.shape[0]) or out.shape != (m, n):
             raise KernelError(f"{what}: shapes {a.dtype} a{tuple(a.shape)} w{w.shape} out{tuple(out.shape)} do not fit")
@@ -800,6 +801,8 @@ class Kernels:
             raise KernelError(f"{what}: dense rows of bfloat16 or float32, not {qkv.dtype} {tuple(qkv.shape)}")
         if len(table) != 2 or table_stride[1] != 1:
             raise KernelError(f"{what}: block_table rows must be dense")
+        if row_stride[0] > _MOST or table_stride[0] > _MOST:
+            raise KernelError(f"{what}: rows lie at most {_MOST} elements apart, not {row_stride[0]} and {table_stride[0]}")
         m, n_req = rows[0], len(ctx.host.q_lens)
         if sum(ctx.host.q_lens) != m or positions.numel() < m or req_index.numel() < m or q_start.numel() != n_req + 1 \
                 or ctx_lens.numel() != n_req or table[0] < n_req:
@@ -822,7 +825,7 @@ class Kernels:
         if width != (heads + 2 * kv_heads) * head_dim or q_out.shape != (m, heads * head_dim):
             raise KernelError("rope_store_int8: widths do not fit the head counts")
         out_stride = q_out.stride()
-        if q_out.get_device() != device or q_out.dtype != qkv.dtype or out_stride[1] != 1:
+        if q_out.get_device() != device or q_out.dtype != qkv.dtype or out_stride[1] != 1 or out_stride[0] > _MOST:
             raise KernelError(f"rope_store_int8: q_out is {q_out.dtype} on {q_out.device}, {qkv.dtype} in dense rows on {qkv.device} is wanted")
         cos = sin = rot = rows = 0
         if rotary is not None:
@@ -869,8 +872,8 @@ class Kernels:
         n_req, m, width, q_stride, pages, bt_width, bt_stride = self._cache_int8("attention_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table,
                                                                                  k_pages, v_pages, k_scales, v_scales)
         dtype = _DT[qkv.dtype]
-        if heads <= 0 or heads % kv_heads or width < heads * head_dim or out.shape != (m, heads * head_dim) or window < 0:
-            raise KernelError("attention_int8: widths do not fit the head counts")
+        if heads <= 0 or heads % kv_heads or width < heads * head_dim or out.shape != (m, heads * head_dim) or not 0 <= window <= _MOST:
+            raise KernelError("attention_int8: widths do not fit the head counts, or the window is out of range")
         if out.get_device() != qkv.get_device() or out.dtype != qkv.dtype or not out.is_contiguous():
             _here(out, qkv.dtype, "attention_int8 out")
         if m == 0:

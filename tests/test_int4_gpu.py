@@ -256,3 +256,14 @@ def test_codes_and_scales_off_their_words_are_refused(ops, m):
         scales = torch.empty(w.scales.numel() + 2, dtype=torch.bfloat16, device="cuda")[lead_scales:lead_scales + w.scales.numel()].copy_(w.scales.reshape(-1))
         with pytest.raises(KernelError):
             ops.linear(x, Int4Matrix(codes, scales, w.shape, w.group, w.bf16_exact), None, out, "store")
+
+
+def test_rows_further_apart_than_32_bits_are_refused(ops):
+    from nanoinfer_b200.csrc.lib import KernelError
+    w, _ = matrix(64, 128, 64, 25)
+    for dtype in (torch.bfloat16, torch.float32):
+        x, out = rows(1, 128, dtype, 26).cuda(), torch.empty(1, 64, dtype=dtype, device="cuda")
+        ops.linear(x, w, None, out, "store")
+        for bad in ((x.as_strided((1, 128), (2 ** 31, 1)), out), (x, out.as_strided((1, 64), (2 ** 31, 1)))):
+            with pytest.raises(KernelError):
+                ops.linear(bad[0], w, None, bad[1], "store")

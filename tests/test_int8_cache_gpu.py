@@ -742,3 +742,28 @@ def test_portions_of_a_captured_call_may_be_longer_at_a_replay(ops, dtype, bound
         graph.replay()
         b.ctx.host.ctx_lens, b.ctx.host.ctx_bounds = [n + p for n, p in zip(q_lens, before)], None
         assert torch.equal(out, attention_rows(k, b)), before
+
+
+def test_rows_further_apart_than_32_bits_are_refused(ops):
+    """Strides go to the kernels in 32 bits. (One row each: nothing lies at the stride's end.)"""
+    from nanoinfer_b200.csrc.lib import KernelError
+    far = 2 ** 31
+    for q_lens, before in (([1], [5]), ([40], [5])):
+        b = Batch(4, 2, 64, 64, 16, q_lens, before, torch.bfloat16, seed=170)
+        m = q_lens[0]
+        q = torch.empty(m, 256, dtype=torch.bfloat16, device="cuda")
+        b.append(ops, q_out=q)
+        one = m == 1
+        rows = b.qkv.as_strided(b.qkv.shape, (far, 1)) if one else b.qkv
+        out = q.as_strided(q.shape, (far, 1)) if one else q
+        table = b.table.as_strided(b.table.shape, (far, 1))
+        for change in [dict(block_table=table)] + ([dict(qkv=rows), dict(q_out=out)] if one else []):
+            a = dict(qkv=b.qkv, q_out=q, heads=4, kv_heads=2, head_dim=64, ctx=b.ctx, rotary=b.rotary, block_table=b.table, page_size=16,
+                     k_pages=b.pools[0], v_pages=b.pools[1], k_scales=b.pool_scales[0], v_scales=b.pool_scales[1])
+            with pytest.raises(KernelError):
+                ops.rope_store_int8(**{**a, **change})
+        for change in [dict(block_table=table), dict(window=far)] + ([dict(qkv=rows)] if one else []):
+            a = dict(qkv=b.qkv, out=q, heads=4, kv_heads=2, head_dim=64, scale=0.125, window=0, ctx=b.ctx, block_table=b.table, page_size=16,
+                     k_pages=b.pools[0], v_pages=b.pools[1], k_scales=b.pool_scales[0], v_scales=b.pool_scales[1])
+            with pytest.raises(KernelError):
+                ops.attention_int8(**{**a, **change})
