@@ -913,7 +913,7 @@ class Kernels:
                 held = -(-min(length, span) // 64)
                 room += min(held, (n + window + 61) // 64 + 1) if window else held      # (n + window - 1 positions lie in no more)
         room = max(1, room)
-        if not qkv.is_contiguous() or qkv.data_ptr() % 16:          # (the prompt kernels copy aligned, dense rows)
+        if not qkv.is_contiguous() or qkv.data_ptr() % 16 or qkv.shape[1] % 2:          # (the prompt kernels copy aligned, dense rows)
             qkv = qkv[:, :heads * head_dim].clone(memory_format=torch.contiguous_format)
         rows = out if out.data_ptr() % 16 == 0 else torch.empty_like(out)
         keys = torch.empty((room, kv_heads, 64, head_dim), dtype=qkv.dtype, device=qkv.device)

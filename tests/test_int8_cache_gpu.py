@@ -767,3 +767,17 @@ def test_rows_further_apart_than_32_bits_are_refused(ops):
                      k_pages=b.pools[0], v_pages=b.pools[1], k_scales=b.pool_scales[0], v_scales=b.pool_scales[1])
             with pytest.raises(KernelError):
                 ops.attention_int8(**{**a, **change})
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_portions_of_dense_rows_of_odd_width(ops, dtype):
+    for heads, kv, d in ((4, 2, 64), (12, 2, 128), (3, 1, 33)):
+        b = Batch(heads, kv, d, 0, 16, [1, 40, 2], [30, 20, 9], dtype, seed=171)
+        want = attention_rows(ops, b)
+        wide = torch.zeros(43, b.qkv.shape[1] + 1 + b.qkv.shape[1] % 2, dtype=dtype, device="cuda")
+        assert wide.shape[1] % 2 and wide.is_contiguous()
+        wide[:, :b.qkv.shape[1]] = b.qkv
+        out = torch.empty_like(want)
+        ops.attention_int8(wide, out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, 16, *b.pools, *b.pool_scales)
+        # a decoded token whose rows lie off 4 bytes goes to another kernel, whose weights are not rounded to 16 bits
+        assert (out[0].double() - want[0].double()).abs().max() <= 2.0 ** -6 * want[0].double().abs().max() and torch.equal(out[1:], want[1:])
