@@ -226,3 +226,44 @@ def test_captured_portions_beside_decoded_tokens_follow_their_lengths(model_dirs
     assert_close(runs[0][:, 0], want, torch.bfloat16, "the prompt")
     want = plain_rows(model, long + more, [700] + [1] * 15, page)[700:]
     assert_close(runs[0][:, 1], want, torch.bfloat16, "the decoded tokens")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_layer_that_reads_another_layers_8_bit_cache(tmp_path, dtype, monkeypatch):
+    """A run order in which a layer reads the cache of an earlier one and writes none: its queries alone are rotated, and it sees the codes."""
+    import test_toy_parts_gpu as toy
+    from nanoinfer_b200.engine import StepEntry
+    from nanoinfer_b200.registry import config_from_json_dict
+    from nanoinfer_b200.weights import write_random_model
+    toy._register()
+    d, page = str(tmp_path / "toy"), 8
+    write_random_model(config_from_json_dict(toy.TOY), d, seed=3)
+    w, ids = toy.read_weights(d), tokens(61, 97, 14)
+    other = toy.plain_toy(w, ids)
+
+    def coded(x):
+        pages = -(-x.shape[0] // page)
+        codes, scales = torch.zeros(pages, x.shape[1], page, x.shape[2], dtype=torch.float64), torch.ones(pages, x.shape[1], dtype=torch.float64)
+        ref.append(codes, scales, x, 0, list(range(pages)), page)
+        return ref.values(codes, scales).permute(0, 2, 1, 3).reshape(-1, *x.shape[1:])[:x.shape[0]]
+
+    attention = toy.causal_attention_fast
+    monkeypatch.setattr(toy, "causal_attention_fast", lambda q, k, v: attention(q, coded(k), coded(v)))
+    want = toy.plain_toy(w, ids)
+    eng = engine(d, page, dtype, num_pages=40, max_batch=3, cache_dtype="int8")
+    needs = eng.model.cache_needs()
+    assert needs[4][0] is None and needs[4][2] == 1
+    rc = eng.open("a")
+    got = eng.step([StepEntry(rc, ids, list(range(61)))]).cpu().double()
+    if dtype == "float32":
+        assert rms(got - want) <= 0.1 * rms(want - other)
+    else:
+        assert_close(got, want, torch.bfloat16, "one portion")
+    # decoded on: a token's own page is re-rounded as it fills, by less than a step, which is what the codes are from the plain model
+    more = tokens(9, 97, 15)
+    rows = torch.cat([eng.step([StepEntry(rc, [t], [0])]) for t in more]).cpu().double()
+    want = toy.plain_toy(w, ids + more)[61:]
+    monkeypatch.undo()
+    assert rms(rows - want) <= 2 * rms(want - toy.plain_toy(w, ids + more)[61:]) + (0.015 * rms(want) if dtype == "bfloat16" else 0)
+    eng.close(rc)
+    eng.cache.check()
