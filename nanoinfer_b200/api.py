@@ -35,7 +35,8 @@ class Model:
 
         ``use_cache=False`` is the reference's ``--no-cache`` (nanoinfer/generate.py:44-60, 94-98): every
         token is computed from the whole sequence so far with nothing kept between tokens. It is slow and
-        exists to check the cache: both ways give the same tokens."""
+        exists to check the cache: both ways give the same tokens. Not with ``cache_dtype`` "int8": the codes of a page depend on how its
+        tokens came (see ``EngineConfig.cache_dtype``), and a token may come out differently."""
         params = params or SamplingParams()
         if params.seed is not None:
             seed = params.seed

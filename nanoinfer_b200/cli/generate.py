@@ -69,7 +69,8 @@ def main(argv=None) -> int:
     add_model_args(p)
     add_sampling_args(p)
     p.add_argument("--no-cache", dest="use_cache", action="store_false",
-                   help="recompute the whole sequence for every token (slow; checks the cache: same output)")
+                   help="recompute the whole sequence for every token (slow; checks the cache: same output, "
+                        "but for rounding with --cache-dtype int8)")
     args = p.parse_args(argv)
 
     from ..api import generate, load_model

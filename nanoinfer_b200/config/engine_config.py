@@ -17,7 +17,10 @@ _DTYPES = {"bfloat16": "bfloat16", "bf16": "bfloat16", "float32": "float32", "fp
 @dataclass(frozen=True)
 class EngineConfig:
     dtype: str = "bfloat16"          # "bfloat16": serving kernels; "float32": true 32-bit everywhere
-    cache_dtype: str = "auto"        # keys and values: "auto" as dtype; "int8" codes of 8 bits, a scale for each page and kv head
+    # keys and values: "auto" as dtype; "int8" codes of 8 bits, a scale for each page and kv head. A page whose tokens came one by one may hold an
+    # element up to a step off what it holds where they came together, so what a request continues with may depend on how its prompt was cut,
+    # on a preemption (its tokens are computed anew, together) and on a truncation (the scale that a forgotten token made larger stays)
+    cache_dtype: str = "auto"
     weight_format: str = "auto"      # matrices of attention and feed-forward: "auto" as dtype; "int4" codes of 4 bits, quantized at load
     weight_group: int = 64           # int4: weights of a row that share a scale (32, 64 or 128)
     page_size: int = 16              # tokens per cache page

@@ -84,7 +84,8 @@ class Engine:
 
     def truncate(self, rc: RequestCache, new_length: int) -> None:
         """The request forgets its positions from ``new_length`` on (to recompute them, or to decode from the same
-        context again). A model whose mixers keep per-request state cannot go back."""
+        context again). A model whose mixers keep per-request state cannot go back. In a cache of 8 bits the last page keeps the scale that
+        it has come to, also where a forgotten token made it larger."""
         if self.storage.state:
             raise ValueError("a model with per-request state cannot be truncated: the state has no history")
         self.cache.truncate(rc, new_length)

@@ -9,7 +9,8 @@ The reference's scheduler (cpp/python/ni/scheduler.py:200-375) has the same queu
 counters, but prefills each admitted prompt whole and alone and reserves the worst case of pages up
 front. Here pages are taken step by step. When the pool cannot hold a step's new tokens, the request
 admitted last is preempted: its pages are given back, it returns to the head of the waiting queue
-and is later recomputed from its prompt and the tokens it had generated.
+and is later recomputed from its prompt and the tokens it had generated (over a cache of 8 bits in codes
+that may be a step off those it had, see EngineConfig.cache_dtype).
 """
 from __future__ import annotations
 

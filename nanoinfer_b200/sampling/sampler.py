@@ -3,7 +3,8 @@
 Order (nanoinfer/sampling.py:126-151): repetition penalty -> greedy when temperature is 0 ->
 temperature -> top-k -> top-p -> softmax -> draw. The uniform number of a draw is a function of
 (seed, number of tokens the request has generated), so what a request samples does not depend on
-the batch it is in, nor on whether it was preempted and recomputed. The reference draws from a
+the batch it is in, nor on whether it was preempted and recomputed (as far as its logits do not: with a cache of 8 bits, whose codes
+depend on how a page's tokens came, they may). The reference draws from a
 stateful generator per sequence (cpp/python/ni/scheduler.py:69), so its sampled tokens are
 reproducible only within one engine; so are these.
 """

@@ -87,3 +87,11 @@ def test_commands_take_the_options(monkeypatch, tmp_path):
         with pytest.raises(KeyboardInterrupt):
             main(["--model-dir", str(tmp_path), "--cache-dtype", "int8", "--weights", "int4", "--weight-group", "32"] + extra)
     assert all(k["cache_dtype"] == "int8" and k["weight_format"] == "int4" and k["weight_group"] == 32 for k in seen) and len(seen) == 2
+
+
+def test_what_an_8_bit_cache_does_not_promise_is_said_where_it_is_promised():
+    from nanoinfer_b200.api import Model
+    from nanoinfer_b200.engine import scheduler
+    from nanoinfer_b200.engine.engine import Engine
+    for text in (Model.generate.__doc__, Engine.truncate.__doc__, scheduler.__doc__):
+        assert "int8" in text or "8 bits" in text
