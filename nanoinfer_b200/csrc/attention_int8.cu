@@ -807,7 +807,7 @@ long long any_smem(int n_rep, int hd) { return 4LL * (2LL * n_rep * hd + GT * (2
 constexpr long long MAX_SMEM = 226 * 1024;         // (and what a CTA has besides)
 
 template <typename T, int CH>
-int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int threads, long long smem, const void* q, void* out, cudaStream_t stream) {
+int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int sms, int threads, long long smem, const void* q, void* out, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = a.shares ? dim3(a.shares) : dim3(a.csize, a.n_tokens, a.kv_heads);
     cfg.blockDim = dim3(threads);
@@ -830,7 +830,7 @@ int launch_rows(void (*kernel)(const T*, T*, Args), const Args& a, int threads, 
     cfg.attrs = attr;
     cfg.numAttrs = n;
     NIB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const T*)q, (T*)out, a));
-    if (a.shares) NIB_CUDA(launch_pdl(merge_int8_kernel<T, CH>, dim3(a.heads, a.n_tokens), dim3(a.heads * a.n_tokens <= 2 * 148 ? MERGE_THREADS : MERGE_THREADS / 2), (size_t)0, stream, (T*)out, a));
+    if (a.shares) NIB_CUDA(launch_pdl(merge_int8_kernel<T, CH>, dim3(a.heads, a.n_tokens), dim3(a.heads * a.n_tokens <= 2 * sms ? MERGE_THREADS : MERGE_THREADS / 2), (size_t)0, stream, (T*)out, a));
     return 0;
 }
 
@@ -848,7 +848,7 @@ struct NibAttendInt8 {
     const void* q; void* out; const int* ctx_lens; const int* block_table; const void* k_pages; const void* v_pages; const float* k_scales;
     const float* v_scales; float* part_o; float* part_ml;
     int q_stride, bt_stride, bt_width, page_size, num_pages, n_tokens, heads, kv_heads, head_dim, window, ctas, shares, dtype, early;
-    float scale; int pad;
+    float scale; int sms;       // sms: SMs of the device
 };
 
 // Attention of n_tokens single tokens (token i is request i, at position ctx_lens[i] - 1) whose keys and values are in the pages.
@@ -869,7 +869,7 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     } else {
         NIB_REQUIRE(c.ctas == 1 || c.ctas == 2 || c.ctas == 4 || c.ctas == 8, "attention (8-bit cache): 1, 2, 4 or 8 CTAs share a row's keys, not %d", c.ctas);
     }
-    NIB_REQUIRE(n_tokens <= 65535 && kv_heads <= 65535, "attention (8-bit cache): too many tokens or heads for one launch");
+    NIB_REQUIRE(c.sms > 0 && n_tokens <= 65535 && kv_heads <= 65535, "attention (8-bit cache): too many tokens or heads for one launch");
     if (n_tokens == 0) return 0;
     int shift = -1;
     if ((page_size & (page_size - 1)) == 0) for (shift = 0; (1 << shift) < page_size;) ++shift;
@@ -882,7 +882,7 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
 #define CALL(KERNEL, T, CH, THREADS, SMEM, MOST)                                                                                \
     do {                                                                                                                        \
         NIB_CUDA((allow_smem_once<KERNEL>((int)(MOST))));                                                                       \
-        rc = launch_rows<T, CH>((KERNEL), a, THREADS, SMEM, q, out, stream);                                                      \
+        rc = launch_rows<T, CH>((KERNEL), a, c.sms, THREADS, SMEM, q, out, stream);                                                      \
     } while (0)
 #define MMA(HD, NH, WHOLE)                                                                                                      \
     CALL((attention_int8_mma_kernel<HD, NH, WHOLE>), __nv_bfloat16, (Mma<HD, NH>::CHUNK), WARPS * 32, (Mma<HD, NH>::BYTES), (Mma<HD, NH>::BYTES))

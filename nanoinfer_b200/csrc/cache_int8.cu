@@ -146,10 +146,10 @@ __device__ __forceinline__ unsigned magnitude_up(const Two& y) {
     const unsigned bits = __float_as_uint(y.hi) & 0x7fffffffu;
     return bits + ((y.lo != 0.f && (y.lo > 0.f) == (y.hi > 0.f) && bits < 0x7f800000u) ? 1u : 0u);
 }
-// rint((hi + lo) / s) within -127..127, inv = 1 / s, a power of two: the product with it is exact. Of a NaN: 0 (its block's scale
-// says so).
+// rint((hi + lo) / s) within -127..127, inv = 1 / s, a power of two: the product with it is exact. Of a NaN: -127 (a code like any other; its
+// block's scale, NaN too, is what says that it is undefined).
 __device__ __forceinline__ int code_of(const Two& y, float inv) {
-    const float v = fminf(fmaxf(__fmul_rn(y.hi, inv), -127.f), 127.f);          // (a NaN becomes a bound; the scale is what says so)
+    const float v = fminf(fmaxf(__fmul_rn(y.hi, inv), -127.f), 127.f);
     float r = rintf(v);
     if (fabsf(v - r) == 0.5f && y.lo != 0.f) r = y.lo > 0.f ? ceilf(v) : floorf(v);
     return (int)r;

@@ -532,9 +532,15 @@ class Kernels:
 
     def _linear_int4(self, what, a, w, bias32, out, mode, glu):
         """A product with 4-bit weights. Up to 64 tokens of bfloat16 multiply with the codes (gemm_int4.cu); more, and 32-bit rows, with
-        the weights unpacked into a scratch matrix of their own type, by the products above. Weights whose scales need more than
-        bfloat16's 8 bits are rounded there where the result is rounded to bfloat16 itself; a 32-bit result gets what the rounding
-        left by a second product."""
+        the weights unpacked into a scratch matrix of their own type, by the products above. (At 33 to 64 tokens unpacking is the slower way
+        too, us in a chain, codes / unpacked / bfloat16 weights: 64 tokens at the 7B widths, q/k/v 12.7 / 21.3 / 15.5, gate/up 80 / 112 / 48, down
+        49 / 119 / 95, 1.5B gate/up 22.1 / 22.8 / 11.6; the 0.5B gate/up alone is even, 13.9 / 13.4 / 7.9, and 16.0 / 18.7 from memory.)
+
+        Weights whose scales need more than bfloat16's 8 bits are rounded by the unpacking where the result is rounded to bfloat16 itself: the
+        same matrix is then another one, by half a step of bfloat16 for every weight, for 65 tokens and for 64. That is chosen for its time:
+        1,536 x 8,960 and 601 tokens 37 us, off 64 bits by 0.0022 (rms, relative), where a second product with what the rounding left
+        took 67, off by 0.0017, which the result's own rounding is. A 32-bit result gets the second product. ``Int4Matrix.quantize``, which
+        the engine's weights come from, makes scales with which every weight is a bfloat16 number and nothing is rounded."""
         if isinstance(a, LazyNorm):
             a = self._resolve(a, a.shape[0] <= 16)
         device = torch.cuda.current_device()
@@ -561,9 +567,11 @@ class Kernels:
             if not self.weights_ahead:
                 self._lib.nib_pdl_skip_next()
             alpha, limit, shift = (0.0, 0.0, 0.0) if glu is None else glu
-            # Activations prepared as 16-bit floats: 11 instructions of every tile's 65 for a kernel before (3.5 us by itself at 8 tokens of 3,584), which pays
-            # where a product takes twenty (7B widths, us with / without: gate/up at 8 tokens 18.8 / 23.1, at 16 24.4 / 26.4, at 32 45.8 /
-            # 42.5; down at 8 23.0 / 20.7).
+            # Activations prepared as 16-bit floats: fewer instructions for every tile, and a kernel before (3.5 us by itself at 8 tokens of 3,584),
+            # which pays for large matrices. us with / without, 1, 8 and 16 tokens: 16 MB of codes (2,048 wide) 7.8 / 7.7, 8.2 / 8.0, 10.3 / 9.3; 28 MB (14,336 wide)
+            # 13.8 / 12.6, 14.4 / 13.1, 17.1 / 15.1; 32 MB (4,096 wide) 18.1 / 19.4, 19.2 / 20.2, 24.0 / 23.6, (18,944 wide) 17.0 / 16.3, 17.6 / 16.9, 21.4 / 19.4;
+            # 48 MB 25.8 / 27.7, 27.0 / 28.8, 33.9 / 33.4; 50 MB (20,480 wide) 21.3 / 21.8, 21.8 / 22.3, 26.5 / 25.7; 65 MB 18.2 / 21.6, 18.8 / 21.8, 23.7 / 24.8.
+            # (32 tokens, 65 MB: 45.8 / 42.5.)
             scratch = self._lib.nib_gemm_int4_scratch(m, k) if m <= 16 and w.packed.numel() >= 48 << 20 else 0
             room = torch.empty(scratch, dtype=torch.uint8, device=a.device) if scratch else None
             args = _GEMM_INT4.pack(a.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), 0 if bias32 is None else bias32.data_ptr(), out.data_ptr(),
@@ -895,12 +903,13 @@ class Kernels:
                 self.launches += 1
             args = _ATTEND_INT8.pack(
                 qkv.data_ptr(), out.data_ptr(), ctx.ctx_lens.data_ptr(), block_table.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, q_stride, bt_stride, bt_width, page_size, pages, n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 1 if earlier_complete else 0, scale, 0)
+                k_scales.data_ptr(), v_scales.data_ptr(), part_o, part_ml, q_stride, bt_stride, bt_width, page_size, pages, n_dec, heads, kv_heads, head_dim, window, ctas, shares, dtype, 1 if earlier_complete else 0, scale, self.sm_count)
             self._check(self._lib.nib_attention_int8_decode(args, self._stream()), "attention decode (8-bit cache)")
         if n_dec == m:          # (all rows: a request may bring none)
             return
         # The other requests' positions are read back once, in order, and the prompt kernels run on them: a portion reads its keys once for each
-        # of its row tiles, and what the tensor cores multiply is 16 bits wide either way. The scratch is as long as what these requests' tokens
+        # of its row tiles, and what the tensor cores multiply is 16 bits wide either way. (Their weights are rounded to bfloat16 there, as they are
+        # over a cache of 16 bits: 0.0023 from 64 bits in place of 0.0017, which a single token's row has.) The scratch is as long as what these requests' tokens
         # see of their own pages: of 60 prompts of 40 tokens beside a token at 128k it is 4 MB (2 kv heads of 128), by the table's width 8 GB.
         n_rest, span = n_req - n_dec, block_table.shape[1] * page_size
         width = -(-span // 64)
