@@ -866,6 +866,8 @@ NIB_API int nib_attention_int8_decode(const void* args, cudaStream_t stream) {
     NIB_REQUIRE(kind >= 0, "attention (8-bit cache): %d/%d heads of %d are not supported", heads, kv_heads, head_dim);
     if (c.shares) {
         NIB_REQUIRE(c.ctas == 1 && c.shares > 0 && c.part_o && c.part_ml, "attention (8-bit cache): shares need scratch memory");
+        // (chunks are counted in 32 bits; of 32 keys at least)
+        NIB_REQUIRE(((long long)c.bt_width * page_size / GT + 1) * kv_heads * n_tokens < (1LL << 31), "attention (8-bit cache): too many keys for one launch");
     } else {
         NIB_REQUIRE(c.ctas == 1 || c.ctas == 2 || c.ctas == 4 || c.ctas == 8, "attention (8-bit cache): 1, 2, 4 or 8 CTAs share a row's keys, not %d", c.ctas);
     }

@@ -781,3 +781,15 @@ def test_portions_of_dense_rows_of_odd_width(ops, dtype):
         ops.attention_int8(wide, out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, 16, *b.pools, *b.pool_scales)
         # a decoded token whose rows lie off 4 bytes goes to another kernel, whose weights are not rounded to 16 bits
         assert (out[0].double() - want[0].double()).abs().max() <= 2.0 ** -6 * want[0].double().abs().max() and torch.equal(out[1:], want[1:])
+
+
+def test_more_keys_than_a_launch_counts_are_refused(ops):
+    """Chunks of all rows are counted in 32 bits: a table of 2^20 pages of 64 for each of 600 tokens may have more."""
+    from nanoinfer_b200.csrc.lib import KernelError
+    b = Batch(4, 2, 64, 0, 64, [1] * 600, [3] * 600, torch.bfloat16, seed=180)
+    table = torch.zeros(1, 1 << 20, dtype=torch.int32, device="cuda").expand(600, 1 << 20)
+    out, k = torch.empty(600, 256, dtype=torch.bfloat16, device="cuda"), ops.with_options(fixed_decode_splits=40)
+    with pytest.raises(KernelError, match="too many keys"):
+        k.attention_int8(b.qkv, out, 4, 2, 64, 0.125, 0, b.ctx, table, 64, *b.pools, *b.pool_scales)
+    k.attention_int8(b.qkv, out, 4, 2, 64, 0.125, 0, b.ctx, table[:, :1 << 16], 64, *b.pools, *b.pool_scales)
+    assert torch.isfinite(out).all()
