@@ -240,9 +240,11 @@ rotate_queries_kernel(const T* qkv, T* q_out, const AppendArgs a, long long item
 // search for the largest magnitude to their codes. (A warp for each of keys and values took 29 us for 4,096 tokens of 4 heads of 128,
 // waiting for one load after another.)
 // WIDE: chunks of 8 elements of queries and values and 4 of keys; 1 where widths or addresses do not allow it.
-// QUERIES: CTAs from kv_blocks on rotate a token's queries each (one launch for few tokens). Without, a kernel of its own rotates them
-// before: its threads hold 40 registers where these hold 125, which a portion's many queries need (2,048 and 1,741 tokens of 28 + 2 x 4 heads
-// of 128: 20.3 us, all in one launch 21.6 to 24.2).
+// QUERIES: CTAs from kv_blocks on rotate a token's queries each, one launch up to ONE_LAUNCH tokens. Without, a kernel of its own rotates them
+// before: its threads hold 40 registers where these hold 125, which many tokens' queries need. us, two launches / one, 16-bit rows in a chain, 300,
+// 1,000, 1,500, 2,048 and 4,096 tokens: 14 + 2 x 2 heads of 64 4.7 / 3.0, 5.0 / 3.3, 5.2 / 4.1, 5.5 / 5.3, 7.0 / 9.0; 12 + 2 x 2 of 128 5.9 / 4.3, 6.5 / 4.8, 7.1 / 5.3,
+// 7.7 / 6.6, 10.3 / 12.4; 28 + 2 x 4 of 128 6.1 / 4.9, 7.6 / 6.0, 9.2 / 8.9, 10.7 / 11.7, 21.8 / 24.5.
+constexpr int ONE_LAUNCH = 1536;
 template <typename T, int V> struct KeyRaw { float x1[V], x2[V], cs[V], sn[V]; int row, d; bool pair; };       // the second chunk only of a rotated pair
 template <int V> struct KeyItem { Two y1[V], y2[V]; int row, d; bool pair; };
 template <typename T, int V> struct ValueItem { float x[V]; int row, d; };
@@ -505,7 +507,7 @@ gather_int8_kernel(const signed char* k_pages, const signed char* v_pages, const
 template <typename T, bool WIDE>
 int launch_append(const void* qkv, void* q_out, const AppendArgs& a, cudaStream_t stream) {
     NIB_REQUIRE((long long)a.m + a.kv_blocks < (1LL << 31) - 1, "rope_store_int8: too many tokens for one launch");
-    if (a.m <= 64) {
+    if (a.m <= ONE_LAUNCH) {
         NIB_CUDA(launch_pdl(append_int8_kernel<T, WIDE, true>, dim3((unsigned)(a.m + a.kv_blocks)), dim3(KV_THREADS), (size_t)0, stream, (const T*)qkv, (T*)q_out, a));
         return 0;
     }

@@ -849,7 +849,7 @@ class Kernels:
             qkv.data_ptr(), q_out.data_ptr(), ctx.positions.data_ptr(), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), cos, sin, block_table.data_ptr(),
             k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), q_stride, out_stride[0], n_req, units, rows, rot,
             bt_stride, bt_width, page_size, pages, m, heads, kv_heads, head_dim, _DT[qkv.dtype], 0)
-        self.launches += 1 if m > 64 else 0         # (queries, and keys and values, each a kernel)
+        self.launches += 1 if m > 1536 else 0         # (ONE_LAUNCH: queries, and keys and values, each a kernel)
         self._check(self._lib.nib_rope_store_int8(args, self._stream()), "rope_store (8-bit cache)")
 
     def unpack_int8(self, pages, scales, out):

@@ -521,8 +521,10 @@ def test_rows_that_the_kernel_before_makes(ops, q_lens, before):
     start = [t.clone() for t in b.pools + b.pool_scales]
     q, out = (torch.empty(m, heads * d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
 
+    product = ops.with_options(tc_splits=1)          # (parts of K would add up as they come)
+
     def run(x, wait):
-        for step in (lambda: ops.linear(x, w, None, b.qkv, "store"), lambda: b.append(ops, q_out=q),
+        for step in (lambda: product.linear(x, w, None, b.qkv, "store"), lambda: b.append(ops, q_out=q),
                      lambda: ops.attention_int8(q, out, heads, kv, d, d ** -0.5, 0, b.ctx, b.table, 16, *b.pools, *b.pool_scales)):
             step()
             if wait:
@@ -793,3 +795,10 @@ def test_more_keys_than_a_launch_counts_are_refused(ops):
         k.attention_int8(b.qkv, out, 4, 2, 64, 0.125, 0, b.ctx, table, 64, *b.pools, *b.pool_scales)
     k.attention_int8(b.qkv, out, 4, 2, 64, 0.125, 0, b.ctx, table[:, :1 << 16], 64, *b.pools, *b.pool_scales)
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [64, 65, 1536, 1537])
+def test_queries_in_the_keys_launch_and_in_one_of_their_own(ops, m, dtype):
+    """On both sides of where the launches part."""
+    check_append(ops, Batch(6, 2, 64, 64, 16, [1, m - 1], [20, 37], dtype, seed=190))

@@ -171,7 +171,7 @@ def test_decoding_behind_prompts_of_hundreds_of_tokens(model_dirs, tmp_path, wei
     """Contexts of several chunks of the decode kernel, whose earlier pages are sent for while the append still runs: logits of replayed and
     of eager steps against the plain model with the same codes, with weights of 16 bits and of 4. Replayed and eager are equal where both cut
     the keys alike: by themselves they choose 8 CTAs a row for the 1,024 keys that a graph is captured for and 4 for 534, whose sums of
-    32 bits are of other terms. So the number is fixed."""
+    32 bits are of other terms. So the number is fixed; so is that of the prompt's products' parts of K, which add up as they come."""
     from nanoinfer_b200.config import KernelOptions
     from nanoinfer_b200.engine import StepEntry
     d, page = model_dirs["C"]
@@ -185,7 +185,7 @@ def test_decoding_behind_prompts_of_hundreds_of_tokens(model_dirs, tmp_path, wei
     want = [plain_rows(model, p + more[r::3], [len(p)] + [1] * steps, page)[len(p) - 1:] for r, p in enumerate(prompts)]
     runs = []
     for graphs in (True, False):
-        eng = engine(d, page, "bfloat16", num_pages=300, cache_dtype="int8", cuda_graphs=graphs, kernel_options=KernelOptions(fixed_decode_splits=4), **kw)
+        eng = engine(d, page, "bfloat16", num_pages=300, cache_dtype="int8", cuda_graphs=graphs, kernel_options=KernelOptions(fixed_decode_splits=4, tc_splits=1), **kw)
         rcs = [eng.open(i) for i in range(3)]
         rows = [eng.step([StepEntry(rc, p, [len(p) - 1]) for rc, p in zip(rcs, prompts)]).clone()]
         for t in range(steps):
@@ -208,7 +208,7 @@ def test_captured_portions_beside_decoded_tokens_follow_their_lengths(model_dirs
     long, prompt, more = tokens(700, model.cfg["vocab"], 11), tokens(450, model.cfg["vocab"], 12), tokens(15, model.cfg["vocab"], 13)
     runs = []
     for graphs in (True, False):
-        eng = engine(d, page, "bfloat16", num_pages=300, cache_dtype="int8", cuda_graphs=graphs, kernel_options=KernelOptions(fixed_decode_splits=4))
+        eng = engine(d, page, "bfloat16", num_pages=300, cache_dtype="int8", cuda_graphs=graphs, kernel_options=KernelOptions(fixed_decode_splits=4, tc_splits=1))
         if graphs:
             eng._portion_graphs.min_tokens, eng._portion_graphs.sightings = 16, 2
         a, b = eng.open("a"), eng.open("b")
