@@ -826,7 +826,8 @@ class Kernels:
         and kv head, a power of two; a value is code * scale. What a page held before the step's first token keeps its value up to
         the rounding to a larger scale, if a new token needs one; a page that the step begins anew forgets its old scale. A
         token whose key or value is not finite, or whose position the tables of ``rotary`` do not hold, makes its block's scale NaN.
-        No two requests may append to the same page."""
+        No two requests may append to the same page. Keys are rotated by their places in the request (``ctx.ctx_lens``), queries by
+        ``ctx.positions``; these, the tables and ``block_table`` are inputs of the step (see ``StepContext``)."""
         n_req, m, width, q_stride, pages, bt_width, bt_stride = self._cache_int8("rope_store_int8", qkv, kv_heads, page_size, head_dim, ctx, block_table,
                                                                                  k_pages, v_pages, k_scales, v_scales)
         device = qkv.get_device()

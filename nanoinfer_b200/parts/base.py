@@ -125,7 +125,9 @@ class HostBatch:
 class StepContext:
     """What every part sees of one step: the flat token batch and where each token belongs.
 
-    All device tensors are int32. Tokens of one request are contiguous and in position order.
+    All device tensors are int32. Tokens of one request are contiguous and in position order. Positions, lengths and block tables are
+    inputs of the step: kernels read them while the kernels before them may still run, so they come by copies (as the engine's do) and are
+    not what a kernel launched just before leaves.
     """
     num_tokens: int
     token_ids: torch.Tensor        # [M]
